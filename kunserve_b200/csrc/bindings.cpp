@@ -338,6 +338,8 @@ void fill_normal_op(torch::Tensor t, int64_t seed, double std) {
 
 }  // namespace
 
+void bind_cache_ops(py::module& m);   // cache_bindings.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "kunserve_b200 native library: sm_100a kernels and the Llama engine";
   py::class_<EngineShape>(m, "EngineShape")
@@ -443,6 +445,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("tp_reduce", &tp_reduce_op);
   m.def("raise_error_flag", &raise_error_flag, "host-side fault injection: set the device error flag");
   m.def("num_sms", &num_sms);
+  bind_cache_ops(m);
   m.attr("EPI_BF16") = (int)EPI_BF16;
   m.attr("EPI_F32") = (int)EPI_F32;
   m.attr("EPI_SILU") = (int)EPI_SILU;

@@ -9,6 +9,9 @@
 #include "attention_tc.cu"
 #include "attention_decode.cu"
 #include "init.cu"
+#include "rotary.cu"
+#include "attention_cached.cu"
+#include "evict.cu"
 
 namespace kus {
 void set_pdl(bool on) { pdl_flag() = on; }

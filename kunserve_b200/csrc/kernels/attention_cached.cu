@@ -1,0 +1,421 @@
+// Attention over planned work units: the parts of a batch whose requests
+// share prefixes, and single-token attention that keeps every key's weight.
+//
+//   out = softmax(scale q K^T) V over a query's keys, computed in parts: for
+//   a range R of keys, m = max s, l = sum exp(s - m), O = sum exp(s - m) v;
+//   parts join as M = max m, out = sum exp(m - M) O / sum exp(m - M) l.
+//
+// The keys of a shared prefix form ranges whose rows are the queries of all
+// the requests behind it, so each key is read once for up to 16 (row kernel)
+// or 128 rows (tile kernel, attention_prefix.cu).  A row without any key
+// gives zeros.  All statistics and partial sums are fp32.
+//
+// Row kernel: one warp per (unit, KV head), no barriers beyond the warp.
+// Stages of 16 keys (K and V rows, 16-byte cp.async, ends filled with zeros)
+// run through a ring in shared memory; S = Q K^T and O += P V are m16n8k16
+// tensor products with the unit's rows as M, so a key costs the same HBM
+// bytes for 1 to 16 rows: bound by HBM.
+#include "../common.cuh"
+#include "cache_ops.h"
+#include <cuda_fp16.h>
+
+namespace kus {
+namespace cat {
+
+constexpr int kWarps = 4;
+constexpr int kKeys = 16;       // keys per stage
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int HD>
+struct RowCfg {
+  static constexpr int kTile = kKeys * HD * 2;        // K or V of a stage
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kStages = HD == 128 ? 3 : 6;   // 24 KB a warp, two blocks of four warps an SM
+  static constexpr int kSmem = kWarps * kStages * kStage;
+};
+
+KUS_DEVICE void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+KUS_DEVICE void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+KUS_DEVICE void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+KUS_DEVICE void ldsm4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+KUS_DEVICE void ldsm4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+template <typename T>
+KUS_DEVICE void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+KUS_DEVICE void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+KUS_DEVICE void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Byte offset of 16-byte chunk `ch` of tile row `r` (rows of HD elements,
+// chunks exchanged within groups of 8 so that ldmatrix meets no bank twice).
+template <int HD>
+KUS_DEVICE uint32_t swz(int r, int ch) {
+  return (uint32_t)(r * HD * 2 + (((ch & ~7) | ((ch ^ r) & 7)) << 4));
+}
+
+// Rounded part and remainder of two values as packed 16-bit pairs: hi + lo
+// carries about 16 bits of P, so the product with V loses nothing that shows
+// in a 16-bit output.  The second product is free where HBM is the bound.
+template <typename T>
+KUS_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<T>(a, b);
+  const float2 r = Elem<T>::to_f2(*reinterpret_cast<typename Elem<T>::V2*>(&hi));
+  lo = pack2<T>(a - r.x, b - r.y);
+}
+
+template <typename T, int HD, bool SCORES>
+__global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float scale_log2) {
+  using Cf = RowCfg<HD>;
+  constexpr int kStages = Cf::kStages;
+  constexpr int kCh = HD / 8;              // 16-byte chunks of a row
+  constexpr int kRowsPer = 32 / kCh;       // rows that one load of the warp covers
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int kvh = a.g.kvh, G = a.nq / kvh;
+  pdl_wait();
+  pdl_trigger();
+  const int item = blockIdx.x * kWarps + warp;
+  if (item >= a.n_row_units * kvh) return;
+  const int u = item / kvh, kh = item - u * kvh;   // heads fastest: neighbours read the same cache rows
+  const int4 u0 = __ldg(reinterpret_cast<const int4*>(a.row_units) + 2 * u);
+  const int4 u1 = __ldg(reinterpret_cast<const int4*>(a.row_units) + 2 * u + 1);
+  const int tok0 = u0.x, ntok = u0.y & 255, ng = (u0.y >> 8) & 255, g0 = u0.y >> 16;
+  const int key_lo = u0.z, key_hi = u0.w, lim0 = u1.x;
+  const int* table = a.pages + u1.y;
+  const int rows = ntok * ng;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * Cf::kStage;
+  const int nst = (key_hi - key_lo + kKeys - 1) / kKeys;
+  const long long layer_elems = a.g.layer_stride / (int)sizeof(T);
+
+  // keys: lane l (and l + 16) looks up stage key l's page one stage ahead
+  auto page_of = [&](int i) {
+    const int key = key_lo + i * kKeys + (lane & 15);
+    return key < key_hi ? __ldg(table + kv_page_col(a.g, key)) : -1;
+  };
+  int page = page_of(0);
+  auto load = [&](int i) {
+    long long off = -1;
+    if (page >= 0) {
+      const int key = key_lo + i * kKeys + (lane & 15);
+      off = kv_slot(a.g, page, a.layer) * layer_elems + ((long long)kv_page_slot(a.g, key) * kvh + kh) * HD;
+    }
+    page = page_of(i + 1);
+    const uint32_t dst = ring + (i % kStages) * Cf::kStage;
+    const T* base = reinterpret_cast<const T*>(a.g.base);
+#pragma unroll
+    for (int p = 0; p < kKeys / kRowsPer; ++p) {
+      const int r = p * kRowsPer + lane / kCh, ch = lane % kCh;
+      const long long o = __shfl_sync(0xffffffffu, off, r);
+      // rows past the range read nothing and become zeros: stale cache
+      // contents (NaN included) never meet a zero weight
+      const int bytes = o >= 0 ? 16 : 0;
+      const T* src = base + (o >= 0 ? o + ch * 8 : 0);
+      cp_async16(dst + swz<HD>(r, ch), src, bytes);
+      cp_async16(dst + Cf::kTile + swz<HD>(r, ch), src + (o >= 0 ? layer_elems / 2 : 0), bytes);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (i < nst) load(i);
+    cp_commit();
+  }
+
+  // A fragments: rows lane / 4 and lane / 4 + 8 of the unit (zeros past its rows)
+  const int r_lo = lane >> 2;
+  uint32_t qf[HD / 16][4];
+  int lim[2];
+#pragma unroll
+  for (int hi = 0; hi < 2; ++hi) {
+    const int r = r_lo + 8 * hi;
+    const int j = r < rows ? r / ng : 0, gi = r < rows ? r - j * ng : 0;
+    lim[hi] = lim0 + j;
+    const T* qr = reinterpret_cast<const T*>(a.q) + (tok0 + j) * a.qt + (long long)(kh * G + g0 + gi) * a.qh +
+                  2 * (lane & 3);
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      qf[ks][hi] = r < rows ? *reinterpret_cast<const uint32_t*>(qr + ks * 16) : 0u;
+      qf[ks][2 + hi] = r < rows ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8) : 0u;
+    }
+  }
+  float o[HD / 8][4];
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float* srow = nullptr;
+  long long spitch = 0;
+  if (SCORES) {
+    // scores of the request: nq rows of its keys rounded up to a stage
+    spitch = (lim0 + kKeys - 1) / kKeys * kKeys;
+    srow = a.scores + (long long)u1.w * a.nq + (kh * G + g0) * spitch;
+  }
+
+  for (int i = 0; i < nst; ++i) {
+    if (i + kStages - 1 < nst) load(i + kStages - 1);
+    cp_commit();
+    cp_wait<kStages - 1>();
+    __syncwarp();
+    const uint32_t kt = ring + (i % kStages) * Cf::kStage, vt = kt + Cf::kTile;
+    float s[2][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      uint32_t b0, b1, b2, b3;
+      ldsm4(kt + swz<HD>(((lane >> 4) << 3) + (lane & 7), ks * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
+      mma<T>(s[0], qf[ks], b0, b1);
+      mma<T>(s[1], qf[ks], b2, b3);
+    }
+    const int key = key_lo + i * kKeys + 2 * (lane & 3);
+    uint32_t ph[4], pl[4];
+    float alpha[2];
+#pragma unroll
+    for (int hi = 0; hi < 2; ++hi) {
+      const int end = min(key_hi, lim[hi]);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& x = s[nt][2 * hi + e];
+          x = key + nt * 8 + e < end ? x * scale_log2 : -INFINITY;
+          mx = fmaxf(mx, x);
+        }
+      if (SCORES && r_lo + 8 * hi < rows) {
+        float* dst = srow + (r_lo + 8 * hi) * spitch + key;
+        *reinterpret_cast<float2*>(dst) = make_float2(s[0][2 * hi], s[0][2 * hi + 1]);
+        *reinterpret_cast<float2*>(dst + 8) = make_float2(s[1][2 * hi], s[1][2 * hi + 1]);
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[hi], mx);
+      const float ref = mn == -INFINITY ? 0.f : mn;   // no key seen yet
+      alpha[hi] = exp2f(m[hi] - ref);
+      m[hi] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const float p0 = exp2f(s[nt][2 * hi] - ref), p1 = exp2f(s[nt][2 * hi + 1] - ref);
+        sum += p0 + p1;
+        split2<T>(p0, p1, ph[2 * nt + hi], pl[2 * nt + hi]);
+      }
+      l[hi] = l[hi] * alpha[hi] + sum;
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 8; ++d) {
+      o[d][0] *= alpha[0];
+      o[d][1] *= alpha[0];
+      o[d][2] *= alpha[1];
+      o[d][3] *= alpha[1];
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) {
+      uint32_t b0, b1, b2, b3;
+      ldsm4_t(vt + swz<HD>((lane & 7) + (((lane >> 3) & 1) << 3), d * 2 + (lane >> 4)), b0, b1, b2, b3);
+      mma<T>(o[2 * d], ph, b0, b1);
+      mma<T>(o[2 * d + 1], ph, b2, b3);
+      mma<T>(o[2 * d], pl, b0, b1);
+      mma<T>(o[2 * d + 1], pl, b2, b3);
+    }
+    __syncwarp();   // the slot is refilled in the next iteration
+  }
+  cp_wait<0>();
+
+#pragma unroll
+  for (int hi = 0; hi < 2; ++hi) {
+    float sum = l[hi];
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    const int r = r_lo + 8 * hi;
+    if (r >= rows) continue;
+    const long long prow = u1.z + (long long)kh * rows + r;
+    float* dst = a.part_o + prow * HD + 2 * (lane & 3);
+#pragma unroll
+    for (int d = 0; d < HD / 8; ++d)
+      *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * hi], o[d][2 * hi + 1]);
+    if ((lane & 3) == 0) a.part_ml[prow] = make_float2(m[hi], sum);
+  }
+}
+
+// ------------------------------------------------------------------ joins
+// Parts of one (token, head): entry e's row for this head.
+KUS_DEVICE long long part_row(const CachedAttn& a, int e, int kh, int g) {
+  const int2 p = __ldg(a.merge + e);
+  return p.x + (long long)kh * p.y + g;
+}
+
+// Largest max and joint sum of parts [e0, e1) as the warp's lanes see them.
+KUS_DEVICE float2 join_stats(const CachedAttn& a, int e0, int e1, int kh, int g, int lane) {
+  float M = -INFINITY, L = 0.f;
+  for (int e = e0 + lane; e < e1; e += 32) {
+    const float2 ml = __ldcg(a.part_ml + part_row(a, e, kh, g));
+    const float n = fmaxf(M, ml.x);
+    if (n != -INFINITY) {
+      L = L * exp2f(M - n) + ml.y * exp2f(ml.x - n);
+      M = n;
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, M, off), l2 = __shfl_xor_sync(0xffffffffu, L, off);
+    const float n = fmaxf(M, m2);
+    if (n != -INFINITY) {
+      L = L * exp2f(M - n) + l2 * exp2f(m2 - n);
+      M = n;
+    }
+  }
+  return make_float2(M, L);
+}
+
+// Blocks [0, joins): W warps per (token, head) row join its parts.  Blocks
+// after them (weighted plans): one (chunk of keys, KV head) each, whose
+// weights exp(s - M) / L, summed over the group's heads, are added to the
+// cache's.  Each weight has one writer: no atomics.
+template <typename T, int HD, int W>
+__global__ void __launch_bounds__(128) join_kernel(CachedAttn a, unsigned joins) {
+  constexpr int kPer = HD / 32;   // dims a lane holds
+  constexpr int kRows = 4 / W;    // rows a block joins
+  __shared__ float sh_o[4][HD];
+  __shared__ float sh_m[128], sh_l[128];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int kvh = a.g.kvh, G = a.nq / kvh;
+  if (blockIdx.x < joins) {
+    const long long row = (long long)blockIdx.x * kRows + warp / W;
+    const bool have = row < (long long)a.T * a.nq;
+    const int t = have ? (int)(row / a.nq) : 0, h = have ? (int)(row - (long long)t * a.nq) : 0;
+    const int kh = h / G, g = h - kh * G;
+    const int list = t * a.head_chunks + g / kRowUnitRows;
+    const int e0 = a.merge_off[list], e1 = have ? a.merge_off[list + 1] : e0;
+    const float2 st = join_stats(a, e0, e1, kh, g, lane);
+    float acc[kPer] = {};
+    for (int b = e0 + 32 * (warp % W); b < e1; b += 32 * W) {
+      float w = 0.f;
+      long long prow = 0;
+      if (b + lane < e1) {
+        prow = part_row(a, b + lane, kh, g);
+        const float m = __ldcg(a.part_ml + prow).x;
+        w = m == -INFINITY ? 0.f : exp2f(m - st.x);
+      }
+      const int n = min(32, e1 - b);
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);
+        const long long ri = __shfl_sync(0xffffffffu, prow, i);
+        const float* src = a.part_o + ri * HD + lane * kPer;
+        if (kPer == 4) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+          acc[0] += wi * v.x;
+          acc[1] += wi * v.y;
+          acc[kPer - 2] += wi * v.z;
+          acc[kPer - 1] += wi * v.w;
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+          acc[0] += wi * v.x;
+          acc[1] += wi * v.y;
+        }
+      }
+    }
+    if (W > 1) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) sh_o[warp][lane * kPer + i] = acc[i];
+      __syncthreads();
+      if (warp % W) return;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        for (int j = 1; j < W; ++j) acc[i] += sh_o[warp + j][lane * kPer + i];
+    }
+    if (!have) return;
+    const float inv = st.y > 0.f ? 1.f / st.y : 0.f;
+    T* dst = reinterpret_cast<T*>(a.out) + t * a.ot + h * a.oh + lane * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; i += 2)
+      *reinterpret_cast<uint32_t*>(dst + i) = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
+    return;
+  }
+  const unsigned w = blockIdx.x - joins;
+  const int* c = a.chunks + (size_t)kChunkInts * (w / kvh);
+  const int kh = w % kvh;
+  const int t = c[0], key0 = c[1], key1 = c[2], first_page = c[3], len = c[4], col = c[5];
+  const long long pitch = (len + kKeys - 1) / kKeys * kKeys;
+  const float* srow = a.scores + (long long)col * a.nq + kh * G * pitch;
+  for (int g = warp; g < G; g += 4) {
+    const int list = t * a.head_chunks + g / kRowUnitRows;
+    const float2 st = join_stats(a, a.merge_off[list], a.merge_off[list + 1], kh, g, lane);
+    if (lane == 0) {
+      sh_m[g] = st.x;
+      sh_l[g] = 1.f / st.y;
+    }
+  }
+  __syncthreads();
+  for (int key = key0 + threadIdx.x; key < key1; key += 128) {
+    float x = 0.f;
+#pragma unroll 4
+    for (int g = 0; g < G; ++g) x += exp2f(__ldcg(srow + g * pitch + key) - sh_m[g]) * sh_l[g];
+    const int page = __ldg(a.pages + first_page + kv_page_col(a.g, key));
+    float* dst = a.weights + ((long long)page * kvh + kh) * a.g.block_size + kv_page_slot(a.g, key);
+    *dst += x;
+  }
+}
+
+template <typename T, int HD>
+void launch(const CachedAttn& a, cudaStream_t s) {
+  const float sl2 = a.scale * kLog2e;
+  if (a.n_row_units > 0) {
+    const dim3 grid((unsigned)(((long long)a.n_row_units * a.g.kvh + kWarps - 1) / kWarps));
+    constexpr int smem = RowCfg<HD>::kSmem;
+    if (a.scores) {
+      ensure_smem_attr(reinterpret_cast<const void*>(rows_kernel<T, HD, true>), smem);
+      launch_k(rows_kernel<T, HD, true>, grid, dim3(kWarps * 32), smem, s, a, sl2);
+    } else {
+      ensure_smem_attr(reinterpret_cast<const void*>(rows_kernel<T, HD, false>), smem);
+      launch_k(rows_kernel<T, HD, false>, grid, dim3(kWarps * 32), smem, s, a, sl2);
+    }
+  }
+  const long long rows = (long long)a.T * a.nq;
+  const unsigned extra = a.scores ? (unsigned)a.n_chunks * a.g.kvh : 0u;
+  // up to 32 parts a row fit one warp's lanes
+  if (a.most_parts <= 32)
+    launch_k(join_kernel<T, HD, 1>, dim3((unsigned)((rows + 3) / 4) + extra), dim3(128), 0, s, a,
+             (unsigned)((rows + 3) / 4));
+  else
+    launch_k(join_kernel<T, HD, 4>, dim3((unsigned)rows + extra), dim3(128), 0, s, a, (unsigned)rows);
+}
+
+}  // namespace cat
+
+void cached_attention(const CachedAttn& a, int type, cudaStream_t s) {
+  if (a.T <= 0) return;
+  if (type == kTypeBF16) {
+    a.hd == 128 ? cat::launch<__nv_bfloat16, 128>(a, s) : cat::launch<__nv_bfloat16, 64>(a, s);
+  } else {
+    a.hd == 128 ? cat::launch<__half, 128>(a, s) : cat::launch<__half, 64>(a, s);
+  }
+}
+
+}  // namespace kus

@@ -1,0 +1,205 @@
+// Rotary positions, fused with the append to the paged cache.
+//
+// Pair i of a head turns by the angle position * f_i:
+//   (a, b) -> m (a cos - b sin, b cos + a sin)
+// with (a, b) = dims (i, i + rot/2) of the half layout or (2i, 2i + 1) of the
+// interleaved one, for the first `rot` dims of a head; the rest pass through.
+// f_i is given in turns (f_i / 2 pi) as a 64-bit fraction, so position * f_i
+// modulo one turn is a 64-bit integer product: exact for every 32-bit
+// position, where position * f_i in fp32 is off by 2^-8 rad at 10^5.  sinpi
+// and cospi then take the remaining fraction in half turns.
+//
+// Bound by HBM: each element is read once and written once.  A block takes
+// one token (its cos and sin computed once, into shared memory, for all
+// heads); a thread turns 16 elements of a head as two 16-byte vectors.
+#include "../common.cuh"
+#include "cache_ops.h"
+#include <cuda_fp16.h>
+
+namespace kus {
+
+// 16-bit element types of the cache operators.
+template <typename T>
+struct Elem;
+template <>
+struct Elem<__nv_bfloat16> {
+  using V2 = __nv_bfloat162;
+  KUS_DEVICE static float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+  KUS_DEVICE static __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
+  KUS_DEVICE static float2 to_f2(V2 x) { return __bfloat1622float2(x); }
+  KUS_DEVICE static V2 from_f2(float a, float b) { return __floats2bfloat162_rn(a, b); }
+};
+template <>
+struct Elem<__half> {
+  using V2 = __half2;
+  KUS_DEVICE static float to_f(__half x) { return __half2float(x); }
+  KUS_DEVICE static __half from_f(float x) { return __float2half_rn(x); }
+  KUS_DEVICE static float2 to_f2(V2 x) { return __half22float2(x); }
+  KUS_DEVICE static V2 from_f2(float a, float b) { return __floats2half2_rn(a, b); }
+};
+
+template <typename T>
+KUS_DEVICE void unpack8(const uint4& u, float (&f)[8]) {
+  const typename Elem<T>::V2* h = reinterpret_cast<const typename Elem<T>::V2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = Elem<T>::to_f2(h[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+template <typename T>
+KUS_DEVICE uint32_t pack2(float a, float b) {
+  typename Elem<T>::V2 v = Elem<T>::from_f2(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <typename T>
+KUS_DEVICE uint4 pack8(const float (&f)[8]) {
+  return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+}
+
+namespace rot {
+
+constexpr int kThreads = 256;
+
+// VEC: 16-byte vectors (bases and strides of 16 bytes, hd and rot multiples
+// of 16, interleaved rot of 8); otherwise single elements, one pair or one
+// unrotated element a thread.
+template <typename T, bool INTER, bool VEC>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
+  extern __shared__ float2 cs[];   // (cos, sin) of the token's rot / 2 pairs
+  pdl_wait();
+  pdl_trigger();
+  const int t = blockIdx.x;
+  const long long pos = a.positions[t];
+  const int half = a.rot / 2;
+  for (int i = threadIdx.x; i < half; i += kThreads) {
+    const unsigned long long turn = (unsigned long long)pos * a.steps[i];
+    float s, c;
+    sincospif((float)(long long)turn * 0x1p-63f, &s, &c);
+    cs[i] = make_float2(c * a.scale, s * a.scale * a.sign);
+  }
+  const int heads = a.nq + 2 * a.nkv;
+  T* krow = nullptr;   // the token's cache row, KV head 0
+  T* vrow = nullptr;
+  if (a.nkv) {
+    // a bad row would corrupt the cache: recorded, its keys and values dropped
+    const int page = a.pages[t], slot = a.slots[t];
+    if (page < 0 || page >= a.g.pages_total || slot < 0 || slot >= a.g.block_size) {
+      if (threadIdx.x == 0 && blockIdx.y == 0) set_error(kErrBounds, page);
+    } else {
+      const long long off = (long long)slot * a.g.kvh * a.g.hd * (int)sizeof(T);
+      krow = reinterpret_cast<T*>(a.g.base + kv_offset(a.g, page, a.layer, false) + off);
+      vrow = reinterpret_cast<T*>(a.g.base + kv_offset(a.g, page, a.layer, true) + off);
+      if (a.weights && blockIdx.y == 0)
+        for (int h = threadIdx.x; h < a.nkv; h += kThreads) {
+          const long long i = ((long long)page * a.nkv + h) * a.g.block_size + slot;
+          a.weights[i] = 0.f;
+          a.slot_positions[i] = (int)pos;
+        }
+    }
+  }
+  __syncthreads();
+  const T* xrow = reinterpret_cast<const T*>(a.x) + t * a.xt;
+  T* orow = reinterpret_cast<T*>(a.out) + t * a.ot;
+  // head h's destination; null: not written
+  auto dest = [&](int h) -> T* {
+    if (h < a.nq) return orow + h * a.oh;
+    if (!krow) return nullptr;
+    return h < a.nq + a.nkv ? krow + (long long)(h - a.nq) * a.hd : vrow + (long long)(h - a.nq - a.nkv) * a.hd;
+  };
+  if (VEC) {
+    const int per = a.hd / 16, items = heads * per, turned = a.rot / 16;
+    for (int u = blockIdx.y * kThreads + threadIdx.x; u < items; u += gridDim.y * kThreads) {
+      const int h = u / per, j = u - h * per;
+      T* dst = dest(h);
+      if (!dst) continue;
+      const T* src = xrow + h * a.xh;
+      const bool turn = h < a.nq + a.nkv && j < turned;
+      // the two vectors' dims: pairs (i, i + rot/2) when turned in the half
+      // layout, else neighbours
+      const int d0 = (!INTER && turn) ? 8 * j : 16 * j;
+      const int d1 = (!INTER && turn) ? d0 + half : d0 + 8;
+      uint4 v0 = *reinterpret_cast<const uint4*>(src + d0);
+      uint4 v1 = *reinterpret_cast<const uint4*>(src + d1);
+      if (turn) {
+        float x0[8], x1[8];
+        unpack8<T>(v0, x0);
+        unpack8<T>(v1, x1);
+        if (INTER) {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float2 p = cs[d0 / 2 + e / 2], r = cs[d1 / 2 + e / 2];
+            const float a0 = x0[e], a1 = x1[e];
+            x0[e] = a0 * p.x - x0[e + 1] * p.y;
+            x0[e + 1] = x0[e + 1] * p.x + a0 * p.y;
+            x1[e] = a1 * r.x - x1[e + 1] * r.y;
+            x1[e + 1] = x1[e + 1] * r.x + a1 * r.y;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 p = cs[d0 + e];
+            const float a0 = x0[e];
+            x0[e] = a0 * p.x - x1[e] * p.y;
+            x1[e] = x1[e] * p.x + a0 * p.y;
+          }
+        }
+        v0 = pack8<T>(x0);
+        v1 = pack8<T>(x1);
+      }
+      *reinterpret_cast<uint4*>(dst + d0) = v0;
+      *reinterpret_cast<uint4*>(dst + d1) = v1;
+    }
+  } else {
+    const int per = half + (a.hd - a.rot), items = heads * a.hd;
+    for (int u = blockIdx.y * kThreads + threadIdx.x; u < items; u += gridDim.y * kThreads) {
+      const int h = u / a.hd, j = u - h * a.hd;
+      T* dst = dest(h);
+      if (!dst) continue;
+      const T* src = xrow + h * a.xh;
+      if (h >= a.nq + a.nkv) {
+        dst[j] = src[j];
+      } else if (j < half) {
+        const int d0 = INTER ? 2 * j : j, d1 = INTER ? 2 * j + 1 : j + half;
+        const float x0 = Elem<T>::to_f(src[d0]), x1 = Elem<T>::to_f(src[d1]);
+        const float2 p = cs[j];
+        dst[d0] = Elem<T>::from_f(x0 * p.x - x1 * p.y);
+        dst[d1] = Elem<T>::from_f(x1 * p.x + x0 * p.y);
+      } else if (j < per) {
+        dst[j + half] = src[j + half];
+      }
+    }
+  }
+}
+
+template <typename T, bool INTER>
+void launch(const RotaryArgs& a, cudaStream_t s) {
+  auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  const bool vec = al(a.x) && al(a.out) && (a.nkv == 0 || al(a.g.base)) && a.xt % 8 == 0 && a.xh % 8 == 0 &&
+                   a.ot % 8 == 0 && a.oh % 8 == 0 && a.hd % 16 == 0 && a.rot % 16 == 0;
+  const int items = (a.nq + 2 * a.nkv) * (vec ? a.hd / 16 : a.hd);
+  // few tokens: several blocks a token, each with the heads' share, so that
+  // one token's heads are all in flight at once
+  const int per_token = (items + kThreads - 1) / kThreads;
+  const int split = a.T >= 2 * 148 ? 1 : per_token;
+  const dim3 grid(a.T, split);
+  const size_t smem = (size_t)a.rot / 2 * sizeof(float2);
+  if (vec)
+    launch_k(rotary_kernel<T, INTER, true>, grid, dim3(kThreads), smem, s, a);
+  else
+    launch_k(rotary_kernel<T, INTER, false>, grid, dim3(kThreads), smem, s, a);
+}
+
+}  // namespace rot
+
+void rotary(const RotaryArgs& a, int type, cudaStream_t s) {
+  if (a.T <= 0) return;
+  if (type == kTypeBF16) {
+    a.interleaved ? rot::launch<__nv_bfloat16, true>(a, s) : rot::launch<__nv_bfloat16, false>(a, s);
+  } else {
+    a.interleaved ? rot::launch<__half, true>(a, s) : rot::launch<__half, false>(a, s);
+  }
+}
+
+}  // namespace kus

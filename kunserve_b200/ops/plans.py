@@ -1,0 +1,138 @@
+"""Work units of the cached-attention kernels for one batch (host side).
+
+A plan is made once per step and serves every layer.  It cuts each set of
+query rows (the tokens behind a shared prefix, or one request's tokens) into
+row tiles, and the keys they see into ranges, so that the units spread over
+the GPU whatever the mix of lengths; and it lists for every (token, head)
+which partial rows to join.  ``csrc/kernels/cache_ops.h`` describes the
+records; everything the kernels index with is checked here.
+"""
+from typing import Dict, List, NamedTuple, Sequence, Tuple
+
+import numpy as np
+
+UNIT_INTS = 8
+ROW_UNIT_ROWS = 16
+STAGE_KEYS = 16          # keys per stage of the row kernel
+CHUNK_KEYS = 512         # keys per block that adds up weights
+NO_LIMIT = 1 << 30
+ROW_SLOTS = 8            # warps of the row kernel an SM holds
+ROW_MIN_STAGES = 4       # shortest range of a row unit, in stages
+
+
+class Span(NamedTuple):
+    """Query rows of consecutive tokens over one page list: ``limit`` keys are
+    visible to the first token and one more to each further one, never more
+    than ``keys``."""
+    token: int
+    tokens: int
+    keys: int
+    limit: int
+    page: int            # first entry of the page list
+
+
+def _row_tiles(spans: Sequence[Span], group: int, rows: int) -> np.ndarray:
+    """Tiles of at most ``rows`` rows: columns token, tokens, heads, first
+    head, visible keys, limit, page list, span."""
+    out: List[Tuple[int, ...]] = []
+    step = max(1, rows // group)
+    for i, s in enumerate(spans):
+        for j in range(0, s.tokens, step):
+            n = min(step, s.tokens - j)
+            keys = min(s.keys, s.limit + j + n - 1)
+            if keys <= 0:
+                continue
+            for g in range(0, group, rows):
+                out.append((s.token + j, n, min(rows, group - g), g, keys, min(s.limit + j, NO_LIMIT), s.page, i))
+    return np.array(out, dtype=np.int64).reshape(-1, 8)
+
+
+def _cut(tiles: np.ndarray, kv_heads: int, slots: int, stage: int, min_stages: int) -> np.ndarray:
+    """Cut the tiles' keys into ranges of about one slot's share of all
+    stages: columns of the tile, then first key and end of the range."""
+    stages = -(-tiles[:, 4] // stage)
+    share = max(min_stages, -(-int(stages.sum()) * kv_heads // slots))
+    parts = np.maximum(1, stages // share)
+    each = -(-stages // parts)
+    parts = -(-stages // each)                       # no empty range at the end
+    idx = np.repeat(np.arange(len(tiles)), parts)
+    k = np.arange(len(idx)) - np.repeat(np.cumsum(parts) - parts, parts)
+    lo = k * each[idx] * stage
+    hi = np.minimum(lo + each[idx] * stage, tiles[idx, 4])
+    return np.concatenate([tiles[idx], lo[:, None], hi[:, None]], axis=1)
+
+
+def build(row_spans: Sequence[Span], pages: np.ndarray, tokens: int, num_q_heads: int, kv_heads: int, sms: int,
+          score_cols: Sequence[int] = ()) -> Tuple[np.ndarray, Dict[str, int]]:
+    """The int32 blob of a plan and its section table.  ``score_cols``: first
+    score column of each span (weighted plans)."""
+    if num_q_heads % kv_heads:
+        raise ValueError(f"{num_q_heads} query heads are no multiple of {kv_heads} KV heads")
+    group = num_q_heads // kv_heads
+    if group > 128:
+        raise ValueError(f"at most 128 query heads per KV head, got {group}")
+    rows = _cut(_row_tiles(row_spans, group, ROW_UNIT_ROWS), kv_heads, sms * ROW_SLOTS, STAGE_KEYS, ROW_MIN_STAGES)
+    head_chunks = -(-group // ROW_UNIT_ROWS)
+
+    units = rows
+    n_rows = units[:, 1] * units[:, 2]
+    part = np.cumsum(n_rows * kv_heads) - n_rows * kv_heads
+    rec = np.zeros((len(units), UNIT_INTS), dtype=np.int64)
+    rec[:, 0] = units[:, 0]
+    rec[:, 1] = units[:, 1] | units[:, 2] << 8 | units[:, 3] << 16
+    rec[:, 2:4] = units[:, 8:10]
+    rec[:, 4] = units[:, 5]
+    rec[:, 5] = units[:, 6]
+    rec[:, 6] = part
+    if len(score_cols):
+        rec[:, 7] = np.asarray(score_cols, dtype=np.int64)[units[:, 7]]
+    part_rows = int((n_rows * kv_heads).sum())
+
+    # the partial rows of each (token, chunk of 16 group heads)
+    idx = np.repeat(np.arange(len(units)), units[:, 1])
+    j = np.arange(len(idx)) - np.repeat(np.cumsum(units[:, 1]) - units[:, 1], units[:, 1])
+    key = (units[idx, 0] + j) * head_chunks + units[idx, 3] // ROW_UNIT_ROWS
+    order = np.argsort(key, kind="stable")
+    entries = np.stack([part[idx] + j * units[idx, 2] - units[idx, 3], n_rows[idx]], axis=1)[order]
+    counts = np.bincount(key, minlength=tokens * head_chunks)
+    off = np.concatenate([[0], np.cumsum(counts)])
+    if part_rows >= 1 << 31:
+        raise ValueError("the batch needs too many partial rows")
+
+    table = dict(tokens=tokens, num_q_heads=num_q_heads, row_units=len(rows), tile_units=0, head_chunks=head_chunks,
+                 most_parts=int(counts.max()) if counts.size else 0, part_rows=part_rows,
+                 max_page=int(pages.max()) if pages.size else -1, chunks=0, requests=0, most_tokens=0, score_cols=0)
+    return _pack(table, row_units=rec, tile_units=rec[len(rows):], merge=entries, merge_off=off, pages=pages)
+
+
+def _pack(table: Dict[str, int], **sections: np.ndarray) -> Tuple[np.ndarray, Dict[str, int]]:
+    """Lay the sections out on 16-byte boundaries; ``table`` gains ``at_<name>``."""
+    at, chunks = 0, []
+    for name, a in sections.items():
+        a = np.ascontiguousarray(a, dtype=np.int32).reshape(-1)
+        table["at_" + name] = at
+        chunks += [a, np.zeros(-a.size % 4, dtype=np.int32)]
+        at += a.size + (-a.size % 4)
+    return np.concatenate(chunks) if chunks else np.zeros(0, np.int32), table
+
+
+def append_sections(blob: np.ndarray, table: Dict[str, int], **sections: np.ndarray) -> np.ndarray:
+    """More sections behind those of ``blob``."""
+    more, t = _pack({}, **sections)
+    table.update({k: v + blob.size for k, v in t.items()})
+    return np.concatenate([blob, more])
+
+
+def check_pages(pages: Sequence[int], tokens: int, block_size: int, pages_total: int, what: str) -> List[int]:
+    """The pages that hold ``tokens`` tokens, checked against the cache."""
+    if tokens < 0:
+        raise ValueError(f"{what}: {tokens} tokens")
+    if tokens >= NO_LIMIT:
+        raise ValueError(f"{what}: {tokens} tokens are too many")
+    need = -(-tokens // block_size)
+    pages = list(pages)[:need]
+    if len(pages) < need:
+        raise ValueError(f"{what}: {tokens} tokens need {need} pages of {block_size}, got {len(pages)}")
+    if pages and (min(pages) < 0 or max(pages) >= pages_total):
+        raise ValueError(f"{what}: page ids must lie in [0, {pages_total}), got {min(pages)} to {max(pages)}")
+    return pages

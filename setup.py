@@ -31,7 +31,7 @@ def ext_modules():
             "--expt-relaxed-constexpr", "-Xptxas=-v" if os.environ.get("KUS_PTXAS_VERBOSE") else "-DKUS_QUIET"]
     ext = CUDAExtension(
         name="kunserve_b200._C",
-        sources=[os.path.join(CSRC, "bindings.cpp"), os.path.join(CSRC, "engine", "engine.cpp"),
+        sources=[os.path.join(CSRC, "bindings.cpp"), os.path.join(CSRC, "cache_bindings.cpp"), os.path.join(CSRC, "engine", "engine.cpp"),
                  os.path.join(CSRC, "engine", "arena.cpp"), os.path.join(CSRC, "kernels", "all.cu")],
         include_dirs=[os.path.join(ROOT, CSRC), inc],
         library_dirs=[lib],
