@@ -43,6 +43,8 @@ struct PagedKV {
   torch::Tensor pool;
   KVGeom g{};
   int type;
+  CUtensorMap map;
+  bool tiles;   // the tile kernel can read this pool (map is valid)
 
   PagedKV(torch::Tensor p, int64_t P, int64_t N, int64_t Ls, int64_t L, int64_t block_size, int64_t kvh, int64_t hd)
       : pool(std::move(p)) {
@@ -65,6 +67,8 @@ struct PagedKV {
     g.kvh = (int)kvh;
     g.hd = (int)hd;
     finish_geom(g, bytes - P * g.page_stride);
+    c10::cuda::CUDAGuard guard(pool.device());
+    tiles = make_cache_tile_map(&map, g, bytes, type);
   }
 
   int checked_layer(int64_t layer) const {
@@ -137,6 +141,7 @@ struct CachePlan {
   const int* ints(int64_t at) const { return blob.data_ptr<int>() + at; }
   // The plan fits this cache, and outlives the work queued on the current stream.
   void use(const PagedKV& kv) const {
+    KUS_CHECK(n_tile_units == 0 || kv.tiles, "the plan was made for a cache of another shape");
     KUS_CHECK(kv.g.kvh == kvh && kv.g.block_size == block_size && kv.g.hd == hd && max_page < kv.g.pages_total &&
                     kv.pool.device() == blob.device(),
                 "the plan was made for a cache of another shape");
@@ -283,7 +288,7 @@ torch::Tensor cached_attention_op(const torch::Tensor& q, const PagedKV& kv, int
     a.chunks = plan.ints(plan.o_chunks);
     a.n_chunks = plan.n_chunks;
   }
-  cached_attention(a, kv.type, at::cuda::getCurrentCUDAStream());
+  cached_attention(a, &kv.map, kv.type, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return o;
 }
@@ -362,6 +367,7 @@ void bind_cache_ops(py::module& m) {
       .def_property_readonly("block_size", [](const PagedKV& k) { return k.g.block_size; })
       .def_property_readonly("num_kv_heads", [](const PagedKV& k) { return k.g.kvh; })
       .def_property_readonly("head_dim", [](const PagedKV& k) { return k.g.hd; })
+      .def_property_readonly("tiles", [](const PagedKV& k) { return k.tiles; })
       .def_property_readonly("pool", [](const PagedKV& k) { return k.pool; });
   py::class_<CachePlan>(m, "CachePlan")
       .def(py::init<const torch::Tensor&, const PagedKV&, const std::map<std::string, int64_t>&>());

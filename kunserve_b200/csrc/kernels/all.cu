@@ -10,6 +10,7 @@
 #include "attention_decode.cu"
 #include "init.cu"
 #include "rotary.cu"
+#include "attention_prefix.cu"
 #include "attention_cached.cu"
 #include "evict.cu"
 

@@ -16,8 +16,8 @@
 // tensor products with the unit's rows as M, so a key costs the same HBM
 // bytes for 1 to 16 rows: bound by HBM.
 #include "../common.cuh"
+#include "cache_elem.cuh"
 #include "cache_ops.h"
-#include <cuda_fp16.h>
 
 namespace kus {
 namespace cat {
@@ -90,8 +90,11 @@ KUS_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   lo = pack2<T>(a - r.x, b - r.y);
 }
 
+// `second`: launched behind the tile kernel of the same call, whose results it
+// does not need: it starts beside it, and only ends after it, so that the join
+// (which waits for this kernel) finds both done.
 template <typename T, int HD, bool SCORES>
-__global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float scale_log2) {
+__global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float scale_log2, bool second) {
   using Cf = RowCfg<HD>;
   constexpr int kStages = Cf::kStages;
   constexpr int kCh = HD / 8;              // 16-byte chunks of a row
@@ -99,10 +102,13 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float s
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int kvh = a.g.kvh, G = a.nq / kvh;
-  pdl_wait();
+  if (!second) pdl_wait();
   pdl_trigger();
   const int item = blockIdx.x * kWarps + warp;
-  if (item >= a.n_row_units * kvh) return;
+  if (item >= a.n_row_units * kvh) {
+    if (second) pdl_wait();
+    return;
+  }
   const int u = item / kvh, kh = item - u * kvh;   // heads fastest: neighbours read the same cache rows
   const int4 u0 = __ldg(reinterpret_cast<const int4*>(a.row_units) + 2 * u);
   const int4 u1 = __ldg(reinterpret_cast<const int4*>(a.row_units) + 2 * u + 1);
@@ -214,12 +220,12 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float s
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float mn = fmaxf(m[hi], mx);
       const float ref = mn == -INFINITY ? 0.f : mn;   // no key seen yet
-      alpha[hi] = exp2f(m[hi] - ref);
+      alpha[hi] = ex2(m[hi] - ref);
       m[hi] = mn;
       float sum = 0.f;
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
-        const float p0 = exp2f(s[nt][2 * hi] - ref), p1 = exp2f(s[nt][2 * hi + 1] - ref);
+        const float p0 = ex2(s[nt][2 * hi] - ref), p1 = ex2(s[nt][2 * hi + 1] - ref);
         sum += p0 + p1;
         split2<T>(p0, p1, ph[2 * nt + hi], pl[2 * nt + hi]);
       }
@@ -259,6 +265,7 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float s
       *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * hi], o[d][2 * hi + 1]);
     if ((lane & 3) == 0) a.part_ml[prow] = make_float2(m[hi], sum);
   }
+  if (second) pdl_wait();
 }
 
 // ------------------------------------------------------------------ joins
@@ -275,7 +282,7 @@ KUS_DEVICE float2 join_stats(const CachedAttn& a, int e0, int e1, int kh, int g,
     const float2 ml = __ldcg(a.part_ml + part_row(a, e, kh, g));
     const float n = fmaxf(M, ml.x);
     if (n != -INFINITY) {
-      L = L * exp2f(M - n) + ml.y * exp2f(ml.x - n);
+      L = L * ex2(M - n) + ml.y * ex2(ml.x - n);
       M = n;
     }
   }
@@ -284,7 +291,7 @@ KUS_DEVICE float2 join_stats(const CachedAttn& a, int e0, int e1, int kh, int g,
     const float m2 = __shfl_xor_sync(0xffffffffu, M, off), l2 = __shfl_xor_sync(0xffffffffu, L, off);
     const float n = fmaxf(M, m2);
     if (n != -INFINITY) {
-      L = L * exp2f(M - n) + l2 * exp2f(m2 - n);
+      L = L * ex2(M - n) + l2 * ex2(m2 - n);
       M = n;
     }
   }
@@ -320,7 +327,7 @@ __global__ void __launch_bounds__(128) join_kernel(CachedAttn a, unsigned joins)
       if (b + lane < e1) {
         prow = part_row(a, b + lane, kh, g);
         const float m = __ldcg(a.part_ml + prow).x;
-        w = m == -INFINITY ? 0.f : exp2f(m - st.x);
+        w = m == -INFINITY ? 0.f : ex2(m - st.x);
       }
       const int n = min(32, e1 - b);
 #pragma unroll 8
@@ -328,16 +335,17 @@ __global__ void __launch_bounds__(128) join_kernel(CachedAttn a, unsigned joins)
         const float wi = __shfl_sync(0xffffffffu, w, i);
         const long long ri = __shfl_sync(0xffffffffu, prow, i);
         const float* src = a.part_o + ri * HD + lane * kPer;
+        // a part without keys has weight 0, whatever its sums hold
         if (kPer == 4) {
           const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-          acc[0] += wi * v.x;
-          acc[1] += wi * v.y;
-          acc[kPer - 2] += wi * v.z;
-          acc[kPer - 1] += wi * v.w;
+          acc[0] += wi != 0.f ? wi * v.x : 0.f;
+          acc[1] += wi != 0.f ? wi * v.y : 0.f;
+          acc[kPer - 2] += wi != 0.f ? wi * v.z : 0.f;
+          acc[kPer - 1] += wi != 0.f ? wi * v.w : 0.f;
         } else {
           const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-          acc[0] += wi * v.x;
-          acc[1] += wi * v.y;
+          acc[0] += wi != 0.f ? wi * v.x : 0.f;
+          acc[1] += wi != 0.f ? wi * v.y : 0.f;
         }
       }
     }
@@ -376,45 +384,60 @@ __global__ void __launch_bounds__(128) join_kernel(CachedAttn a, unsigned joins)
   for (int key = key0 + threadIdx.x; key < key1; key += 128) {
     float x = 0.f;
 #pragma unroll 4
-    for (int g = 0; g < G; ++g) x += exp2f(__ldcg(srow + g * pitch + key) - sh_m[g]) * sh_l[g];
+    for (int g = 0; g < G; ++g) x += ex2(__ldcg(srow + g * pitch + key) - sh_m[g]) * sh_l[g];
     const int page = __ldg(a.pages + first_page + kv_page_col(a.g, key));
     float* dst = a.weights + ((long long)page * kvh + kh) * a.g.block_size + kv_page_slot(a.g, key);
     *dst += x;
   }
 }
 
+// Launch whose grid may start while the previous one of the stream ends.
+template <typename... KArgs, typename... Args>
+void launch_behind(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, Args... args) {
+  bool& pdl = pdl_flag();
+  const bool was = pdl;
+  pdl = true;
+  launch_k(kern, dim3(grid), dim3(block), smem, s, args...);
+  pdl = was;
+}
+
+template <typename T, int HD, bool SCORES>
+void launch_rows(const CachedAttn& a, bool second, cudaStream_t s) {
+  constexpr int smem = RowCfg<HD>::kSmem;
+  ensure_smem_attr(reinterpret_cast<const void*>(rows_kernel<T, HD, SCORES>), smem);
+  const unsigned grid = (unsigned)(((long long)a.n_row_units * a.g.kvh + kWarps - 1) / kWarps);
+  if (second)
+    launch_behind(rows_kernel<T, HD, SCORES>, grid, kWarps * 32, smem, s, a, a.scale * kLog2e, true);
+  else
+    launch_k(rows_kernel<T, HD, SCORES>, dim3(grid), dim3(kWarps * 32), smem, s, a, a.scale * kLog2e, false);
+}
+
 template <typename T, int HD>
-void launch(const CachedAttn& a, cudaStream_t s) {
-  const float sl2 = a.scale * kLog2e;
-  if (a.n_row_units > 0) {
-    const dim3 grid((unsigned)(((long long)a.n_row_units * a.g.kvh + kWarps - 1) / kWarps));
-    constexpr int smem = RowCfg<HD>::kSmem;
-    if (a.scores) {
-      ensure_smem_attr(reinterpret_cast<const void*>(rows_kernel<T, HD, true>), smem);
-      launch_k(rows_kernel<T, HD, true>, grid, dim3(kWarps * 32), smem, s, a, sl2);
-    } else {
-      ensure_smem_attr(reinterpret_cast<const void*>(rows_kernel<T, HD, false>), smem);
-      launch_k(rows_kernel<T, HD, false>, grid, dim3(kWarps * 32), smem, s, a, sl2);
-    }
-  }
+void launch(const CachedAttn& a, const CUtensorMap* map, int type, cudaStream_t s) {
+  const bool tiles = a.n_tile_units > 0;
+  if (tiles) cached_attention_tiles(a, *map, type, s);
+  if (a.n_row_units > 0) a.scores ? launch_rows<T, HD, true>(a, tiles, s) : launch_rows<T, HD, false>(a, tiles, s);
   const long long rows = (long long)a.T * a.nq;
   const unsigned extra = a.scores ? (unsigned)a.n_chunks * a.g.kvh : 0u;
   // up to 32 parts a row fit one warp's lanes
-  if (a.most_parts <= 32)
-    launch_k(join_kernel<T, HD, 1>, dim3((unsigned)((rows + 3) / 4) + extra), dim3(128), 0, s, a,
-             (unsigned)((rows + 3) / 4));
+  const bool wide = a.most_parts > 32;
+  const unsigned joins = (unsigned)(wide ? rows : (rows + 3) / 4);
+  if (!tiles && a.n_row_units == 0)   // nothing before it: zeros only
+    launch_k(join_kernel<T, HD, 1>, dim3(joins + extra), dim3(128), 0, s, a, joins);
+  else if (wide)
+    launch_behind(join_kernel<T, HD, 4>, joins + extra, 128, 0, s, a, joins);
   else
-    launch_k(join_kernel<T, HD, 4>, dim3((unsigned)rows + extra), dim3(128), 0, s, a, (unsigned)rows);
+    launch_behind(join_kernel<T, HD, 1>, joins + extra, 128, 0, s, a, joins);
 }
 
 }  // namespace cat
 
-void cached_attention(const CachedAttn& a, int type, cudaStream_t s) {
+void cached_attention(const CachedAttn& a, const CUtensorMap* map, int type, cudaStream_t s) {
   if (a.T <= 0) return;
   if (type == kTypeBF16) {
-    a.hd == 128 ? cat::launch<__nv_bfloat16, 128>(a, s) : cat::launch<__nv_bfloat16, 64>(a, s);
+    a.hd == 128 ? cat::launch<__nv_bfloat16, 128>(a, map, type, s) : cat::launch<__nv_bfloat16, 64>(a, map, type, s);
   } else {
-    a.hd == 128 ? cat::launch<__half, 128>(a, s) : cat::launch<__half, 64>(a, s);
+    a.hd == 128 ? cat::launch<__half, 128>(a, map, type, s) : cat::launch<__half, 64>(a, map, type, s);
   }
 }
 

@@ -82,7 +82,16 @@ struct CachedAttn {
   const int* chunks;             // [n_chunks, kChunkInts]
   int n_chunks;
 };
-void cached_attention(const CachedAttn& a, int type, cudaStream_t s);
+// The call: the tile kernel over the tile units, the row kernel over the row
+// units, the join of their parts.  `map`: of make_cache_tile_map, needed with
+// tile units only.
+void cached_attention(const CachedAttn& a, const CUtensorMap* map, int type, cudaStream_t s);
+void cached_attention_tiles(const CachedAttn& a, const CUtensorMap& map, int type, cudaStream_t s);
+// Keys per TMA box of the tile kernel (a power of two that divides the page)
+// and the tensor map of a pool of `bytes`; false where the tile kernel cannot
+// read the pool: pages that are no multiple of 8 slots, other head sizes.
+int cache_tile_box(const KVGeom& g);
+bool make_cache_tile_map(CUtensorMap* map, const KVGeom& g, long long bytes, int type);
 
 // ---------------------------------------------------------------- eviction
 // Ints of a request: tokens, first page, newest position, 0.

@@ -65,7 +65,7 @@ class SharedPrefixPlan:
             prefix.append(plans.Span(first, t - first, g.length, plans.NO_LIMIT, at))
         self.tokens, self.num_q_heads = t, int(num_q_heads)
         blob, table = plans.build(prefix + own, np.array(pages, dtype=np.int64), t, self.num_q_heads,
-                                  kv.num_kv_heads, _sms(kv.pool.device.index))
+                                  kv.num_kv_heads, _sms(kv.pool.device.index), tiles=kv.tiles)
         blob = plans.append_sections(blob, table, chunks=np.zeros(0), requests=np.zeros(0))
         self._native = native().CachePlan(torch.from_numpy(blob), kv, table)
 
@@ -111,7 +111,7 @@ class DecodePlan:
         self.lengths: List[int] = list(lengths)
         self.num_q_heads = int(num_q_heads)
         blob, table = plans.build(spans, np.array(pages, dtype=np.int64), len(spans), self.num_q_heads,
-                                  kv.num_kv_heads, _sms(kv.pool.device.index), cols)
+                                  kv.num_kv_heads, _sms(kv.pool.device.index), score_cols=cols)
         blob = plans.append_sections(blob, table, chunks=np.array(chunks), requests=np.array(reqs))
         table.update(chunks=len(chunks), requests=len(reqs), most_tokens=max(self.lengths, default=0), score_cols=col)
         self._native = native().CachePlan(torch.from_numpy(blob), kv, table)

@@ -14,10 +14,15 @@ import numpy as np
 UNIT_INTS = 8
 ROW_UNIT_ROWS = 16
 STAGE_KEYS = 16          # keys per stage of the row kernel
+TILE_UNIT_ROWS = 128
+TILE_KEYS = 64           # keys per block of the tile kernel
+TILE_MIN_ROWS = 17       # fewest query rows (tokens x group heads) the tile kernel takes
 CHUNK_KEYS = 512         # keys per block that adds up weights
 NO_LIMIT = 1 << 30
 ROW_SLOTS = 8            # warps of the row kernel an SM holds
 ROW_MIN_STAGES = 4       # shortest range of a row unit, in stages
+TILE_SLOTS = 2           # CTAs of the tile kernel an SM holds
+TILE_MIN_BLOCKS = 4      # shortest range of a tile unit, in blocks
 
 
 class Span(NamedTuple):
@@ -62,19 +67,24 @@ def _cut(tiles: np.ndarray, kv_heads: int, slots: int, stage: int, min_stages: i
     return np.concatenate([tiles[idx], lo[:, None], hi[:, None]], axis=1)
 
 
-def build(row_spans: Sequence[Span], pages: np.ndarray, tokens: int, num_q_heads: int, kv_heads: int, sms: int,
-          score_cols: Sequence[int] = ()) -> Tuple[np.ndarray, Dict[str, int]]:
-    """The int32 blob of a plan and its section table.  ``score_cols``: first
-    score column of each span (weighted plans)."""
+def build(spans: Sequence[Span], pages: np.ndarray, tokens: int, num_q_heads: int, kv_heads: int, sms: int,
+          tiles: bool = False, score_cols: Sequence[int] = ()) -> Tuple[np.ndarray, Dict[str, int]]:
+    """The int32 blob of a plan and its section table.  ``tiles``: spans of
+    many rows go to the tile kernel.  ``score_cols``: first score column of
+    each span (weighted plans, row kernel only)."""
     if num_q_heads % kv_heads:
         raise ValueError(f"{num_q_heads} query heads are no multiple of {kv_heads} KV heads")
     group = num_q_heads // kv_heads
     if group > 128:
         raise ValueError(f"at most 128 query heads per KV head, got {group}")
-    rows = _cut(_row_tiles(row_spans, group, ROW_UNIT_ROWS), kv_heads, sms * ROW_SLOTS, STAGE_KEYS, ROW_MIN_STAGES)
+    many = [tiles and s.tokens * group >= TILE_MIN_ROWS for s in spans]
+    rows = _cut(_row_tiles([s for s, m in zip(spans, many) if not m], group, ROW_UNIT_ROWS), kv_heads,
+                sms * ROW_SLOTS, STAGE_KEYS, ROW_MIN_STAGES)
+    wide = _cut(_row_tiles([s for s, m in zip(spans, many) if m], group, TILE_UNIT_ROWS), kv_heads, sms * TILE_SLOTS,
+                TILE_KEYS, TILE_MIN_BLOCKS)
     head_chunks = -(-group // ROW_UNIT_ROWS)
 
-    units = rows
+    units = np.concatenate([rows, wide])
     n_rows = units[:, 1] * units[:, 2]
     part = np.cumsum(n_rows * kv_heads) - n_rows * kv_heads
     rec = np.zeros((len(units), UNIT_INTS), dtype=np.int64)
@@ -88,10 +98,13 @@ def build(row_spans: Sequence[Span], pages: np.ndarray, tokens: int, num_q_heads
         rec[:, 7] = np.asarray(score_cols, dtype=np.int64)[units[:, 7]]
     part_rows = int((n_rows * kv_heads).sum())
 
-    # the partial rows of each (token, chunk of 16 group heads)
-    idx = np.repeat(np.arange(len(units)), units[:, 1])
-    j = np.arange(len(idx)) - np.repeat(np.cumsum(units[:, 1]) - units[:, 1], units[:, 1])
-    key = (units[idx, 0] + j) * head_chunks + units[idx, 3] // ROW_UNIT_ROWS
+    # the partial rows of each (token, chunk of 16 group heads); a tile unit has all chunks of its tokens
+    chunks = np.where(np.arange(len(units)) < len(rows), 1, head_chunks)
+    per = units[:, 1] * chunks
+    idx = np.repeat(np.arange(len(units)), per)
+    k = np.arange(len(idx)) - np.repeat(np.cumsum(per) - per, per)
+    j = k // chunks[idx]
+    key = (units[idx, 0] + j) * head_chunks + units[idx, 3] // ROW_UNIT_ROWS + k % chunks[idx]
     order = np.argsort(key, kind="stable")
     entries = np.stack([part[idx] + j * units[idx, 2] - units[idx, 3], n_rows[idx]], axis=1)[order]
     counts = np.bincount(key, minlength=tokens * head_chunks)
@@ -99,10 +112,10 @@ def build(row_spans: Sequence[Span], pages: np.ndarray, tokens: int, num_q_heads
     if part_rows >= 1 << 31:
         raise ValueError("the batch needs too many partial rows")
 
-    table = dict(tokens=tokens, num_q_heads=num_q_heads, row_units=len(rows), tile_units=0, head_chunks=head_chunks,
+    table = dict(tokens=tokens, num_q_heads=num_q_heads, row_units=len(rows), tile_units=len(wide), head_chunks=head_chunks,
                  most_parts=int(counts.max()) if counts.size else 0, part_rows=part_rows,
                  max_page=int(pages.max()) if pages.size else -1, chunks=0, requests=0, most_tokens=0, score_cols=0)
-    return _pack(table, row_units=rec, tile_units=rec[len(rows):], merge=entries, merge_off=off, pages=pages)
+    return _pack(table, row_units=rec[:len(rows)], tile_units=rec[len(rows):], merge=entries, merge_off=off, pages=pages)
 
 
 def _pack(table: Dict[str, int], **sections: np.ndarray) -> Tuple[np.ndarray, Dict[str, int]]:

@@ -15,12 +15,12 @@ def _units(blob, table, name):
     return blob[at:at + n * plans.UNIT_INTS].reshape(n, plans.UNIT_INTS)
 
 
-def _check(spans, nq, nkv, sms=148):
+def _check(spans, nq, nkv, sms=148, tiles=False):
     """Every (token, head) row meets each key it sees exactly once, and finds
     all of its partial rows in its list."""
     pages = np.arange(10)
     tokens = max((s.token + s.tokens for s in spans), default=0)
-    blob, table = plans.build(spans, pages, tokens, nq, nkv, sms)
+    blob, table = plans.build(spans, pages, tokens, nq, nkv, sms, tiles)
     G = nq // nkv
     want, got, parts = {}, {}, {}
     for s in spans:
@@ -60,12 +60,14 @@ def _check(spans, nq, nkv, sms=148):
 
 
 @pytest.mark.parametrize("nq,nkv", [(4, 4), (6, 2), (8, 1), (20, 1), (40, 1), (128, 1), (14, 2)])
-def test_units_cover_every_key_once(nq, nkv):
+@pytest.mark.parametrize("tiles", [False, True])
+def test_units_cover_every_key_once(nq, nkv, tiles):
     S = plans.Span
     _check([S(0, 5, 300, plans.NO_LIMIT, 0), S(0, 2, 33, 32, 1), S(2, 3, 3, 1, 2), S(5, 1, 0, 0, 3), S(6, 1, 7, 7, 4)],
-           nq, nkv)
-    _check([], nq, nkv)
-    _check([S(0, 3, 0, plans.NO_LIMIT, 0)], nq, nkv)
+           nq, nkv, tiles=tiles)
+    _check([S(0, 70, 400, plans.NO_LIMIT, 0), S(0, 70, 90, 21, 1)], nq, nkv, tiles=tiles)
+    _check([], nq, nkv, tiles=tiles)
+    _check([S(0, 3, 0, plans.NO_LIMIT, 0)], nq, nkv, tiles=tiles)
 
 
 @pytest.mark.parametrize("seed", range(4))
@@ -81,7 +83,7 @@ def test_random_batches(seed):
             own.append(plans.Span(t, q, n, n - q + 1, 100 * i + len(own)))
             t += q
         spans += [plans.Span(first, t - first, int(rng.integers(0, 2000)), plans.NO_LIMIT, 100 * i + 99)] + own
-    _check(spans, 8, 2)
+    _check(spans, 8, 2, tiles=seed % 2 == 0)
 
 
 def test_long_contexts_spread_over_the_gpu():
