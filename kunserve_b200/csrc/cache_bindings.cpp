@@ -4,6 +4,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
+#include <cmath>
 
 #include "kernels/cache_ops.h"
 
@@ -246,6 +247,7 @@ torch::Tensor cached_attention_op(const torch::Tensor& q, const PagedKV& kv, int
   CachedAttn a{};
   a.g = kv.g;
   KUS_CHECK(a.g.hd == 64 || a.g.hd == 128, "attention takes head_dim 64 or 128, the cache has ", a.g.hd);
+  KUS_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive");
   check_heads(q, plan.T, plan.nq, a.g.hd, kv.pool, "q");
   KUS_CHECK(q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
               "q's heads must start on 16 bytes");

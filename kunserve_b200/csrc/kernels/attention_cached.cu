@@ -22,7 +22,7 @@
 namespace kus {
 namespace cat {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 1;
 constexpr int kKeys = 16;       // keys per stage
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -30,7 +30,7 @@ template <int HD>
 struct RowCfg {
   static constexpr int kTile = kKeys * HD * 2;        // K or V of a stage
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kStages = HD == 128 ? 3 : 6;   // 24 KB a warp, two blocks of four warps an SM
+  static constexpr int kStages = HD == 128 ? 3 : 6;   // 24 KB a warp
   static constexpr int kSmem = kWarps * kStages * kStage;
 };
 
@@ -303,7 +303,7 @@ KUS_DEVICE float2 join_stats(const CachedAttn& a, int e0, int e1, int kh, int g,
 // weights exp(s - M) / L, summed over the group's heads, are added to the
 // cache's.  Each weight has one writer: no atomics.
 template <typename T, int HD, int W>
-__global__ void __launch_bounds__(128) join_kernel(CachedAttn a, unsigned joins) {
+__global__ void __launch_bounds__(128, 8) join_kernel(CachedAttn a, unsigned joins) {
   constexpr int kPer = HD / 32;   // dims a lane holds
   constexpr int kRows = 4 / W;    // rows a block joins
   __shared__ float sh_o[4][HD];

@@ -2,22 +2,24 @@
 // query rows, the queries of many requests behind one shared prefix (or a
 // long chunk of one request), on the sm_100a tensor cores.
 //
-// One CTA takes one (unit, KV head): its rows against blocks of 64 keys,
+// One CTA takes one (unit, KV head): its rows against blocks of 128 keys,
 // S = Q K^T and O += P V by tcgen05.mma with S, P and O in TMEM.
 //
-//   warps 0-3  softmax: thread r holds row r (TMEM lane r), a block's 64
-//              scores in registers; P goes back to TMEM as 16-bit pairs over
-//              the scores it came from, from where O += P V reads it
-//   warp 4     TMA producer: K and V blocks, one box per page and 64-dim half
-//   warp 5     MMA issuer and TMEM owner; QK(i + 1) is issued before PV(i),
-//              so a block's scores are ready when the previous block's
-//              probabilities are written
+//   warps 0-7  softmax: two threads a row (TMEM lane r), 64 of the block's
+//              scores each in registers; the probabilities go as 16-bit
+//              pairs to TMEM, from where O += P V reads them
+//   warps 8, 9 TMA producers of K and of V: one box per page and 64-dim half,
+//              a lane per box, its page looked up a block ahead
+//   warp 10    issues QK (and owns TMEM), warp 11 issues PV: a thread that issues
+//              one product waits for most of it, which would hold the other up
 //
-// Two S buffers; QK(i + 2) waits for PV(i), which reads its P from the same
-// columns.  O is rescaled only when a row's max grew by more than 2^8 (the
-// sum and O share the stale max).
-// Two CTAs an SM (about 100 KB of shared memory, 256 TMEM columns each): one
-// CTA's softmax runs beside the other's products.
+// S and P have two buffers each (with O all 512 TMEM columns, one CTA an SM):
+// QK(i + 1) and PV(i - 1) run while block i's softmax does, which is what
+// bounds an iteration.  Blocks of 128 keys and not 64: the tensor core reads
+// Q from shared memory once per block, which at N = 64 takes longer than the
+// products.  Probabilities are taken against a row's max so far; only where
+// the block's is more than 2^8 times as large are they taken again and O
+// rescaled (the sum and O share the stale max).
 //
 // The keys a unit covers end inside a page or a block: boxes past the end
 // are not loaded, the tail rows of V are zeroed (a stale NaN times a zero
@@ -35,33 +37,35 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn();
 namespace cpt {
 
 constexpr int kRows = kTileUnitRows;
-constexpr int kKeys = 64;
-constexpr int kThreads = 192;
-constexpr uint32_t kCols = 256;          // S0 [0, 64), S1 [64, 128), O [128, 128 + HD)
-constexpr uint32_t kColO = 128;
+constexpr int kKeys = 128;
+constexpr int kSoftmax = 256;            // softmax threads: two a row
+constexpr int kThreads = kSoftmax + 128;
+constexpr uint32_t kCols = 512;          // S0, S1 [0, 256), P0, P1 [256, 384), O [384, 384 + HD)
+constexpr uint32_t kColP = 256;
+constexpr uint32_t kColO = 384;
 constexpr float kRescaleLog2 = 8.0f;
 
 template <int HD>
 struct Cfg {
   static constexpr int kHalves = HD / 64;
   static constexpr int kQHalf = kRows * 128;            // 64 dims of Q (16 KB)
-  static constexpr int kHalf = kKeys * 128;             // 64 dims of a K or V block (8 KB)
+  static constexpr int kHalf = kKeys * 128;             // 64 dims of a K or V block (16 KB)
   static constexpr int kTile = kHalves * kHalf;
-  static constexpr int kStages = HD == 128 ? 2 : 4;
+  static constexpr int kKStages = HD == 128 ? 3 : 5, kVStages = HD == 128 ? 2 : 4;
   static constexpr int kKOff = kHalves * kQHalf;
-  static constexpr int kVOff = kKOff + kStages * kTile;
-  static constexpr int kBarOff = kVOff + kStages * kTile;
-  static constexpr int kSmem = kBarOff + 256 + 1024;    // at least a third of an SM: TMEM holds two CTAs
-  static_assert(kSmem > 76 * 1024 && kSmem <= 113 * 1024, "two CTAs an SM");
+  static constexpr int kVOff = kKOff + kKStages * kTile;
+  static constexpr int kBarOff = kVOff + kVStages * kTile;
+  static constexpr int kMaxOff = kBarOff + 256;         // fp32 [2 halves][rows]
+  static constexpr int kSmem = kMaxOff + 2 * kRows * 4 + 1024;
+  static_assert(kSmem > 114 * 1024 && kSmem <= 200 * 1024, "one CTA an SM, and room for a warp of the row kernel");
 };
 
 template <int HD>
 struct Bars {
   uint64_t q_full;
-  uint64_t k_full[Cfg<HD>::kStages], k_empty[Cfg<HD>::kStages];
-  uint64_t v_full[Cfg<HD>::kStages], v_empty[Cfg<HD>::kStages];
-  uint64_t s_full[2];
-  uint64_t p_full, pv_done;
+  uint64_t k_full[Cfg<HD>::kKStages], k_empty[Cfg<HD>::kKStages];
+  uint64_t v_full[Cfg<HD>::kVStages], v_empty[Cfg<HD>::kVStages];
+  uint64_t s_full[2], s_empty[2], p_full[2], pv_done[2];
   uint32_t tmem;
 };
 
@@ -72,29 +76,65 @@ KUS_DEVICE void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar,
       : "memory");
 }
 
-// 32 lanes x 32 columns, not waited for.
-KUS_DEVICE void tmem_ld32(uint32_t taddr, uint32_t* r) {
+// 32 lanes x 16 columns.  Loads are not waited for; tmem_wait_ld waits for
+// all of this thread's, and r, loaded before, cannot be used above it.
+constexpr int kChunk = 16;
+KUS_DEVICE void tmem_ld(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
-KUS_DEVICE void tmem_st32(uint32_t taddr, const uint32_t* r) {
+KUS_DEVICE void tmem_wait_ld(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+KUS_DEVICE void tmem_st(uint32_t taddr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-KUS_DEVICE void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 KUS_DEVICE void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two fp32 lanes in one instruction, and the largest of three.
+KUS_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
+        "l"(reinterpret_cast<const unsigned long long&>(c)));
+  return reinterpret_cast<float2&>(d);
+}
+KUS_DEVICE float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return reinterpret_cast<float2&>(d);
+}
+KUS_DEVICE float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Whether `pred` holds in any of the `n` threads of named barrier `id`.
+KUS_DEVICE bool barrier_any(int id, int n, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.u32 p, %3, 0;\nbarrier.cta.red.or.pred q, %1, %2, p;\nselp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"(id), "r"(n), "r"((uint32_t)pred)
+      : "memory");
+  return r != 0;
+}
 
 // D(tmem) (+)= A(tmem) * B(smem desc): A's rows are TMEM lanes, a column
 // holds two 16-bit elements.
@@ -121,10 +161,9 @@ KUS_HOST_DEVICE constexpr uint32_t idesc(int N, bool b_mn) {
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant__ CUtensorMap map, CachedAttn a,
+__global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map, CachedAttn a,
                                                            int box, float scale_log2) {
   using Cf = Cfg<HD>;
-  constexpr int kStages = Cf::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -141,20 +180,24 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
   const int nb = (key_hi - key_lo + kKeys - 1) / kKeys;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bars->q_full, kRows);
-    for (int s = 0; s < kStages; ++s) {
+    mbar_init(&bars->q_full, kSoftmax);
+    for (int s = 0; s < Cf::kKStages; ++s) {
       mbar_init(&bars->k_full[s], 1);
       mbar_init(&bars->k_empty[s], 1);
+    }
+    for (int s = 0; s < Cf::kVStages; ++s) {
       mbar_init(&bars->v_full[s], 1);
       mbar_init(&bars->v_empty[s], 1);
     }
-    mbar_init(&bars->s_full[0], 1);
-    mbar_init(&bars->s_full[1], 1);
-    mbar_init(&bars->p_full, kRows);
-    mbar_init(&bars->pv_done, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->s_full[b], 1);
+      mbar_init(&bars->s_empty[b], kSoftmax);
+      mbar_init(&bars->p_full[b], kSoftmax);
+      mbar_init(&bars->pv_done[b], 1);
+    }
     fence_barrier_init();
   }
-  if (warp == 5) tmem_alloc(&bars->tmem, kCols);
+  if (warp == 10) tmem_alloc(&bars->tmem, kCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -162,78 +205,90 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
   pdl_wait();
   pdl_trigger();
 
-  if (warp == 4) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      prefetch_tmap(&map);
-      const int* table = a.pages + u1.y;
-      const int per_slot = 2 * a.g.block_size;   // K rows, then V rows of one (page, layer)
-      bool ok = true;
-      for (int i = 0; i < nb && ok; ++i) {
-        const int s = i % kStages;
-        const uint32_t ph = (uint32_t)(i / kStages) & 1u;
-        const int key0 = key_lo + i * kKeys;
-        const int boxes = (min(kKeys, key_hi - key0) + box - 1) / box;
-        const uint32_t bytes = (uint32_t)boxes * box * HD * 2;
-        ok = mbar_wait(&bars->k_empty[s], ph ^ 1u, kErrWaitEmpty);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&bars->k_full[s], bytes);
-        const uint32_t kd = sbase + Cf::kKOff + s * Cf::kTile, vd = sbase + Cf::kVOff + s * Cf::kTile;
-        auto row_of = [&](int j) {
-          const int key = key0 + j * box;
-          return kv_slot(a.g, __ldg(table + kv_page_col(a.g, key)), a.layer) * per_slot + kv_page_slot(a.g, key);
-        };
-        for (int j = 0; j < boxes; ++j) {
-          const int row = row_of(j);
+  if (warp == 8 || warp == 9) {
+    // ----------------------------------------------------------- producers
+    const bool is_v = warp == 9;
+    const int stages = is_v ? Cf::kVStages : Cf::kKStages;
+    const int* table = a.pages + u1.y;
+    uint64_t* full = is_v ? bars->v_full : bars->k_full;
+    uint64_t* empty = is_v ? bars->v_empty : bars->k_empty;
+    const uint32_t region = sbase + (is_v ? Cf::kVOff : Cf::kKOff);
+    if (lane == 0) prefetch_tmap(&map);
+    // tensor map row of this lane's box of block i (-1: past the keys)
+    auto row_of = [&](int i) {
+      const int key = key_lo + i * kKeys + lane * box;
+      if (lane * box >= kKeys || key >= key_hi) return -1;
+      return kv_slot(a.g, __ldg(table + kv_page_col(a.g, key)), a.layer) * 2 * a.g.block_size +
+             (is_v ? a.g.block_size : 0) + kv_page_slot(a.g, key);
+    };
+    int row = row_of(0), s = 0;
+    uint32_t ph = 1;
+    bool ok = true;
+    for (int i = 0; i < nb; ++i) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph, kErrWaitEmpty));
+      if (!ok) break;
+      const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, row >= 0));
+      if (lane == 0) mbar_arrive_expect_tx(&full[s], boxes * box * HD * 2);
+      __syncwarp();
+      if (row >= 0) {
+        const uint32_t dst = region + s * Cf::kTile + lane * box * 128;
 #pragma unroll
-          for (int h = 0; h < Cf::kHalves; ++h)
-            tma_load_3d(kd + h * Cf::kHalf + j * box * 128, &map, &bars->k_full[s], 64 * h, kh, row);
-        }
-        ok = mbar_wait(&bars->v_empty[s], ph ^ 1u, kErrWaitEmpty);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&bars->v_full[s], bytes);
-        for (int j = 0; j < boxes; ++j) {
-          const int row = row_of(j) + a.g.block_size;
-#pragma unroll
-          for (int h = 0; h < Cf::kHalves; ++h)
-            tma_load_3d(vd + h * Cf::kHalf + j * box * 128, &map, &bars->v_full[s], 64 * h, kh, row);
-        }
+        for (int h = 0; h < Cf::kHalves; ++h) tma_load_3d(dst + h * Cf::kHalf, &map, &full[s], 64 * h, kh, row);
       }
-      // every load has landed before the CTA may leave
-      for (int i = max(0, nb - kStages); i < nb; ++i) {
-        mbar_wait(&bars->k_full[i % kStages], (uint32_t)(i / kStages) & 1u, kErrWaitFull);
-        mbar_wait(&bars->v_full[i % kStages], (uint32_t)(i / kStages) & 1u, kErrWaitFull);
+      row = row_of(i + 1);
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+    // every load has landed before the CTA may leave
+    if (ok)
+      for (int i = max(0, nb - stages); i < nb; ++i)
+        mbar_wait(&full[i % stages], (uint32_t)(i / stages) & 1u, kErrWaitFull);
+    __syncwarp();
+  } else if (warp == 10) {
+    // ------------------------------------------------------- S = Q K^T
+    if (lane == 0) {
+      constexpr uint32_t id_qk = idesc<T>(kKeys, false);
+      bool ok = mbar_wait(&bars->q_full, 0, kErrWaitFull);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int i = 0; i < nb && ok; ++i) {
+        const int b = i & 1;
+        ok = mbar_wait(&bars->k_full[s], ph, kErrWaitFull);
+        // the scores of block i - 2 are read, and its probabilities: S(i) full
+        // tells the softmax that both buffers are free
+        const uint32_t before = (uint32_t)((i >> 1) - 1) & 1u;
+        if (i >= 2)
+          ok = ok && mbar_wait(&bars->s_empty[b], before, kErrWaitTmemEmpty) &&
+               mbar_wait(&bars->pv_done[b], before, kErrWaitTmemEmpty);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t qd = umma_desc_sw128(sbase), kd = umma_desc_sw128(sbase + Cf::kKOff + s * Cf::kTile);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          umma_f16(tmem + b * kKeys, qd + (uint64_t)(((kk >> 2) * Cf::kQHalf >> 4) + 2 * (kk & 3)),
+                   kd + (uint64_t)(((kk >> 2) * Cf::kHalf >> 4) + 2 * (kk & 3)), id_qk, kk > 0 ? 1u : 0u);
+        umma_commit(&bars->s_full[b]);
+        umma_commit(&bars->k_empty[s]);
+        if (++s == Cf::kKStages) {
+          s = 0;
+          ph ^= 1;
+        }
       }
     }
     __syncwarp();
-  } else if (warp == 5) {
-    // ---------------------------------------------------------- MMA issuer
-    constexpr uint32_t id_qk = idesc<T>(kKeys, false), id_pv = idesc<T>(HD, true);
-    bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, 0, kErrWaitFull));
-    auto qk = [&](int i) {
-      const int s = i % kStages;
-      // PV(i - 2) has read its probabilities from the columns S(i) goes to
-      if (i >= 2) ok = ok && mbar_wait(&bars->pv_done, (uint32_t)i & 1u, kErrWaitTmemEmpty);
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->k_full[s], (uint32_t)(i / kStages) & 1u, kErrWaitFull));
-      tc_fence_after();
-      if (ok && lane == 0) {
-        const uint32_t qb = sbase, kb = sbase + Cf::kKOff + s * Cf::kTile;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          umma_f16(tmem + (i & 1) * kKeys, umma_desc_sw128(qb + (kk >> 2) * Cf::kQHalf) + (uint64_t)(2 * (kk & 3)),
-                   umma_desc_sw128(kb + (kk >> 2) * Cf::kHalf) + (uint64_t)(2 * (kk & 3)), id_qk, kk > 0 ? 1u : 0u);
-        umma_commit(&bars->s_full[i & 1]);
-        umma_commit(&bars->k_empty[s]);
-      }
-      __syncwarp();
-    };
-    if (ok) qk(0);
-    for (int i = 0; i < nb && ok; ++i) {
-      if (i + 1 < nb) qk(i + 1);
-      const int s = i % kStages;
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->v_full[s], (uint32_t)(i / kStages) & 1u, kErrWaitFull));
+  } else if (warp == 11) {
+    // ------------------------------------------------------- O += P V
+    constexpr uint32_t id_pv = idesc<T>(HD, true);
+    bool ok = true;
+    int s = 0;
+    uint32_t ph = 0;
+    for (int i = 0; i < nb; ++i) {
+      const int b = i & 1;
+      ok = mbar_wait(&bars->v_full[s], ph, kErrWaitFull);
       const int have = key_hi - (key_lo + i * kKeys);
-      if (ok && have < kKeys) {
+      if (have < kKeys) {
         // rows past the keys: the loaded boxes' stale slots and what was not loaded
         uint8_t* vt = smem + Cf::kVOff + s * Cf::kTile;
         for (int c = lane; c < (kKeys - have) * 8; c += 32)
@@ -243,118 +298,154 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->p_full, (uint32_t)i & 1u, kErrWaitFull));
-      tc_fence_after();
-      if (ok && lane == 0) {
-        const uint32_t vb = sbase + Cf::kVOff + s * Cf::kTile;
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->p_full[b], (uint32_t)(i >> 1) & 1u, kErrWaitFull));
+      if (!ok) break;
+      if (lane == 0) {
+        tc_fence_after();
+        const uint64_t vd = v_desc(sbase + Cf::kVOff + s * Cf::kTile, Cf::kHalf);
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
-          umma_f16_ta(tmem + kColO, tmem + (i & 1) * kKeys + kk * 8, v_desc(vb + kk * 16 * 128, Cf::kHalf), id_pv,
+          umma_f16_ta(tmem + kColO, tmem + kColP + b * (kKeys / 2) + kk * 8, vd + (uint64_t)(kk * 16 * 128 >> 4), id_pv,
                       (i > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&bars->pv_done);
+        umma_commit(&bars->pv_done[b]);
         umma_commit(&bars->v_empty[s]);
       }
       __syncwarp();
+      if (++s == Cf::kVStages) {
+        s = 0;
+        ph ^= 1;
+      }
     }
   } else {
     // --------------------------------------------------- Q, softmax, output
-    const int r = threadIdx.x;
+    const int half = warp >> 2, r = threadIdx.x & (kRows - 1);   // TMEM lane of warp w: 32 (w % 4) + lane
     const bool valid = r < rows;
     const int j = valid ? r / ng : 0, gi = valid ? r - j * ng : 0;
     {
       const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (tok0 + j) * a.qt +
                                                         (long long)(kh * G + g0 + gi) * a.qh);
+      constexpr int kEach = HD / 16;   // 16-byte chunks of a thread
 #pragma unroll
-      for (int h = 0; h < Cf::kHalves; ++h)
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint4 v = valid ? __ldg(src + h * 8 + c) : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(smem + h * Cf::kQHalf + r * 128 + ((c ^ (r & 7)) << 4)) = v;
-        }
+      for (int e = 0; e < kEach; ++e) {
+        const int c = half * kEach + e;
+        const uint4 v = valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(smem + (c >> 3) * Cf::kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&bars->q_full);
     }
     const int end = min(key_hi, lim0 + j);       // keys this row sees
     const int end_min = min(key_hi, lim0);       // and every row sees
-    const uint32_t tl = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t t_o = tl + kColO + half * (HD / 2);
+    float* maxima = reinterpret_cast<float*>(smem + Cf::kMaxOff);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int i = 0; i < nb; ++i) {
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->s_full[i & 1], (uint32_t)(i >> 1) & 1u, kErrWaitTmemFull));
+      const int b = i & 1;
+      const uint32_t t_s = tl + b * kKeys + half * 64, t_p = tl + kColP + b * (kKeys / 2) + half * 32;
+      ok = ok && mbar_wait(&bars->s_full[b], (uint32_t)(i >> 1) & 1u, kErrWaitTmemFull);
+      __syncwarp();
       tc_fence_after();
-      const uint32_t ts = tl + (i & 1) * kKeys;
-      uint32_t sv[64];
-      tmem_ld32(ts, sv);
-      tmem_ld32(ts + 32, sv + 32);
-      tmem_wait_ld();
       const int key0 = key_lo + i * kKeys;
+      uint32_t v[64];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld(t_s + kChunk * c, v + kChunk * c);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_wait_ld(v + kChunk * c);
+      tc_fence_before();
+      mbar_arrive(&bars->s_empty[b]);
       if (key0 + kKeys > end_min) {
+        const int left = end - key0 - half * 64;   // of this thread's keys, those its row sees
 #pragma unroll
         for (int e = 0; e < 64; ++e)
-          if (key0 + e >= end) sv[e] = 0xff800000u;   // -inf
+          if (e >= left) v[e] = 0xff800000u;   // -inf
       }
-      float mx[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sv[e]);
-#pragma unroll
-      for (int e = 4; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(sv[e]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
-      const bool grow = top > m + kRescaleLog2;
-      const float mn = grow ? top : m;
-      const float alpha = grow ? ex2(m - mn) : 1.f;
-      const float ref = mn == -INFINITY ? 0.f : mn;   // no key seen yet
+      // Probabilities against the max so far, the block's own max beside
+      // them: it is only seldom needed, and the exponentials bound this loop.
       uint32_t pk[32];
-      float sum[2] = {0.f, 0.f};
+      float sum;
+      float mx[2] = {-INFINITY, -INFINITY};
+      auto probabilities = [&](float ref) {
+        const float2 scale2 = make_float2(scale_log2, scale_log2), ref2 = make_float2(-ref, -ref);
+        float2 acc[2] = {};
 #pragma unroll
-      for (int e = 0; e < 64; e += 2) {
-        const float p0 = ex2(fmaf(__uint_as_float(sv[e]), scale_log2, -ref));
-        const float p1 = ex2(fmaf(__uint_as_float(sv[e + 1]), scale_log2, -ref));
-        sum[0] += p0;
-        sum[1] += p1;
-        pk[e / 2] = pack2<T>(p0, p1);
+        for (int e = 0; e < 64; e += 2) {
+          const float2 x = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2, ref2);
+          const float2 p = make_float2(ex2(x.x), ex2(x.y));
+          acc[(e / 2) & 1] = add2(acc[(e / 2) & 1], p);
+          pk[e / 2] = pack2<T>(p.x, p.y);
+        }
+        sum = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+      };
+      probabilities(m == -INFINITY ? 0.f : m);
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        mx[0] = max3(mx[0], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+        mx[1] = max3(mx[1], __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
       }
-      tmem_st32(ts, pk);
-      if (i > 0) {
-        // PV(i - 1) is done: O is stable
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->pv_done, (uint32_t)(i - 1) & 1u, kErrWaitTmemFull));
-        tc_fence_after();
-        if (__any_sync(0xffffffffu, grow)) {
+      const float top = fmaxf(mx[0], mx[1]) * scale_log2;
+      if (barrier_any(1 + (warp & 3), 64, top > m + kRescaleLog2)) {
+        // some row of this pair of warps outgrew its max
+        float* mine = maxima + r;
+        mine[half * kRows] = top;
+        named_barrier(1 + (warp & 3), 64);
+        const float both = fmaxf(top, mine[(half ^ 1) * kRows]);
+        const bool grow = both > m + kRescaleLog2;
+        const float mn = grow ? both : m;
+        const float alpha = grow ? ex2(m - mn) : 1.f;
+        probabilities(mn == -INFINITY ? 0.f : mn);   // no key seen yet: zeros
+        if (i > 0) {
+          // PV(i - 1) is done: O is stable
+          ok = ok && mbar_wait(&bars->pv_done[b ^ 1], (uint32_t)((i - 1) >> 1) & 1u, kErrWaitTmemFull);
+          __syncwarp();
+          tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tl + kColO + 32 * c, o);
-            tmem_wait_ld();
+          for (int c = 0; c < HD / 2 / kChunk; ++c) {
+            uint32_t o[kChunk];
+            tmem_ld(t_o + kChunk * c, o);
+            tmem_wait_ld(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st32(tl + kColO + 32 * c, o);
+            for (int e = 0; e < kChunk; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st(t_o + kChunk * c, o);
           }
         }
+        l *= alpha;
+        m = mn;
       }
+      tmem_st(t_p, pk);
+      tmem_st(t_p + kChunk, pk + kChunk);
+      l += sum;
       tmem_wait_st();
-      l = l * alpha + sum[0] + sum[1];
-      m = mn;
       tc_fence_before();
-      mbar_arrive(&bars->p_full);
+      mbar_arrive(&bars->p_full[b]);
     }
-    ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->pv_done, (uint32_t)(nb - 1) & 1u, kErrWaitTmemFull));
+    // the halves' sums (m is the same in both)
+    named_barrier(1 + (warp & 3), 64);
+    float* mine = maxima + r;
+    mine[half * kRows] = l;
+    named_barrier(1 + (warp & 3), 64);
+    l += mine[(half ^ 1) * kRows];
+    ok = ok && mbar_wait(&bars->pv_done[(nb - 1) & 1], (uint32_t)((nb - 1) >> 1) & 1u, kErrWaitTmemFull);
+    __syncwarp();
     tc_fence_after();
     const long long prow = u1.z + (long long)kh * rows + r;
-    float* dst = a.part_o + prow * HD;
-#pragma unroll 1
-    for (int c = 0; c < HD / 32; ++c) {
-      uint32_t o[32];
-      tmem_ld32(tl + kColO + 32 * c, o);
-      tmem_wait_ld();
+    float* dst = a.part_o + prow * HD + half * (HD / 2);
+#pragma unroll
+    for (int c = 0; c < HD / 2 / kChunk; ++c) {
+      uint32_t o[kChunk];
+      tmem_ld(t_o + kChunk * c, o);
+      tmem_wait_ld(o);
       if (valid)
 #pragma unroll
-        for (int e = 0; e < 32; e += 4)
-          *reinterpret_cast<uint4*>(dst + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        for (int e = 0; e < kChunk; e += 4)
+          *reinterpret_cast<uint4*>(dst + kChunk * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
     }
-    if (valid) a.part_ml[prow] = make_float2(m, l);
+    if (valid && half == 0) a.part_ml[prow] = make_float2(m, l);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) tmem_dealloc(tmem, kCols);
+  if (warp == 10) tmem_dealloc(tmem, kCols);
 }
 
 template <typename T, int HD>

@@ -15,14 +15,16 @@ UNIT_INTS = 8
 ROW_UNIT_ROWS = 16
 STAGE_KEYS = 16          # keys per stage of the row kernel
 TILE_UNIT_ROWS = 128
-TILE_KEYS = 64           # keys per block of the tile kernel
+TILE_KEYS = 128          # keys per block of the tile kernel
 TILE_MIN_ROWS = 17       # fewest query rows (tokens x group heads) the tile kernel takes
 CHUNK_KEYS = 512         # keys per block that adds up weights
 NO_LIMIT = 1 << 30
-ROW_SLOTS = 8            # warps of the row kernel an SM holds
+ROW_SLOTS = 9            # warps of the row kernel an SM holds
 ROW_MIN_STAGES = 4       # shortest range of a row unit, in stages
-TILE_SLOTS = 2           # CTAs of the tile kernel an SM holds
-TILE_MIN_BLOCKS = 4      # shortest range of a tile unit, in blocks
+ROW_WAVES = 4            # units a slot takes, at least, when there is work for more than one
+TILE_SLOTS = 1           # CTAs of the tile kernel an SM holds
+TILE_MIN_BLOCKS = 2      # shortest range of a tile unit, in blocks
+TILE_START = 3           # what starting and ending a unit takes, in blocks
 
 
 class Span(NamedTuple):
@@ -52,14 +54,32 @@ def _row_tiles(spans: Sequence[Span], group: int, rows: int) -> np.ndarray:
     return np.array(out, dtype=np.int64).reshape(-1, 8)
 
 
-def _cut(tiles: np.ndarray, kv_heads: int, slots: int, stage: int, min_stages: int) -> np.ndarray:
-    """Cut the tiles' keys into ranges of about one slot's share of all
-    stages: columns of the tile, then first key and end of the range."""
+def _parts(stages: np.ndarray, share: int) -> np.ndarray:
+    """Equal ranges of at most ``share`` stages per tile."""
+    parts = -(-stages // share)
+    return -(-stages // np.maximum(-(-stages // np.maximum(parts, 1)), 1))   # no empty range at the end
+
+
+def _cut(tiles: np.ndarray, kv_heads: int, slots: int, stage: int, min_stages: int, waves: int) -> np.ndarray:
+    """Cut the tiles' keys into ranges: columns of the tile, then first key
+    and end of the range.
+
+    Up to ``waves`` slots' worth of units a slot, the range is the one whose
+    waves of units (each as long as its longest, and a start's worth of
+    stages more) take least; beyond that the hardware evens units out, and
+    the range is a slot's share over ``waves``."""
     stages = -(-tiles[:, 4] // stage)
-    share = max(min_stages, -(-int(stages.sum()) * kv_heads // slots))
-    parts = np.maximum(1, stages // share)
-    each = -(-stages // parts)
-    parts = -(-stages // each)                       # no empty range at the end
+    total = int(stages.sum()) * kv_heads
+    share = max(min_stages, -(-total // (slots * waves)))
+    if len(tiles) and waves == 1:
+        most = int(stages.max())
+        tries = sorted({max(min_stages, -(-most // k)) for k in range(1, 65)} | {share})
+        def cost(c):
+            parts = _parts(stages, c)
+            return -(-int(parts.sum()) * kv_heads // slots) * (int((-(-stages // parts)).max()) + TILE_START)
+        share = min(tries, key=cost)
+    parts = _parts(stages, share)
+    each = -(-stages // np.maximum(parts, 1))
     idx = np.repeat(np.arange(len(tiles)), parts)
     k = np.arange(len(idx)) - np.repeat(np.cumsum(parts) - parts, parts)
     lo = k * each[idx] * stage
@@ -79,9 +99,9 @@ def build(spans: Sequence[Span], pages: np.ndarray, tokens: int, num_q_heads: in
         raise ValueError(f"at most 128 query heads per KV head, got {group}")
     many = [tiles and s.tokens * group >= TILE_MIN_ROWS for s in spans]
     rows = _cut(_row_tiles([s for s, m in zip(spans, many) if not m], group, ROW_UNIT_ROWS), kv_heads,
-                sms * ROW_SLOTS, STAGE_KEYS, ROW_MIN_STAGES)
+                sms * ROW_SLOTS, STAGE_KEYS, ROW_MIN_STAGES, ROW_WAVES)
     wide = _cut(_row_tiles([s for s, m in zip(spans, many) if m], group, TILE_UNIT_ROWS), kv_heads, sms * TILE_SLOTS,
-                TILE_KEYS, TILE_MIN_BLOCKS)
+                TILE_KEYS, TILE_MIN_BLOCKS, 1)
     head_chunks = -(-group // ROW_UNIT_ROWS)
 
     units = np.concatenate([rows, wide])
