@@ -275,17 +275,20 @@ torch::Tensor cached_attention_op(const torch::Tensor& q, const PagedKV& kv, int
   a.merge = reinterpret_cast<const int2*>(plan.ints(plan.o_merge));
   a.head_chunks = plan.head_chunks;
   a.most_parts = plan.most_parts;
-  // scratch of this call: partial rows (fp32 sums, max and sum), then the scores
+  // scratch of this call, in fp32: partial sums, (weighted) scores, partial
+  // (max, sum) and the rows' statistics; all but the last are read in vectors
   const bool weighted = weights.has_value();
-  const int64_t scores = weighted ? plan.score_cols * plan.nq : 0;
-  torch::Tensor scratch = torch::empty({plan.part_rows * (a.g.hd + 2) + scores},
+  const int64_t n_o = plan.part_rows * a.g.hd, n_s = weighted ? plan.score_cols * plan.nq : 0,
+                n_st = weighted ? 2LL * plan.T * plan.nq : 0;
+  torch::Tensor scratch = torch::empty({n_o + n_s + 2 * plan.part_rows + n_st},
                                        torch::TensorOptions().dtype(torch::kFloat32).device(kv.pool.device()));
   a.part_o = scratch.data_ptr<float>();
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + plan.part_rows * a.g.hd);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + n_o + n_s);
   if (weighted) {
     KUS_CHECK(plan.n_reqs > 0, "weights need a decode plan");
     kv.check_side(*weights, torch::kFloat32, "weights");
-    a.scores = a.part_o + plan.part_rows * (a.g.hd + 2);
+    a.scores = a.part_o + n_o;
+    a.stats = a.part_ml + plan.part_rows;
     a.weights = weights->data_ptr<float>();
     a.chunks = plan.ints(plan.o_chunks);
     a.n_chunks = plan.n_chunks;

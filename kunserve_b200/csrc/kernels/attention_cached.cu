@@ -269,47 +269,78 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float s
 }
 
 // ------------------------------------------------------------------ joins
-// Parts of one (token, head): entry e's row for this head.
-KUS_DEVICE long long part_row(const CachedAttn& a, int e, int kh, int g) {
-  const int2 p = __ldg(a.merge + e);
-  return p.x + (long long)kh * p.y + g;
+// (M, L) of two parts: the larger max, the sums brought to it.
+KUS_DEVICE float2 join2(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x);
+  if (m == -INFINITY) return make_float2(m, 0.f);
+  return make_float2(m, a.y * ex2(a.x - m) + b.y * ex2(b.x - m));
 }
-
-// Largest max and joint sum of parts [e0, e1) as the warp's lanes see them.
-KUS_DEVICE float2 join_stats(const CachedAttn& a, int e0, int e1, int kh, int g, int lane) {
-  float M = -INFINITY, L = 0.f;
-  for (int e = e0 + lane; e < e1; e += 32) {
-    const float2 ml = __ldcg(a.part_ml + part_row(a, e, kh, g));
-    const float n = fmaxf(M, ml.x);
-    if (n != -INFINITY) {
-      L = L * ex2(M - n) + ml.y * ex2(ml.x - n);
-      M = n;
-    }
-  }
+KUS_DEVICE float2 warp_join(float2 s) {
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, M, off), l2 = __shfl_xor_sync(0xffffffffu, L, off);
-    const float n = fmaxf(M, m2);
-    if (n != -INFINITY) {
-      L = L * ex2(M - n) + l2 * ex2(m2 - n);
-      M = n;
-    }
-  }
-  return make_float2(M, L);
+  for (int off = 16; off > 0; off >>= 1)
+    s = join2(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, off), __shfl_xor_sync(0xffffffffu, s.y, off)));
+  return s;
 }
 
-// Blocks [0, joins): W warps per (token, head) row join its parts.  Blocks
-// after them (weighted plans): one (chunk of keys, KV head) each, whose
-// weights exp(s - M) / L, summed over the group's heads, are added to the
-// cache's.  Each weight has one writer: no atomics.
+// Partial row of list entry p for a KV head and a head of its group.
+KUS_DEVICE long long part_row(int2 p, int kh, int g) { return p.x + (long long)kh * p.y + g; }
+
+// The keys [key0, key1) of one (request, KV head): their weights
+// exp(s - M) / L, summed over the group's heads, are added to the cache's;
+// sh_m, sh_l: the heads' M and 1 / L.  A thread takes four neighbouring keys.
+KUS_DEVICE void add_weights(const CachedAttn& a, const int* c, int kh, const float* sh_m, const float* sh_l) {
+  const int G = a.nq / a.g.kvh, bs = a.g.block_size;
+  const int key1 = c[2], first_page = c[3], len = c[4], col = c[5];
+  const long long pitch = (len + kKeys - 1) / kKeys * kKeys;
+  const int key = c[1] + 4 * threadIdx.x;
+  if (key >= key1) return;
+  // the rows of scores run on to a multiple of 16 keys
+  const float* src = a.scores + (long long)col * a.nq + kh * G * pitch + key;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int g = 0; g < G; ++g) {
+    const float4 s = __ldcg(reinterpret_cast<const float4*>(src + g * pitch));
+    const float m = sh_m[g], inv = sh_l[g];
+    x.x += ex2(s.x - m) * inv;
+    x.y += ex2(s.y - m) * inv;
+    x.z += ex2(s.z - m) * inv;
+    x.w += ex2(s.w - m) * inv;
+  }
+  auto at = [&](int k) {
+    const int page = __ldg(a.pages + first_page + kv_page_col(a.g, k));
+    return a.weights + ((long long)page * a.g.kvh + kh) * bs + kv_page_slot(a.g, k);
+  };
+  if (bs % 4 == 0 && key + 4 <= key1 && reinterpret_cast<uintptr_t>(a.weights) % 16 == 0) {
+    float4* w = reinterpret_cast<float4*>(at(key));
+    float4 v = *w;
+    v.x += x.x;
+    v.y += x.y;
+    v.z += x.z;
+    v.w += x.w;
+    *w = v;
+  } else {
+    const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (key + i < key1) *at(key + i) += xs[i];
+  }
+}
+
+constexpr int kJoinThreads = 128;
+
+// Blocks [0, joins): W warps per (token, head) row join its parts, 4 / W rows
+// a block; with a.stats the row's M and 1 / L are kept.  Blocks after them
+// (weighted plans of few parts): one (chunk of keys, KV head) each, with the
+// statistics joined again.  Each weight has one writer: no atomics.
+// What the plan says is read before the wait on the kernels that wrote the
+// parts.
 template <typename T, int HD, int W>
-__global__ void __launch_bounds__(128, 8) join_kernel(CachedAttn a, unsigned joins) {
-  constexpr int kPer = HD / 32;   // dims a lane holds
-  constexpr int kRows = 4 / W;    // rows a block joins
-  __shared__ float sh_o[4][HD];
+__global__ void __launch_bounds__(32 * (W > 4 ? W : 4), W > 4 ? 4 : 8) join_kernel(CachedAttn a, unsigned joins) {
+  constexpr int kPer = HD / 32;           // dims a lane holds
+  constexpr int kRows = W > 4 ? 1 : 4 / W;
+  __shared__ float sh_o[W > 1 ? W : 1][HD];
+  __shared__ float2 sh_ml[W > 1 ? W : 1];
   __shared__ float sh_m[128], sh_l[128];
-  pdl_wait();
-  pdl_trigger();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int kvh = a.g.kvh, G = a.nq / kvh;
   if (blockIdx.x < joins) {
@@ -318,17 +349,24 @@ __global__ void __launch_bounds__(128, 8) join_kernel(CachedAttn a, unsigned joi
     const int t = have ? (int)(row / a.nq) : 0, h = have ? (int)(row - (long long)t * a.nq) : 0;
     const int kh = h / G, g = h - kh * G;
     const int list = t * a.head_chunks + g / kRowUnitRows;
-    const int e0 = a.merge_off[list], e1 = have ? a.merge_off[list + 1] : e0;
-    const float2 st = join_stats(a, e0, e1, kh, g, lane);
+    const int e0 = __ldg(a.merge_off + list), e1 = have ? __ldg(a.merge_off + list + 1) : e0;
+    const int first = e0 + 32 * (warp % W);
+    int2 p = first + lane < e1 ? __ldg(a.merge + first + lane) : make_int2(0, 0);
+    pdl_wait();
+    pdl_trigger();
+    float2 st = make_float2(-INFINITY, 0.f);
     float acc[kPer] = {};
-    for (int b = e0 + 32 * (warp % W); b < e1; b += 32 * W) {
-      float w = 0.f;
-      long long prow = 0;
-      if (b + lane < e1) {
-        prow = part_row(a, b + lane, kh, g);
-        const float m = __ldcg(a.part_ml + prow).x;
-        w = m == -INFINITY ? 0.f : ex2(m - st.x);
-      }
+    for (int b = first; b < e1; b += 32 * W) {
+      if (b != first && b + lane < e1) p = __ldg(a.merge + b + lane);
+      const long long prow = part_row(p, kh, g);
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (b + lane < e1) ml = __ldcg(a.part_ml + prow);
+      const float2 sn = join2(st, warp_join(ml));
+      const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - sn.x);
+      const float keep = st.x == -INFINITY ? 0.f : ex2(st.x - sn.x);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) acc[i] *= keep;
+      st = sn;
       const int n = min(32, e1 - b);
 #pragma unroll 8
       for (int i = 0; i < n; ++i) {
@@ -352,11 +390,19 @@ __global__ void __launch_bounds__(128, 8) join_kernel(CachedAttn a, unsigned joi
     if (W > 1) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) sh_o[warp][lane * kPer + i] = acc[i];
+      if (lane == 0) sh_ml[warp] = st;
       __syncthreads();
       if (warp % W) return;
+      float2 all = st;
+      for (int j = 1; j < W; ++j) all = join2(all, sh_ml[j]);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        for (int j = 1; j < W; ++j) acc[i] += sh_o[warp + j][lane * kPer + i];
+      for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+      for (int j = 0; j < W; ++j) {
+        const float w = sh_ml[j].x == -INFINITY ? 0.f : ex2(sh_ml[j].x - all.x);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) acc[i] += w * sh_o[j][lane * kPer + i];
+      }
+      st = all;
     }
     if (!have) return;
     const float inv = st.y > 0.f ? 1.f / st.y : 0.f;
@@ -364,31 +410,48 @@ __global__ void __launch_bounds__(128, 8) join_kernel(CachedAttn a, unsigned joi
 #pragma unroll
     for (int i = 0; i < kPer; i += 2)
       *reinterpret_cast<uint32_t*>(dst + i) = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
+    if (a.stats && lane == 0) a.stats[row] = make_float2(st.x, inv);
     return;
   }
   const unsigned w = blockIdx.x - joins;
   const int* c = a.chunks + (size_t)kChunkInts * (w / kvh);
-  const int kh = w % kvh;
-  const int t = c[0], key0 = c[1], key1 = c[2], first_page = c[3], len = c[4], col = c[5];
-  const long long pitch = (len + kKeys - 1) / kKeys * kKeys;
-  const float* srow = a.scores + (long long)col * a.nq + kh * G * pitch;
-  for (int g = warp; g < G; g += 4) {
-    const int list = t * a.head_chunks + g / kRowUnitRows;
-    const float2 st = join_stats(a, a.merge_off[list], a.merge_off[list + 1], kh, g, lane);
-    if (lane == 0) {
-      sh_m[g] = st.x;
-      sh_l[g] = 1.f / st.y;
+  const int kh = w % kvh, t = __ldg(c);
+  if (warp < 4)
+    for (int g = warp; g < G; g += 4) {
+      const int list = t * a.head_chunks + g / kRowUnitRows;
+      const int e0 = __ldg(a.merge_off + list), e1 = __ldg(a.merge_off + list + 1);
+      float2 st = make_float2(-INFINITY, 0.f);
+      for (int e = e0 + lane; e < e1; e += 32) {
+        const int2 p = __ldg(a.merge + e);
+        if (e == e0 + lane && g == warp) pdl_wait();
+        st = join2(st, __ldcg(a.part_ml + part_row(p, kh, g)));
+      }
+      st = warp_join(st);
+      if (lane == 0) {
+        sh_m[g] = st.x;
+        sh_l[g] = 1.f / st.y;
+      }
     }
+  pdl_wait();
+  __syncthreads();
+  if (threadIdx.x < kJoinThreads) add_weights(a, c, kh, sh_m, sh_l);
+}
+
+// Weights of plans with many parts: a block per (chunk of keys, KV head),
+// with the statistics that join_kernel kept.
+__global__ void __launch_bounds__(kJoinThreads, 8) weights_kernel(CachedAttn a) {
+  __shared__ float sh_m[128], sh_l[128];
+  const int kvh = a.g.kvh, G = a.nq / kvh;
+  const int* c = a.chunks + (size_t)kChunkInts * (blockIdx.x / kvh);
+  const int kh = blockIdx.x % kvh, t = __ldg(c);
+  pdl_wait();
+  if (threadIdx.x < G) {
+    const float2 st = __ldcg(a.stats + (long long)t * a.nq + kh * G + threadIdx.x);
+    sh_m[threadIdx.x] = st.x;
+    sh_l[threadIdx.x] = st.y;
   }
   __syncthreads();
-  for (int key = key0 + threadIdx.x; key < key1; key += 128) {
-    float x = 0.f;
-#pragma unroll 4
-    for (int g = 0; g < G; ++g) x += ex2(__ldcg(srow + g * pitch + key) - sh_m[g]) * sh_l[g];
-    const int page = __ldg(a.pages + first_page + kv_page_col(a.g, key));
-    float* dst = a.weights + ((long long)page * kvh + kh) * a.g.block_size + kv_page_slot(a.g, key);
-    *dst += x;
-  }
+  add_weights(a, c, kh, sh_m, sh_l);
 }
 
 // Launch whose grid may start while the previous one of the stream ends.
@@ -418,16 +481,22 @@ void launch(const CachedAttn& a, const CUtensorMap* map, int type, cudaStream_t 
   if (tiles) cached_attention_tiles(a, *map, type, s);
   if (a.n_row_units > 0) a.scores ? launch_rows<T, HD, true>(a, tiles, s) : launch_rows<T, HD, false>(a, tiles, s);
   const long long rows = (long long)a.T * a.nq;
-  const unsigned extra = a.scores ? (unsigned)a.n_chunks * a.g.kvh : 0u;
-  // up to 32 parts a row fit one warp's lanes
+  // up to 32 parts fill one warp's lanes; rows of more take eight warps (their
+  // statistics are then kept for the weights: joining them again for every
+  // chunk of keys took longer than a launch)
   const bool wide = a.most_parts > 32;
   const unsigned joins = (unsigned)(wide ? rows : (rows + 3) / 4);
-  if (!tiles && a.n_row_units == 0)   // nothing before it: zeros only
-    launch_k(join_kernel<T, HD, 1>, dim3(joins + extra), dim3(128), 0, s, a, joins);
-  else if (wide)
-    launch_behind(join_kernel<T, HD, 4>, joins + extra, 128, 0, s, a, joins);
-  else
-    launch_behind(join_kernel<T, HD, 1>, joins + extra, 128, 0, s, a, joins);
+  const unsigned chunks = a.scores ? (unsigned)a.n_chunks * a.g.kvh : 0u;
+  if (!tiles && a.n_row_units == 0) {   // no part at all: zeros
+    launch_k(join_kernel<T, HD, 1>, dim3(joins), dim3(kJoinThreads), 0, s, a, joins);
+  } else if (!wide) {
+    CachedAttn b = a;
+    b.stats = nullptr;
+    launch_behind(join_kernel<T, HD, 1>, joins + chunks, kJoinThreads, 0, s, b, joins);
+  } else {
+    launch_behind(join_kernel<T, HD, 8>, joins, 256, 0, s, a, joins);
+    if (chunks) launch_behind(weights_kernel, chunks, kJoinThreads, 0, s, a);
+  }
 }
 
 }  // namespace cat

@@ -78,6 +78,7 @@ struct CachedAttn {
   // weighted plans: scores [request][nq][keys rounded up to 16] fp32, the
   // weights [pages, kvh, block_size] that each key's attention is added to
   float* scores;
+  float2* stats;                 // [T, nq] (max, 1 / sum) of weighted plans
   float* weights;
   const int* chunks;             // [n_chunks, kChunkInts]
   int n_chunks;
