@@ -11,7 +11,7 @@
 // gives zeros.  All statistics and partial sums are fp32.
 //
 // Row kernel: one warp per (unit, KV head), no barriers beyond the warp.
-// Stages of 16 keys (K and V rows, 16-byte cp.async, ends filled with zeros)
+// Stages of 32 keys (K and V rows, 16-byte cp.async, ends filled with zeros)
 // run through a ring in shared memory; S = Q K^T and O += P V are m16n8k16
 // tensor products with the unit's rows as M, so a key costs the same HBM
 // bytes for 1 to 16 rows: bound by HBM.
@@ -23,14 +23,14 @@ namespace kus {
 namespace cat {
 
 constexpr int kWarps = 1;
-constexpr int kKeys = 16;       // keys per stage
+constexpr int kKeys = 32;       // keys per stage
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int HD>
 struct RowCfg {
   static constexpr int kTile = kKeys * HD * 2;        // K or V of a stage
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kStages = HD == 128 ? 3 : 6;   // 24 KB a warp
+  static constexpr int kStages = HD == 128 ? 2 : 4;   // 32 KB a warp
   static constexpr int kSmem = kWarps * kStages * kStage;
 };
 
@@ -91,8 +91,9 @@ KUS_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
 }
 
 // `second`: launched behind the tile kernel of the same call, whose results it
-// does not need: it starts beside it, and only ends after it, so that the join
-// (which waits for this kernel) finds both done.
+// does not need: it starts beside it, and its first block only ends after it,
+// so that the join (which waits for this kernel) finds both done.  (A block
+// that waits keeps its place on the SM: the others leave it to the next.)
 template <typename T, int HD, bool SCORES>
 __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float scale_log2, bool second) {
   using Cf = RowCfg<HD>;
@@ -105,10 +106,7 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float s
   if (!second) pdl_wait();
   pdl_trigger();
   const int item = blockIdx.x * kWarps + warp;
-  if (item >= a.n_row_units * kvh) {
-    if (second) pdl_wait();
-    return;
-  }
+  if (item >= a.n_row_units * kvh) return;
   const int u = item / kvh, kh = item - u * kvh;   // heads fastest: neighbours read the same cache rows
   const int4 u0 = __ldg(reinterpret_cast<const int4*>(a.row_units) + 2 * u);
   const int4 u1 = __ldg(reinterpret_cast<const int4*>(a.row_units) + 2 * u + 1);
@@ -120,16 +118,16 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float s
   const int nst = (key_hi - key_lo + kKeys - 1) / kKeys;
   const long long layer_elems = a.g.layer_stride / (int)sizeof(T);
 
-  // keys: lane l (and l + 16) looks up stage key l's page one stage ahead
+  // keys: lane l looks up stage key l's page one stage ahead
   auto page_of = [&](int i) {
-    const int key = key_lo + i * kKeys + (lane & 15);
+    const int key = key_lo + i * kKeys + lane;
     return key < key_hi ? __ldg(table + kv_page_col(a.g, key)) : -1;
   };
   int page = page_of(0);
   auto load = [&](int i) {
     long long off = -1;
     if (page >= 0) {
-      const int key = key_lo + i * kKeys + (lane & 15);
+      const int key = key_lo + i * kKeys + lane;
       off = kv_slot(a.g, page, a.layer) * layer_elems + ((long long)kv_page_slot(a.g, key) * kvh + kh) * HD;
     }
     page = page_of(i + 1);
@@ -188,23 +186,26 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float s
     cp_wait<kStages - 1>();
     __syncwarp();
     const uint32_t kt = ring + (i % kStages) * Cf::kStage, vt = kt + Cf::kTile;
-    float s[2][4] = {};
+    constexpr int kNT = kKeys / 8;
+    float s[kNT][4] = {};
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) {
-      uint32_t b0, b1, b2, b3;
-      ldsm4(kt + swz<HD>(((lane >> 4) << 3) + (lane & 7), ks * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
-      mma<T>(s[0], qf[ks], b0, b1);
-      mma<T>(s[1], qf[ks], b2, b3);
-    }
+    for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+      for (int kb = 0; kb < kKeys / 16; ++kb) {
+        uint32_t b0, b1, b2, b3;
+        ldsm4(kt + swz<HD>(kb * 16 + ((lane >> 4) << 3) + (lane & 7), ks * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
+        mma<T>(s[2 * kb], qf[ks], b0, b1);
+        mma<T>(s[2 * kb + 1], qf[ks], b2, b3);
+      }
     const int key = key_lo + i * kKeys + 2 * (lane & 3);
-    uint32_t ph[4], pl[4];
+    uint32_t ph[kKeys / 16][4], pl[kKeys / 16][4];
     float alpha[2];
 #pragma unroll
     for (int hi = 0; hi < 2; ++hi) {
       const int end = min(key_hi, lim[hi]);
       float mx = -INFINITY;
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+      for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float& x = s[nt][2 * hi + e];
@@ -213,8 +214,9 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float s
         }
       if (SCORES && r_lo + 8 * hi < rows) {
         float* dst = srow + (r_lo + 8 * hi) * spitch + key;
-        *reinterpret_cast<float2*>(dst) = make_float2(s[0][2 * hi], s[0][2 * hi + 1]);
-        *reinterpret_cast<float2*>(dst + 8) = make_float2(s[1][2 * hi], s[1][2 * hi + 1]);
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+          *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(s[nt][2 * hi], s[nt][2 * hi + 1]);
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -224,29 +226,33 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float s
       m[hi] = mn;
       float sum = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
+      for (int nt = 0; nt < kNT; ++nt) {
         const float p0 = ex2(s[nt][2 * hi] - ref), p1 = ex2(s[nt][2 * hi + 1] - ref);
         sum += p0 + p1;
-        split2<T>(p0, p1, ph[2 * nt + hi], pl[2 * nt + hi]);
+        split2<T>(p0, p1, ph[nt / 2][2 * (nt & 1) + hi], pl[nt / 2][2 * (nt & 1) + hi]);
       }
       l[hi] = l[hi] * alpha[hi] + sum;
     }
+    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {   // some row's max grew
 #pragma unroll
-    for (int d = 0; d < HD / 8; ++d) {
-      o[d][0] *= alpha[0];
-      o[d][1] *= alpha[0];
-      o[d][2] *= alpha[1];
-      o[d][3] *= alpha[1];
+      for (int d = 0; d < HD / 8; ++d) {
+        o[d][0] *= alpha[0];
+        o[d][1] *= alpha[0];
+        o[d][2] *= alpha[1];
+        o[d][3] *= alpha[1];
+      }
     }
 #pragma unroll
-    for (int d = 0; d < HD / 16; ++d) {
-      uint32_t b0, b1, b2, b3;
-      ldsm4_t(vt + swz<HD>((lane & 7) + (((lane >> 3) & 1) << 3), d * 2 + (lane >> 4)), b0, b1, b2, b3);
-      mma<T>(o[2 * d], ph, b0, b1);
-      mma<T>(o[2 * d + 1], ph, b2, b3);
-      mma<T>(o[2 * d], pl, b0, b1);
-      mma<T>(o[2 * d + 1], pl, b2, b3);
-    }
+    for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+      for (int kb = 0; kb < kKeys / 16; ++kb) {
+        uint32_t b0, b1, b2, b3;
+        ldsm4_t(vt + swz<HD>(kb * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), d * 2 + (lane >> 4)), b0, b1, b2, b3);
+        mma<T>(o[2 * d], ph[kb], b0, b1);
+        mma<T>(o[2 * d + 1], ph[kb], b2, b3);
+        mma<T>(o[2 * d], pl[kb], b0, b1);
+        mma<T>(o[2 * d + 1], pl[kb], b2, b3);
+      }
     __syncwarp();   // the slot is refilled in the next iteration
   }
   cp_wait<0>();
@@ -265,7 +271,7 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float s
       *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * hi], o[d][2 * hi + 1]);
     if ((lane & 3) == 0) a.part_ml[prow] = make_float2(m[hi], sum);
   }
-  if (second) pdl_wait();
+  if (second && blockIdx.x == 0) pdl_wait();
 }
 
 // ------------------------------------------------------------------ joins

@@ -2,8 +2,8 @@
 // query rows, the queries of many requests behind one shared prefix (or a
 // long chunk of one request), on the sm_100a tensor cores.
 //
-// One CTA takes one (unit, KV head): its rows against blocks of 128 keys,
-// S = Q K^T and O += P V by tcgen05.mma with S, P and O in TMEM.
+// A CTA takes (unit, KV head) pairs in turn: the unit's rows against blocks
+// of 128 keys, S = Q K^T and O += P V by tcgen05.mma with S, P and O in TMEM.
 //
 //   warps 0-7  softmax: two threads a row (TMEM lane r), 64 of the block's
 //              scores each in registers; the probabilities go as 16-bit
@@ -13,6 +13,8 @@
 //   warp 10    issues QK (and owns TMEM), warp 11 issues PV: a thread that issues
 //              one product waits for most of it, which would hold the other up
 //
+// The grid is persistent and every role counts blocks over the CTA's units,
+// so the loads of a unit's first blocks run beside the end of the one before.
 // S and P have two buffers each (with O all 512 TMEM columns, one CTA an SM):
 // QK(i + 1) and PV(i - 1) run while block i's softmax does, which is what
 // bounds an iteration.  Blocks of 128 keys and not 64: the tensor core reads
@@ -29,6 +31,7 @@
 #include "cache_elem.cuh"
 #include "cache_ops.h"
 #include <cudaTypedefs.h>
+#include <algorithm>
 
 namespace kus {
 namespace gemm_impl {
@@ -160,6 +163,30 @@ KUS_HOST_DEVICE constexpr uint32_t idesc(int N, bool b_mn) {
          ((uint32_t)(kRows >> 4) << 24);
 }
 
+// What a unit record says (cache_ops.h), for one KV head.
+struct Unit {
+  int kh, tok0, ntok, ng, g0, key_lo, key_hi, lim0, page0, part0, nb;
+};
+KUS_DEVICE Unit unit_at(const CachedAttn& a, int item) {
+  // heads vary fastest: CTAs of one unit read the same cache rows together
+  const int u = item / a.g.kvh;
+  const int4 u0 = __ldg(reinterpret_cast<const int4*>(a.tile_units) + 2 * u);
+  const int4 u1 = __ldg(reinterpret_cast<const int4*>(a.tile_units) + 2 * u + 1);
+  Unit r;
+  r.kh = item - u * a.g.kvh;
+  r.tok0 = u0.x;
+  r.ntok = u0.y & 255;
+  r.ng = (u0.y >> 8) & 255;
+  r.g0 = u0.y >> 16;
+  r.key_lo = u0.z;
+  r.key_hi = u0.w;
+  r.lim0 = u1.x;
+  r.page0 = u1.y;
+  r.part0 = u1.z;
+  r.nb = (r.key_hi - r.key_lo + kKeys - 1) / kKeys;
+  return r;
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map, CachedAttn a,
                                                            int box, float scale_log2) {
@@ -169,15 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   const uint32_t sbase = smem_u32(smem);
   Bars<HD>* bars = reinterpret_cast<Bars<HD>*>(smem + Cf::kBarOff);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int kvh = a.g.kvh, G = a.nq / kvh;
-  // heads vary fastest: the CTAs of one unit read the same cache rows together
-  const int unit = blockIdx.x / kvh, kh = blockIdx.x - unit * kvh;
-  const int4 u0 = __ldg(reinterpret_cast<const int4*>(a.tile_units) + 2 * unit);
-  const int4 u1 = __ldg(reinterpret_cast<const int4*>(a.tile_units) + 2 * unit + 1);
-  const int tok0 = u0.x, ntok = u0.y & 255, ng = (u0.y >> 8) & 255, g0 = u0.y >> 16;
-  const int key_lo = u0.z, key_hi = u0.w, lim0 = u1.x;
-  const int rows = ntok * ng;
-  const int nb = (key_hi - key_lo + kKeys - 1) / kKeys;
+  const int G = a.nq / a.g.kvh, n_items = a.n_tile_units * a.g.kvh;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, kSoftmax);
@@ -209,71 +228,79 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     // ----------------------------------------------------------- producers
     const bool is_v = warp == 9;
     const int stages = is_v ? Cf::kVStages : Cf::kKStages;
-    const int* table = a.pages + u1.y;
     uint64_t* full = is_v ? bars->v_full : bars->k_full;
     uint64_t* empty = is_v ? bars->v_empty : bars->k_empty;
     const uint32_t region = sbase + (is_v ? Cf::kVOff : Cf::kKOff);
     if (lane == 0) prefetch_tmap(&map);
-    // tensor map row of this lane's box of block i (-1: past the keys)
-    auto row_of = [&](int i) {
-      const int key = key_lo + i * kKeys + lane * box;
-      if (lane * box >= kKeys || key >= key_hi) return -1;
-      return kv_slot(a.g, __ldg(table + kv_page_col(a.g, key)), a.layer) * 2 * a.g.block_size +
-             (is_v ? a.g.block_size : 0) + kv_page_slot(a.g, key);
-    };
-    int row = row_of(0), s = 0;
+    int s = 0, loaded = 0;
     uint32_t ph = 1;
     bool ok = true;
-    for (int i = 0; i < nb; ++i) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph, kErrWaitEmpty));
-      if (!ok) break;
-      const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, row >= 0));
-      if (lane == 0) mbar_arrive_expect_tx(&full[s], boxes * box * HD * 2);
-      __syncwarp();
-      if (row >= 0) {
-        const uint32_t dst = region + s * Cf::kTile + lane * box * 128;
+    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+      const Unit un = unit_at(a, item);
+      const int* table = a.pages + un.page0;
+      // tensor map row of this lane's box of block i (-1: past the keys)
+      auto row_of = [&](int i) {
+        const int key = un.key_lo + i * kKeys + lane * box;
+        if (lane * box >= kKeys || key >= un.key_hi) return -1;
+        return kv_slot(a.g, __ldg(table + kv_page_col(a.g, key)), a.layer) * 2 * a.g.block_size +
+               (is_v ? a.g.block_size : 0) + kv_page_slot(a.g, key);
+      };
+      int row = row_of(0);
+      for (int i = 0; i < un.nb; ++i) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph, kErrWaitEmpty));
+        if (!ok) break;
+        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, row >= 0));
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], boxes * box * HD * 2);
+        __syncwarp();
+        if (row >= 0) {
+          const uint32_t dst = region + s * Cf::kTile + lane * box * 128;
 #pragma unroll
-        for (int h = 0; h < Cf::kHalves; ++h) tma_load_3d(dst + h * Cf::kHalf, &map, &full[s], 64 * h, kh, row);
-      }
-      row = row_of(i + 1);
-      if (++s == stages) {
-        s = 0;
-        ph ^= 1;
+          for (int h = 0; h < Cf::kHalves; ++h) tma_load_3d(dst + h * Cf::kHalf, &map, &full[s], 64 * h, un.kh, row);
+        }
+        row = row_of(i + 1);
+        ++loaded;
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1;
+        }
       }
     }
     // every load has landed before the CTA may leave
-    if (ok)
-      for (int i = max(0, nb - stages); i < nb; ++i)
-        mbar_wait(&full[i % stages], (uint32_t)(i / stages) & 1u, kErrWaitFull);
+    for (int i = max(0, loaded - stages); i < loaded; ++i)
+      mbar_wait(&full[i % stages], (uint32_t)(i / stages) & 1u, kErrWaitFull);
     __syncwarp();
   } else if (warp == 10) {
     // ------------------------------------------------------- S = Q K^T
     if (lane == 0) {
       constexpr uint32_t id_qk = idesc<T>(kKeys, false);
-      bool ok = mbar_wait(&bars->q_full, 0, kErrWaitFull);
-      int s = 0;
-      uint32_t ph = 0;
-      for (int i = 0; i < nb && ok; ++i) {
-        const int b = i & 1;
-        ok = mbar_wait(&bars->k_full[s], ph, kErrWaitFull);
-        // the scores of block i - 2 are read, and its probabilities: S(i) full
-        // tells the softmax that both buffers are free
-        const uint32_t before = (uint32_t)((i >> 1) - 1) & 1u;
-        if (i >= 2)
-          ok = ok && mbar_wait(&bars->s_empty[b], before, kErrWaitTmemEmpty) &&
-               mbar_wait(&bars->pv_done[b], before, kErrWaitTmemEmpty);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t qd = umma_desc_sw128(sbase), kd = umma_desc_sw128(sbase + Cf::kKOff + s * Cf::kTile);
+      bool ok = true;
+      int s = 0, g = 0;   // stage, blocks so far
+      uint32_t ph = 0, q_ph = 0;
+      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, q_ph ^= 1) {
+        const int nb = unit_at(a, item).nb;
+        ok = mbar_wait(&bars->q_full, q_ph, kErrWaitFull);
+        for (int i = 0; i < nb && ok; ++i, ++g) {
+          const int b = g & 1;
+          ok = mbar_wait(&bars->k_full[s], ph, kErrWaitFull);
+          // the scores of block g - 2 are read, and its probabilities: S(g)
+          // full tells the softmax that both buffers are free
+          const uint32_t before = (uint32_t)((g >> 1) - 1) & 1u;
+          if (g >= 2)
+            ok = ok && mbar_wait(&bars->s_empty[b], before, kErrWaitTmemEmpty) &&
+                 mbar_wait(&bars->pv_done[b], before, kErrWaitTmemEmpty);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t qd = umma_desc_sw128(sbase), kd = umma_desc_sw128(sbase + Cf::kKOff + s * Cf::kTile);
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          umma_f16(tmem + b * kKeys, qd + (uint64_t)(((kk >> 2) * Cf::kQHalf >> 4) + 2 * (kk & 3)),
-                   kd + (uint64_t)(((kk >> 2) * Cf::kHalf >> 4) + 2 * (kk & 3)), id_qk, kk > 0 ? 1u : 0u);
-        umma_commit(&bars->s_full[b]);
-        umma_commit(&bars->k_empty[s]);
-        if (++s == Cf::kKStages) {
-          s = 0;
-          ph ^= 1;
+          for (int kk = 0; kk < HD / 16; ++kk)
+            umma_f16(tmem + b * kKeys, qd + (uint64_t)(((kk >> 2) * Cf::kQHalf >> 4) + 2 * (kk & 3)),
+                     kd + (uint64_t)(((kk >> 2) * Cf::kHalf >> 4) + 2 * (kk & 3)), id_qk, kk > 0 ? 1u : 0u);
+          umma_commit(&bars->s_full[b]);
+          umma_commit(&bars->k_empty[s]);
+          if (++s == Cf::kKStages) {
+            s = 0;
+            ph ^= 1;
+          }
         }
       }
     }
@@ -282,166 +309,175 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     // ------------------------------------------------------- O += P V
     constexpr uint32_t id_pv = idesc<T>(HD, true);
     bool ok = true;
-    int s = 0;
+    int s = 0, g = 0;
     uint32_t ph = 0;
-    for (int i = 0; i < nb; ++i) {
-      const int b = i & 1;
-      ok = mbar_wait(&bars->v_full[s], ph, kErrWaitFull);
-      const int have = key_hi - (key_lo + i * kKeys);
-      if (have < kKeys) {
-        // rows past the keys: the loaded boxes' stale slots and what was not loaded
-        uint8_t* vt = smem + Cf::kVOff + s * Cf::kTile;
-        for (int c = lane; c < (kKeys - have) * 8; c += 32)
+    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+      const Unit un = unit_at(a, item);
+      for (int i = 0; i < un.nb; ++i, ++g) {
+        const int b = g & 1;
+        ok = mbar_wait(&bars->v_full[s], ph, kErrWaitFull);
+        const int have = un.key_hi - (un.key_lo + i * kKeys);
+        if (have < kKeys) {
+          // rows past the keys: the loaded boxes' stale slots and what was not loaded
+          uint8_t* vt = smem + Cf::kVOff + s * Cf::kTile;
+          for (int c = lane; c < (kKeys - have) * 8; c += 32)
 #pragma unroll
-          for (int h = 0; h < Cf::kHalves; ++h)
-            *reinterpret_cast<uint4*>(vt + h * Cf::kHalf + have * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            for (int h = 0; h < Cf::kHalves; ++h)
+              *reinterpret_cast<uint4*>(vt + h * Cf::kHalf + have * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->p_full[b], (uint32_t)(g >> 1) & 1u, kErrWaitFull));
+        if (!ok) break;
+        if (lane == 0) {
+          tc_fence_after();
+          const uint64_t vd = v_desc(sbase + Cf::kVOff + s * Cf::kTile, Cf::kHalf);
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            umma_f16_ta(tmem + kColO, tmem + kColP + b * (kKeys / 2) + kk * 8, vd + (uint64_t)(kk * 16 * 128 >> 4),
+                        id_pv, (i > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&bars->pv_done[b]);
+          umma_commit(&bars->v_empty[s]);
+        }
         __syncwarp();
-      }
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->p_full[b], (uint32_t)(i >> 1) & 1u, kErrWaitFull));
-      if (!ok) break;
-      if (lane == 0) {
-        tc_fence_after();
-        const uint64_t vd = v_desc(sbase + Cf::kVOff + s * Cf::kTile, Cf::kHalf);
-#pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-          umma_f16_ta(tmem + kColO, tmem + kColP + b * (kKeys / 2) + kk * 8, vd + (uint64_t)(kk * 16 * 128 >> 4), id_pv,
-                      (i > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&bars->pv_done[b]);
-        umma_commit(&bars->v_empty[s]);
-      }
-      __syncwarp();
-      if (++s == Cf::kVStages) {
-        s = 0;
-        ph ^= 1;
+        if (++s == Cf::kVStages) {
+          s = 0;
+          ph ^= 1;
+        }
       }
     }
   } else {
     // --------------------------------------------------- Q, softmax, output
     const int half = warp >> 2, r = threadIdx.x & (kRows - 1);   // TMEM lane of warp w: 32 (w % 4) + lane
-    const bool valid = r < rows;
-    const int j = valid ? r / ng : 0, gi = valid ? r - j * ng : 0;
-    {
-      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (tok0 + j) * a.qt +
-                                                        (long long)(kh * G + g0 + gi) * a.qh);
-      constexpr int kEach = HD / 16;   // 16-byte chunks of a thread
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int c = half * kEach + e;
-        const uint4 v = valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(smem + (c >> 3) * Cf::kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(&bars->q_full);
-    }
-    const int end = min(key_hi, lim0 + j);       // keys this row sees
-    const int end_min = min(key_hi, lim0);       // and every row sees
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t t_o = tl + kColO + half * (HD / 2);
     float* maxima = reinterpret_cast<float*>(smem + Cf::kMaxOff);
-    float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int i = 0; i < nb; ++i) {
-      const int b = i & 1;
-      const uint32_t t_s = tl + b * kKeys + half * 64, t_p = tl + kColP + b * (kKeys / 2) + half * 32;
-      ok = ok && mbar_wait(&bars->s_full[b], (uint32_t)(i >> 1) & 1u, kErrWaitTmemFull);
+    int g = 0;   // blocks so far
+    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+      const Unit un = unit_at(a, item);
+      const int rows = un.ntok * un.ng;
+      const bool valid = r < rows;
+      const int j = valid ? r / un.ng : 0, gi = valid ? r - j * un.ng : 0;
+      {
+        // every product with the Q before is done: its last scores were read
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (un.tok0 + j) * a.qt +
+                                                          (long long)(un.kh * G + un.g0 + gi) * a.qh);
+        constexpr int kEach = HD / 16;   // 16-byte chunks of a thread
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const int c = half * kEach + e;
+          const uint4 v = valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(smem + (c >> 3) * Cf::kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&bars->q_full);
+      }
+      const int end = min(un.key_hi, un.lim0 + j);       // keys this row sees
+      const int end_min = min(un.key_hi, un.lim0);       // and every row sees
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < un.nb; ++i, ++g) {
+        const int b = g & 1;
+        const uint32_t t_s = tl + b * kKeys + half * 64, t_p = tl + kColP + b * (kKeys / 2) + half * 32;
+        ok = ok && mbar_wait(&bars->s_full[b], (uint32_t)(g >> 1) & 1u, kErrWaitTmemFull);
+        __syncwarp();
+        tc_fence_after();
+        const int key0 = un.key_lo + i * kKeys;
+        uint32_t v[64];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld(t_s + kChunk * c, v + kChunk * c);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_wait_ld(v + kChunk * c);
+        tc_fence_before();
+        mbar_arrive(&bars->s_empty[b]);
+        if (key0 + kKeys > end_min) {
+          const int left = end - key0 - half * 64;   // of this thread's keys, those its row sees
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (e >= left) v[e] = 0xff800000u;   // -inf
+        }
+        // Probabilities against the max so far, the block's own max beside
+        // them: it is only seldom needed, and the exponentials bound this loop.
+        uint32_t pk[32];
+        float sum;
+        float mx[2] = {-INFINITY, -INFINITY};
+        auto probabilities = [&](float ref) {
+          const float2 scale2 = make_float2(scale_log2, scale_log2), ref2 = make_float2(-ref, -ref);
+          float2 acc[2] = {};
+#pragma unroll
+          for (int e = 0; e < 64; e += 2) {
+            const float2 x = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2, ref2);
+            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+            acc[(e / 2) & 1] = add2(acc[(e / 2) & 1], p);
+            pk[e / 2] = pack2<T>(p.x, p.y);
+          }
+          sum = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+        };
+        probabilities(m == -INFINITY ? 0.f : m);
+#pragma unroll
+        for (int e = 0; e < 64; e += 4) {
+          mx[0] = max3(mx[0], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+          mx[1] = max3(mx[1], __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+        }
+        const float top = fmaxf(mx[0], mx[1]) * scale_log2;
+        if (barrier_any(1 + (warp & 3), 64, top > m + kRescaleLog2)) {
+          // some row of this pair of warps outgrew its max
+          float* mine = maxima + r;
+          mine[half * kRows] = top;
+          named_barrier(1 + (warp & 3), 64);
+          const float both = fmaxf(top, mine[(half ^ 1) * kRows]);
+          const bool grow = both > m + kRescaleLog2;
+          const float mn = grow ? both : m;
+          const float alpha = grow ? ex2(m - mn) : 1.f;
+          probabilities(mn == -INFINITY ? 0.f : mn);   // no key seen yet: zeros
+          if (i > 0) {
+            // PV of the block before is done: O is stable
+            ok = ok && mbar_wait(&bars->pv_done[b ^ 1], (uint32_t)((g - 1) >> 1) & 1u, kErrWaitTmemFull);
+            __syncwarp();
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD / 2 / kChunk; ++c) {
+              uint32_t o[kChunk];
+              tmem_ld(t_o + kChunk * c, o);
+              tmem_wait_ld(o);
+#pragma unroll
+              for (int e = 0; e < kChunk; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st(t_o + kChunk * c, o);
+            }
+          }
+          l *= alpha;
+          m = mn;
+        }
+        tmem_st(t_p, pk);
+        tmem_st(t_p + kChunk, pk + kChunk);
+        l += sum;
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars->p_full[b]);
+      }
+      // the halves' sums (m is the same in both)
+      named_barrier(1 + (warp & 3), 64);
+      float* mine = maxima + r;
+      mine[half * kRows] = l;
+      named_barrier(1 + (warp & 3), 64);
+      l += mine[(half ^ 1) * kRows];
+      ok = ok && mbar_wait(&bars->pv_done[(g - 1) & 1], (uint32_t)((g - 1) >> 1) & 1u, kErrWaitTmemFull);
       __syncwarp();
       tc_fence_after();
-      const int key0 = key_lo + i * kKeys;
-      uint32_t v[64];
+      const long long prow = un.part0 + (long long)un.kh * rows + r;
+      float* dst = a.part_o + prow * HD + half * (HD / 2);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld(t_s + kChunk * c, v + kChunk * c);
+      for (int c = 0; c < HD / 2 / kChunk; ++c) {
+        uint32_t o[kChunk];
+        tmem_ld(t_o + kChunk * c, o);
+        tmem_wait_ld(o);
+        if (valid)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_wait_ld(v + kChunk * c);
-      tc_fence_before();
-      mbar_arrive(&bars->s_empty[b]);
-      if (key0 + kKeys > end_min) {
-        const int left = end - key0 - half * 64;   // of this thread's keys, those its row sees
-#pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (e >= left) v[e] = 0xff800000u;   // -inf
+          for (int e = 0; e < kChunk; e += 4)
+            *reinterpret_cast<uint4*>(dst + kChunk * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
       }
-      // Probabilities against the max so far, the block's own max beside
-      // them: it is only seldom needed, and the exponentials bound this loop.
-      uint32_t pk[32];
-      float sum;
-      float mx[2] = {-INFINITY, -INFINITY};
-      auto probabilities = [&](float ref) {
-        const float2 scale2 = make_float2(scale_log2, scale_log2), ref2 = make_float2(-ref, -ref);
-        float2 acc[2] = {};
-#pragma unroll
-        for (int e = 0; e < 64; e += 2) {
-          const float2 x = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2, ref2);
-          const float2 p = make_float2(ex2(x.x), ex2(x.y));
-          acc[(e / 2) & 1] = add2(acc[(e / 2) & 1], p);
-          pk[e / 2] = pack2<T>(p.x, p.y);
-        }
-        sum = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
-      };
-      probabilities(m == -INFINITY ? 0.f : m);
-#pragma unroll
-      for (int e = 0; e < 64; e += 4) {
-        mx[0] = max3(mx[0], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-        mx[1] = max3(mx[1], __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
-      }
-      const float top = fmaxf(mx[0], mx[1]) * scale_log2;
-      if (barrier_any(1 + (warp & 3), 64, top > m + kRescaleLog2)) {
-        // some row of this pair of warps outgrew its max
-        float* mine = maxima + r;
-        mine[half * kRows] = top;
-        named_barrier(1 + (warp & 3), 64);
-        const float both = fmaxf(top, mine[(half ^ 1) * kRows]);
-        const bool grow = both > m + kRescaleLog2;
-        const float mn = grow ? both : m;
-        const float alpha = grow ? ex2(m - mn) : 1.f;
-        probabilities(mn == -INFINITY ? 0.f : mn);   // no key seen yet: zeros
-        if (i > 0) {
-          // PV(i - 1) is done: O is stable
-          ok = ok && mbar_wait(&bars->pv_done[b ^ 1], (uint32_t)((i - 1) >> 1) & 1u, kErrWaitTmemFull);
-          __syncwarp();
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < HD / 2 / kChunk; ++c) {
-            uint32_t o[kChunk];
-            tmem_ld(t_o + kChunk * c, o);
-            tmem_wait_ld(o);
-#pragma unroll
-            for (int e = 0; e < kChunk; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st(t_o + kChunk * c, o);
-          }
-        }
-        l *= alpha;
-        m = mn;
-      }
-      tmem_st(t_p, pk);
-      tmem_st(t_p + kChunk, pk + kChunk);
-      l += sum;
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&bars->p_full[b]);
+      if (valid && half == 0) a.part_ml[prow] = make_float2(m, l);
     }
-    // the halves' sums (m is the same in both)
-    named_barrier(1 + (warp & 3), 64);
-    float* mine = maxima + r;
-    mine[half * kRows] = l;
-    named_barrier(1 + (warp & 3), 64);
-    l += mine[(half ^ 1) * kRows];
-    ok = ok && mbar_wait(&bars->pv_done[(nb - 1) & 1], (uint32_t)((nb - 1) >> 1) & 1u, kErrWaitTmemFull);
-    __syncwarp();
-    tc_fence_after();
-    const long long prow = u1.z + (long long)kh * rows + r;
-    float* dst = a.part_o + prow * HD + half * (HD / 2);
-#pragma unroll
-    for (int c = 0; c < HD / 2 / kChunk; ++c) {
-      uint32_t o[kChunk];
-      tmem_ld(t_o + kChunk * c, o);
-      tmem_wait_ld(o);
-      if (valid)
-#pragma unroll
-        for (int e = 0; e < kChunk; e += 4)
-          *reinterpret_cast<uint4*>(dst + kChunk * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-    }
-    if (valid && half == 0) a.part_ml[prow] = make_float2(m, l);
   }
   tc_fence_before();
   __syncthreads();
@@ -451,7 +487,11 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 template <typename T, int HD>
 void launch(const CachedAttn& a, const CUtensorMap& map, int box, cudaStream_t s) {
   ensure_smem_attr(reinterpret_cast<const void*>(tile_kernel<T, HD>), Cfg<HD>::kSmem);
-  launch_k(tile_kernel<T, HD>, dim3((unsigned)a.n_tile_units * a.g.kvh), dim3(kThreads), Cfg<HD>::kSmem, s, map, a, box,
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const unsigned grid = (unsigned)std::min<long long>(sms, (long long)a.n_tile_units * a.g.kvh);
+  launch_k(tile_kernel<T, HD>, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, map, a, box,
            a.scale * 1.4426950408889634f);
 }
 

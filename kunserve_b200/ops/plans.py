@@ -13,18 +13,18 @@ import numpy as np
 
 UNIT_INTS = 8
 ROW_UNIT_ROWS = 16
-STAGE_KEYS = 16          # keys per stage of the row kernel
+STAGE_KEYS = 32          # keys per stage of the row kernel
 TILE_UNIT_ROWS = 128
 TILE_KEYS = 128          # keys per block of the tile kernel
 TILE_MIN_ROWS = 17       # fewest query rows (tokens x group heads) the tile kernel takes
 CHUNK_KEYS = 512         # keys per block that adds up weights
 NO_LIMIT = 1 << 30
-ROW_SLOTS = 9            # warps of the row kernel an SM holds
-ROW_MIN_STAGES = 4       # shortest range of a row unit, in stages
-ROW_WAVES = 4            # units a slot takes, at least, when there is work for more than one
+ROW_SLOTS = 6            # warps of the row kernel an SM takes at once
+ROW_MIN_STAGES = 2       # shortest range of a row unit, in stages
+ROW_START = 1            # what starting and ending a unit takes, in stages
 TILE_SLOTS = 1           # CTAs of the tile kernel an SM holds
 TILE_MIN_BLOCKS = 2      # shortest range of a tile unit, in blocks
-TILE_START = 3           # what starting and ending a unit takes, in blocks
+TILE_START = 2           # what starting and ending a unit takes, in blocks
 
 
 class Span(NamedTuple):
@@ -60,26 +60,33 @@ def _parts(stages: np.ndarray, share: int) -> np.ndarray:
     return -(-stages // np.maximum(-(-stages // np.maximum(parts, 1)), 1))   # no empty range at the end
 
 
-def _cut(tiles: np.ndarray, kv_heads: int, slots: int, stage: int, min_stages: int, waves: int) -> np.ndarray:
-    """Cut the tiles' keys into ranges: columns of the tile, then first key
-    and end of the range.
+def _cut(tiles: np.ndarray, kv_heads: int, slots: int, stage: int, least: int, start: float) -> np.ndarray:
+    """Cut the tiles' keys into equal ranges: columns of the tile, then first
+    key and end of the range.
 
-    Up to ``waves`` slots' worth of units a slot, the range is the one whose
-    waves of units (each as long as its longest, and a start's worth of
-    stages more) take least; beyond that the hardware evens units out, and
-    the range is a slot's share over ``waves``."""
+    Of a few dozen range lengths the one that takes least is used, in stages:
+    units that all start at once take as long as the longest; more of them
+    take a slot's share of all, and the longest once more at the end.  A unit
+    costs ``start`` stages and an eighth of one per row (its partial sums)
+    besides its keys; each part of a row costs the join 1/32."""
+    if not len(tiles):
+        return np.zeros((0, 10), dtype=np.int64)
     stages = -(-tiles[:, 4] // stage)
-    total = int(stages.sum()) * kv_heads
-    share = max(min_stages, -(-total // (slots * waves)))
-    if len(tiles) and waves == 1:
-        most = int(stages.max())
-        tries = sorted({max(min_stages, -(-most // k)) for k in range(1, 65)} | {share})
-        def cost(c):
-            parts = _parts(stages, c)
-            return -(-int(parts.sum()) * kv_heads // slots) * (int((-(-stages // parts)).max()) + TILE_START)
-        share = min(tries, key=cost)
-    parts = _parts(stages, share)
-    each = -(-stages // np.maximum(parts, 1))
+    most, total = int(stages.max()), int(stages.sum()) * kv_heads
+    extra = start + tiles[:, 1] * tiles[:, 2] / 8.0 * STAGE_KEYS / stage
+    tries = {-(-most // k) for k in range(1, 49)} | {-(-total * k // (slots * 8)) for k in range(1, 17)}
+    best = None
+    for c in sorted({max(least, t) for t in tries}):
+        parts = _parts(stages, c)
+        each = -(-stages // parts) + extra
+        n = int(parts.sum()) * kv_heads
+        cost = float(each.max()) + int(parts.max()) / 32.0
+        if n > slots:
+            cost += float((each * parts).sum()) * kv_heads / slots
+        if best is None or cost < best[0]:
+            best = (cost, parts)
+    parts = best[1]
+    each = -(-stages // parts)
     idx = np.repeat(np.arange(len(tiles)), parts)
     k = np.arange(len(idx)) - np.repeat(np.cumsum(parts) - parts, parts)
     lo = k * each[idx] * stage
@@ -99,9 +106,9 @@ def build(spans: Sequence[Span], pages: np.ndarray, tokens: int, num_q_heads: in
         raise ValueError(f"at most 128 query heads per KV head, got {group}")
     many = [tiles and s.tokens * group >= TILE_MIN_ROWS for s in spans]
     rows = _cut(_row_tiles([s for s, m in zip(spans, many) if not m], group, ROW_UNIT_ROWS), kv_heads,
-                sms * ROW_SLOTS, STAGE_KEYS, ROW_MIN_STAGES, ROW_WAVES)
+                sms * ROW_SLOTS, STAGE_KEYS, ROW_MIN_STAGES, ROW_START)
     wide = _cut(_row_tiles([s for s, m in zip(spans, many) if m], group, TILE_UNIT_ROWS), kv_heads, sms * TILE_SLOTS,
-                TILE_KEYS, TILE_MIN_BLOCKS, 1)
+                TILE_KEYS, TILE_MIN_BLOCKS, TILE_START)
     head_chunks = -(-group // ROW_UNIT_ROWS)
 
     units = np.concatenate([rows, wide])
