@@ -339,6 +339,7 @@ void compact_cache_op(const PagedKV& kv, int64_t layer, const CachePlan& plan, c
   c10::cuda::CUDAGuard guard(kv.pool.device());
   CacheCompact a{};
   a.g = kv.g;
+  KUS_CHECK(kv.pool.numel() / kv.g.hd < (1LL << 31), "the pool has too many rows of head_dim ", kv.g.hd);
   a.layer = kv.checked_layer(layer);
   KUS_CHECK(moves.device() == kv.pool.device() && moves.scalar_type() == torch::kInt32 && moves.is_contiguous() &&
                   moves.dim() == 4 && moves.size(0) == plan.n_reqs && moves.size(1) == a.g.kvh && moves.size(3) == 2,

@@ -109,11 +109,12 @@ class DecodePlan:
         if reqs and not -2 ** 31 <= min(r[2] for r in reqs) <= max(r[2] for r in reqs) < 2 ** 31:
             raise ValueError("newest positions must fit 32 bits")
         self.lengths: List[int] = list(lengths)
+        self.longest = max(self.lengths, default=0)
         self.num_q_heads = int(num_q_heads)
         blob, table = plans.build(spans, np.array(pages, dtype=np.int64), len(spans), self.num_q_heads,
                                   kv.num_kv_heads, _sms(kv.pool.device.index), score_cols=cols)
         blob = plans.append_sections(blob, table, chunks=np.array(chunks), requests=np.array(reqs))
-        table.update(chunks=len(chunks), requests=len(reqs), most_tokens=max(self.lengths, default=0), score_cols=col)
+        table.update(chunks=len(chunks), requests=len(reqs), most_tokens=self.longest, score_cols=col)
         self._native = native().CachePlan(torch.from_numpy(blob), kv, table)
         self._kv = kv
 
@@ -141,8 +142,8 @@ def select_evictions(weights: torch.Tensor, slot_positions: torch.Tensor, plan: 
     the ``counts`` int32 [requests, kv heads].  Nothing is changed:
     ``compact_cache`` applies the moves, after which a request holds
     ``min(keep, length)`` tokens."""
-    cap = max([min(keep, n - keep) for n in plan.lengths], default=0)
-    return native().select_evictions(weights, slot_positions, plan._kv, plan._native, keep, sinks, recent, max(cap, 0))
+    most = max(0, min(keep, plan.longest - keep))      # moves of the longest request, at most
+    return native().select_evictions(weights, slot_positions, plan._kv, plan._native, keep, sinks, recent, most)
 
 
 def compact_cache(kv, layer: int, plan: DecodePlan, moves: torch.Tensor, counts: torch.Tensor,
