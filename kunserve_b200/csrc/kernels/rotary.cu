@@ -20,7 +20,8 @@ namespace kus {
 
 namespace rot {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;   // at most; a block has what its items divide into
+constexpr int kItems = 3;        // items (16 elements of a head) whose loads a thread has in flight
 
 // VEC: 16-byte vectors (bases and strides of 16 bytes, hd and rot multiples
 // of 16, interleaved rot of 8); otherwise single elements, one pair or one
@@ -31,15 +32,49 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
   pdl_wait();
   pdl_trigger();
   const int t = blockIdx.x;
-  const long long pos = a.positions[t];
   const int half = a.rot / 2;
-  for (int i = threadIdx.x; i < half; i += kThreads) {
+  const int heads = a.nq + 2 * a.nkv;
+  const T* xrow = reinterpret_cast<const T*>(a.x) + t * a.xt;
+  T* orow = reinterpret_cast<T*>(a.out) + t * a.ot;
+  const int threads = blockDim.x, first = blockIdx.y * threads + threadIdx.x, step = gridDim.y * threads;
+
+  // vector items: j-th 16 elements of head h, as two vectors at dims d0, d1:
+  // the pairs (i, i + rot/2) where the half layout turns, else neighbours
+  const int per = a.hd / 16, items = heads * per, turned = a.rot / 16;
+  struct Item {
+    int h, d0, d1;
+    bool turn;
+  };
+  auto item_at = [&](int u) {
+    Item it;
+    it.h = u / per;
+    const int j = u - it.h * per;
+    it.turn = it.h < a.nq + a.nkv && j < turned;
+    it.d0 = (!INTER && it.turn) ? 8 * j : 16 * j;
+    it.d1 = (!INTER && it.turn) ? it.d0 + half : it.d0 + 8;
+    return it;
+  };
+  uint4 v0[kItems], v1[kItems];
+  auto load = [&](int u0) {
+#pragma unroll
+    for (int k = 0; k < kItems; ++k)
+      if (u0 + k * step < items) {
+        const Item it = item_at(u0 + k * step);
+        const T* src = xrow + it.h * a.xh;
+        v0[k] = *reinterpret_cast<const uint4*>(src + it.d0);
+        v1[k] = *reinterpret_cast<const uint4*>(src + it.d1);
+      }
+  };
+  // the data's loads run beside the angles
+  if (VEC) load(first);
+
+  const long long pos = a.positions[t];
+  for (int i = threadIdx.x; i < half; i += threads) {
     const unsigned long long turn = (unsigned long long)pos * a.steps[i];
     float s, c;
     sincospif((float)(long long)turn * 0x1p-63f, &s, &c);
     cs[i] = make_float2(c * a.scale, s * a.scale * a.sign);
   }
-  const int heads = a.nq + 2 * a.nkv;
   T* krow = nullptr;   // the token's cache row, KV head 0
   T* vrow = nullptr;
   if (a.nkv) {
@@ -52,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
       krow = reinterpret_cast<T*>(a.g.base + kv_offset(a.g, page, a.layer, false) + off);
       vrow = reinterpret_cast<T*>(a.g.base + kv_offset(a.g, page, a.layer, true) + off);
       if (a.weights && blockIdx.y == 0)
-        for (int h = threadIdx.x; h < a.nkv; h += kThreads) {
+        for (int h = threadIdx.x; h < a.nkv; h += threads) {
           const long long i = ((long long)page * a.nkv + h) * a.g.block_size + slot;
           a.weights[i] = 0.f;
           a.slot_positions[i] = (int)pos;
@@ -60,8 +95,6 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
     }
   }
   __syncthreads();
-  const T* xrow = reinterpret_cast<const T*>(a.x) + t * a.xt;
-  T* orow = reinterpret_cast<T*>(a.out) + t * a.ot;
   // head h's destination; null: not written
   auto dest = [&](int h) -> T* {
     if (h < a.nq) return orow + h * a.oh;
@@ -69,51 +102,47 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
     return h < a.nq + a.nkv ? krow + (long long)(h - a.nq) * a.hd : vrow + (long long)(h - a.nq - a.nkv) * a.hd;
   };
   if (VEC) {
-    const int per = a.hd / 16, items = heads * per, turned = a.rot / 16;
-    for (int u = blockIdx.y * kThreads + threadIdx.x; u < items; u += gridDim.y * kThreads) {
-      const int h = u / per, j = u - h * per;
-      T* dst = dest(h);
-      if (!dst) continue;
-      const T* src = xrow + h * a.xh;
-      const bool turn = h < a.nq + a.nkv && j < turned;
-      // the two vectors' dims: pairs (i, i + rot/2) when turned in the half
-      // layout, else neighbours
-      const int d0 = (!INTER && turn) ? 8 * j : 16 * j;
-      const int d1 = (!INTER && turn) ? d0 + half : d0 + 8;
-      uint4 v0 = *reinterpret_cast<const uint4*>(src + d0);
-      uint4 v1 = *reinterpret_cast<const uint4*>(src + d1);
-      if (turn) {
-        float x0[8], x1[8];
-        unpack8<T>(v0, x0);
-        unpack8<T>(v1, x1);
-        if (INTER) {
+    for (int u0 = first; u0 < items; u0 += kItems * step) {
+      if (u0 != first) load(u0);
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float2 p = cs[d0 / 2 + e / 2], r = cs[d1 / 2 + e / 2];
-            const float a0 = x0[e], a1 = x1[e];
-            x0[e] = a0 * p.x - x0[e + 1] * p.y;
-            x0[e + 1] = x0[e + 1] * p.x + a0 * p.y;
-            x1[e] = a1 * r.x - x1[e + 1] * r.y;
-            x1[e + 1] = x1[e + 1] * r.x + a1 * r.y;
-          }
-        } else {
+      for (int k = 0; k < kItems; ++k) {
+        if (u0 + k * step >= items) break;
+        const Item it = item_at(u0 + k * step);
+        T* dst = dest(it.h);
+        if (!dst) continue;
+        if (it.turn) {
+          float x0[8], x1[8];
+          unpack8<T>(v0[k], x0);
+          unpack8<T>(v1[k], x1);
+          if (INTER) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float2 p = cs[d0 + e];
-            const float a0 = x0[e];
-            x0[e] = a0 * p.x - x1[e] * p.y;
-            x1[e] = x1[e] * p.x + a0 * p.y;
+            for (int e = 0; e < 8; e += 2) {
+              const float2 p = cs[it.d0 / 2 + e / 2], r = cs[it.d1 / 2 + e / 2];
+              const float a0 = x0[e], a1 = x1[e];
+              x0[e] = a0 * p.x - x0[e + 1] * p.y;
+              x0[e + 1] = x0[e + 1] * p.x + a0 * p.y;
+              x1[e] = a1 * r.x - x1[e + 1] * r.y;
+              x1[e + 1] = x1[e + 1] * r.x + a1 * r.y;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 p = cs[it.d0 + e];
+              const float a0 = x0[e];
+              x0[e] = a0 * p.x - x1[e] * p.y;
+              x1[e] = x1[e] * p.x + a0 * p.y;
+            }
           }
+          v0[k] = pack8<T>(x0);
+          v1[k] = pack8<T>(x1);
         }
-        v0 = pack8<T>(x0);
-        v1 = pack8<T>(x1);
+        *reinterpret_cast<uint4*>(dst + it.d0) = v0[k];
+        *reinterpret_cast<uint4*>(dst + it.d1) = v1[k];
       }
-      *reinterpret_cast<uint4*>(dst + d0) = v0;
-      *reinterpret_cast<uint4*>(dst + d1) = v1;
     }
   } else {
-    const int per = half + (a.hd - a.rot), items = heads * a.hd;
-    for (int u = blockIdx.y * kThreads + threadIdx.x; u < items; u += gridDim.y * kThreads) {
+    const int pairs = half + (a.hd - a.rot);
+    for (int u = first; u < heads * a.hd; u += step) {
       const int h = u / a.hd, j = u - h * a.hd;
       T* dst = dest(h);
       if (!dst) continue;
@@ -126,7 +155,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
         const float2 p = cs[j];
         dst[d0] = Elem<T>::from_f(x0 * p.x - x1 * p.y);
         dst[d1] = Elem<T>::from_f(x1 * p.x + x0 * p.y);
-      } else if (j < per) {
+      } else if (j < pairs) {
         dst[j + half] = src[j + half];
       }
     }
@@ -141,14 +170,15 @@ void launch(const RotaryArgs& a, cudaStream_t s) {
   const int items = (a.nq + 2 * a.nkv) * (vec ? a.hd / 16 : a.hd);
   // few tokens: several blocks a token, each with the heads' share, so that
   // one token's heads are all in flight at once
-  const int per_token = (items + kThreads - 1) / kThreads;
-  const int split = a.T >= 2 * 148 ? 1 : per_token;
+  const int rounds = (items + kThreads - 1) / kThreads;
+  const int split = a.T >= 2 * 148 ? 1 : rounds;
+  const int threads = ((items + rounds - 1) / rounds + 31) / 32 * 32;   // no round is half empty
   const dim3 grid(a.T, split);
   const size_t smem = (size_t)a.rot / 2 * sizeof(float2);
   if (vec)
-    launch_k(rotary_kernel<T, INTER, true>, grid, dim3(kThreads), smem, s, a);
+    launch_k(rotary_kernel<T, INTER, true>, grid, dim3(threads), smem, s, a);
   else
-    launch_k(rotary_kernel<T, INTER, false>, grid, dim3(kThreads), smem, s, a);
+    launch_k(rotary_kernel<T, INTER, false>, grid, dim3(threads), smem, s, a);
 }
 
 }  // namespace rot
