@@ -165,6 +165,12 @@ void check_heads(const torch::Tensor& t, int64_t T, int64_t heads, int64_t hd, c
               " with contiguous heads, got ", t.scalar_type(), " ", t.sizes(), " strides ", t.strides());
 }
 
+// Every head of a 16-bit [T, heads, hd] tensor starts on 16 bytes.
+bool heads_on_16(const torch::Tensor& t) {
+  return (t.size(0) <= 1 || t.stride(0) % 8 == 0) && (t.size(1) <= 1 || t.stride(1) % 8 == 0) &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
 RotaryArgs rotary_args(const torch::Tensor& x, const torch::Tensor& positions, const torch::Tensor& steps, double scale,
                        int64_t rot, bool interleaved, const torch::Tensor& out, bool inverse) {
   RotaryArgs a{};
@@ -174,7 +180,7 @@ RotaryArgs rotary_args(const torch::Tensor& x, const torch::Tensor& positions, c
                   steps.numel() == rot / 2,
               "the rotary frequencies must be on ", x.device());
   check_index(positions, x.size(0), x, "positions");
-  KUS_CHECK(x.size(0) < (1LL << 31) && x.size(1) * hd < (1 << 24), "too many tokens or heads");
+  KUS_CHECK(x.size(0) < (1LL << 31) && x.size(1) * hd < (1 << 23), "too many tokens or heads");
   a.x = x.data_ptr();
   a.xt = x.stride(0);
   a.xh = x.stride(1);
@@ -249,12 +255,10 @@ torch::Tensor cached_attention_op(const torch::Tensor& q, const PagedKV& kv, int
   KUS_CHECK(a.g.hd == 64 || a.g.hd == 128, "attention takes head_dim 64 or 128, the cache has ", a.g.hd);
   KUS_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive");
   check_heads(q, plan.T, plan.nq, a.g.hd, kv.pool, "q");
-  KUS_CHECK(q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
-              "q's heads must start on 16 bytes");
+  KUS_CHECK(heads_on_16(q), "q's heads must start on 16 bytes");
   torch::Tensor o = out.has_value() ? *out : torch::empty({plan.T, plan.nq, a.g.hd}, kv.pool.options());
   check_heads(o, plan.T, plan.nq, a.g.hd, kv.pool, "out");
-  KUS_CHECK(o.stride(0) % 8 == 0 && o.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0,
-              "out's heads must start on 16 bytes");
+  KUS_CHECK(heads_on_16(o), "out's heads must start on 16 bytes");
   a.layer = kv.checked_layer(layer);
   a.q = q.data_ptr();
   a.qt = q.stride(0);
@@ -285,7 +289,7 @@ torch::Tensor cached_attention_op(const torch::Tensor& q, const PagedKV& kv, int
   a.part_o = scratch.data_ptr<float>();
   a.part_ml = reinterpret_cast<float2*>(a.part_o + n_o + n_s);
   if (weighted) {
-    KUS_CHECK(plan.n_reqs > 0, "weights need a decode plan");
+    KUS_CHECK(plan.n_reqs > 0 || plan.T == 0, "weights need a decode plan");
     kv.check_side(*weights, torch::kFloat32, "weights");
     a.scores = a.part_o + n_o;
     a.stats = a.part_ml + plan.part_rows;
@@ -346,6 +350,7 @@ void compact_cache_op(const PagedKV& kv, int64_t layer, const CachePlan& plan, c
               "moves must be a contiguous int32 tensor [", plan.n_reqs, ", ", a.g.kvh, ", most, 2], got ",
               moves.sizes());
   check_index(counts, (int64_t)plan.n_reqs * a.g.kvh, kv.pool, "counts");
+  KUS_CHECK((int64_t)plan.n_reqs * a.g.kvh * (moves.size(2) / 32 + 1) < (1LL << 31), "too many moves for one launch");
   a.pages = plan.ints(plan.o_pages);
   a.reqs = plan.ints(plan.o_reqs);
   a.n_reqs = plan.n_reqs;

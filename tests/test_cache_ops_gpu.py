@@ -650,3 +650,50 @@ def test_refusals():
         compact_cache(kv, 0, dec, moves, counts[:, :1].contiguous())
     with bad:
         compact_cache(kv, 5, dec, moves, counts)
+
+
+def test_empty_batches():
+    """No tokens, no heads, no requests: empty results, nothing launched."""
+    from kunserve_b200.ops import (DecodePlan, Rotary, compact_cache, rotary_append, rotary_apply, select_evictions,
+                                   weighted_decode_attention)
+    pool, kv, _ = _cache(6, 16, 2, 64, BF)
+    before = pool.clone()
+    i32 = torch.zeros(0, dtype=torch.int32, device="cuda")
+    rot = Rotary(64)
+    assert rotary_apply(torch.zeros(0, 4, 64, device="cuda", dtype=BF), i32, rot).shape == (0, 4, 64)
+    assert rotary_apply(torch.zeros(3, 0, 64, device="cuda", dtype=BF), torch.zeros(3, dtype=torch.int32, device="cuda"),
+                        rot).shape == (3, 0, 64)
+    rotary_append(torch.zeros(0, 6, 64, device="cuda", dtype=BF), i32, i32, i32, rot, kv, 0)
+    plan = DecodePlan([], [], kv, 4)
+    w, sp = torch.zeros(6, 2, 16, device="cuda"), torch.zeros(6, 2, 16, dtype=torch.int32, device="cuda")
+    assert weighted_decode_attention(torch.zeros(0, 4, 64, device="cuda", dtype=BF), kv, 0, plan, w).shape == (0, 4, 64)
+    moves, counts = select_evictions(w, sp, plan, 4)
+    assert moves.shape == (0, 2, 0, 2) and counts.shape == (0, 2)
+    compact_cache(kv, 0, plan, moves, counts, w, sp)
+    # one request that needs no eviction: no moves
+    moves, counts = select_evictions(w, sp, DecodePlan([[0]], [4], kv, 4), 4)
+    assert moves.shape == (1, 2, 0, 2) and (counts == 0).all()
+    assert torch.equal(pool, before)
+    # one token whose row has a stride that no second row uses
+    q = torch.zeros(70 + 4 * 64, device="cuda", dtype=BF)[64:64 + 256].view(1, 4, 64)
+    q = q.as_strided((1, 4, 64), (13, 64, 1))
+    assert weighted_decode_attention(q, kv, 0, DecodePlan([[0]], [4], kv, 4), w).shape == (1, 4, 64)
+
+
+def test_nan_in_unused_places_reaches_nothing():
+    """Slots past a request's tokens hold NaN in the cache and in the weights."""
+    from kunserve_b200.ops import DecodePlan, select_evictions, weighted_decode_attention
+    pool, kv, lay = _cache(5, 16, 2, 64, BF, poison=True)
+    pages, n = [4, 1], 19
+    _fill(pool, lay, pages, n, 0, 1, 1)
+    w = torch.full((kv.pages_total, 2, 16), math.nan, device="cuda")
+    at = torch.arange(n)
+    idx = (torch.tensor(pages)[at // 16], slice(None), at % 16)
+    w[idx] = 0.0
+    sp = torch.zeros(kv.pages_total, 2, 16, dtype=torch.int32, device="cuda")
+    plan = DecodePlan([pages], [n], kv, 4)
+    out = weighted_decode_attention(torch.randn(1, 4, 64, device="cuda").to(BF), kv, 0, plan, w)
+    assert torch.isfinite(out.float()).all() and torch.isfinite(w[idx]).all()
+    assert int(torch.isfinite(w).sum()) == 2 * n
+    moves, counts = select_evictions(w, sp + 100, plan, 10)
+    assert (counts >= 0).all() and (moves < n).all()
