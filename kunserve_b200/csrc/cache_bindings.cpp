@@ -2,6 +2,8 @@
 // handle of a paged cache, the plan of a batch, and one function per operator.
 // Arguments are checked here; kunserve_b200/ops documents them.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 #include <cmath>
@@ -151,6 +153,10 @@ struct CachePlan {
   }
 };
 
+torch::Tensor empty(at::IntArrayRef sizes, torch::ScalarType type, const torch::Device& device) {
+  return torch::Tensor(at::detail::empty_cuda(sizes, type, device, {}));
+}
+
 void check_index(const torch::Tensor& t, int64_t n, const torch::Tensor& like, const char* what) {
   KUS_CHECK(t.device() == like.device() && t.scalar_type() == torch::kInt32 && t.is_contiguous() && t.numel() == n,
               what, " must be a contiguous int32 tensor of ", n, " on ", like.device());
@@ -171,16 +177,31 @@ bool heads_on_16(const torch::Tensor& t) {
          reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
-RotaryArgs rotary_args(const torch::Tensor& x, const torch::Tensor& positions, const torch::Tensor& steps, double scale,
-                       int64_t rot, bool interleaved, const torch::Tensor& out, bool inverse) {
-  RotaryArgs a{};
+// The frequencies of a model's rotary positions (kunserve_b200/ops/rotary.py).
+struct RotaryTable {
+  torch::Tensor steps;
+  float scale;
+  int hd, rot;
+  bool interleaved;
+
+  RotaryTable(torch::Tensor s, double scale_, int64_t hd_, bool interleaved_)
+      : steps(std::move(s)), scale((float)scale_), hd((int)hd_), rot(0), interleaved(interleaved_) {
+    KUS_CHECK(steps.is_cuda() && steps.scalar_type() == torch::kInt64 && steps.is_contiguous() && steps.dim() == 1,
+              "rotary steps must be a contiguous int64 CUDA tensor");
+    const int64_t r = 2 * steps.numel();
+    KUS_CHECK(r > 0 && r <= hd_ && r <= 4096, "rotary_dim ", r, " of head_dim ", hd_);
+    rot = (int)r;
+  }
+};
+
+RotaryArgs rotary_args(const RotaryTable* table, const torch::Tensor& x, const torch::Tensor& positions,
+                       const torch::Tensor& out, bool inverse) {
+  KUS_CHECK(table && table->steps.device() == x.device(), "the rotary frequencies must be on ", x.device());
   const int64_t hd = x.size(2);
-  KUS_CHECK(rot > 0 && rot % 2 == 0 && rot <= hd && rot <= 4096, "rotary_dim ", rot, " of head_dim ", hd);
-  KUS_CHECK(steps.device() == x.device() && steps.scalar_type() == torch::kInt64 && steps.is_contiguous() &&
-                  steps.numel() == rot / 2,
-              "the rotary frequencies must be on ", x.device());
+  KUS_CHECK(hd == table->hd, "head_dim ", hd, ", the rotary frequencies have ", (int64_t)table->hd);
   check_index(positions, x.size(0), x, "positions");
   KUS_CHECK(x.size(0) < (1LL << 31) && x.size(1) * hd < (1 << 23), "too many tokens or heads");
+  RotaryArgs a{};
   a.x = x.data_ptr();
   a.xt = x.stride(0);
   a.xh = x.stride(1);
@@ -188,44 +209,43 @@ RotaryArgs rotary_args(const torch::Tensor& x, const torch::Tensor& positions, c
   a.ot = out.stride(0);
   a.oh = out.stride(1);
   a.positions = positions.data_ptr<int>();
-  a.steps = reinterpret_cast<const unsigned long long*>(steps.data_ptr<int64_t>());
-  a.scale = (float)scale;
+  a.steps = reinterpret_cast<const unsigned long long*>(table->steps.data_ptr<int64_t>());
+  a.scale = table->scale;
   a.sign = inverse ? -1.f : 1.f;
   a.T = (int)x.size(0);
   a.nq = (int)x.size(1);
   a.hd = (int)hd;
-  a.rot = (int)rot;
-  a.interleaved = interleaved;
+  a.rot = table->rot;
+  a.interleaved = table->interleaved;
   return a;
 }
 
-torch::Tensor rotary_apply_op(const torch::Tensor& x, const torch::Tensor& positions, const torch::Tensor& steps,
-                              double scale, int64_t rot, bool interleaved, c10::optional<torch::Tensor> out,
-                              bool inverse) {
+torch::Tensor rotary_apply_op(const torch::Tensor& x, const torch::Tensor& positions, const RotaryTable* table,
+                              const c10::optional<torch::Tensor>& out, bool inverse) {
   KUS_CHECK(x.is_cuda() && x.dim() == 3, "x must be a CUDA tensor [T, heads, head_dim]");
   const int type = elem_type(x, "x");
   c10::cuda::CUDAGuard guard(x.device());
   check_heads(x, x.size(0), x.size(1), x.size(2), x, "x");
-  torch::Tensor o = out.has_value() ? *out : torch::empty(x.sizes(), x.options());
+  torch::Tensor o = out.has_value() ? *out : empty(x.sizes(), x.scalar_type(), x.device());
   check_heads(o, x.size(0), x.size(1), x.size(2), x, "out");
-  rotary(rotary_args(x, positions, steps, scale, rot, interleaved, o, inverse), type,
-         at::cuda::getCurrentCUDAStream());
+  rotary(rotary_args(table, x, positions, o, inverse), type, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return o;
 }
 
 void rotary_append_op(const torch::Tensor& qkv, const torch::Tensor& positions, const torch::Tensor& pages,
-                      const torch::Tensor& slots, const torch::Tensor& steps, double scale, int64_t rot,
-                      bool interleaved, const PagedKV& kv, int64_t layer, c10::optional<torch::Tensor> out,
-                      c10::optional<torch::Tensor> weights, c10::optional<torch::Tensor> slot_positions) {
+                      const torch::Tensor& slots, const RotaryTable* table, const PagedKV& kv, int64_t layer,
+                      const c10::optional<torch::Tensor>& out, const c10::optional<torch::Tensor>& weights,
+                      const c10::optional<torch::Tensor>& slot_positions) {
   const KVGeom& g = kv.g;
   c10::cuda::CUDAGuard guard(kv.pool.device());
-  KUS_CHECK(qkv.dim() == 3 && qkv.size(1) >= 2 * g.kvh, "qkv must be [T, q heads + 2 * ", g.kvh, ", ", g.hd, "]");
+  KUS_CHECK(qkv.dim() == 3 && qkv.size(1) >= 2 * g.kvh, "qkv must be [T, q heads + 2 * ", (int64_t)g.kvh, ", ",
+            (int64_t)g.hd, "]");
   const int64_t T = qkv.size(0), nq = qkv.size(1) - 2 * g.kvh;
   check_heads(qkv, T, nq + 2 * g.kvh, g.hd, kv.pool, "qkv");
-  torch::Tensor o = out.has_value() ? *out : qkv.narrow(1, 0, nq);
-  check_heads(o, T, nq, g.hd, kv.pool, "out");
-  RotaryArgs a = rotary_args(qkv, positions, steps, scale, rot, interleaved, o, false);
+  // without `out` the queries turn in place: they lie first in qkv
+  if (out.has_value()) check_heads(*out, T, nq, g.hd, kv.pool, "out");
+  RotaryArgs a = rotary_args(table, qkv, positions, out.has_value() ? *out : qkv, false);
   check_index(pages, T, qkv, "pages");
   check_index(slots, T, qkv, "slots");
   KUS_CHECK(weights.has_value() == slot_positions.has_value(), "weights and slot_positions come together");
@@ -246,8 +266,9 @@ void rotary_append_op(const torch::Tensor& qkv, const torch::Tensor& positions, 
 }
 
 torch::Tensor cached_attention_op(const torch::Tensor& q, const PagedKV& kv, int64_t layer, const CachePlan& plan,
-                                  double scale, c10::optional<torch::Tensor> out,
-                                  c10::optional<torch::Tensor> weights) {
+                                  c10::optional<double> scale_arg, const c10::optional<torch::Tensor>& out,
+                                  const c10::optional<torch::Tensor>& weights) {
+  const double scale = scale_arg.has_value() ? *scale_arg : 1.0 / std::sqrt((double)kv.g.hd);
   plan.use(kv);
   c10::cuda::CUDAGuard guard(kv.pool.device());
   CachedAttn a{};
@@ -256,7 +277,8 @@ torch::Tensor cached_attention_op(const torch::Tensor& q, const PagedKV& kv, int
   KUS_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive");
   check_heads(q, plan.T, plan.nq, a.g.hd, kv.pool, "q");
   KUS_CHECK(heads_on_16(q), "q's heads must start on 16 bytes");
-  torch::Tensor o = out.has_value() ? *out : torch::empty({plan.T, plan.nq, a.g.hd}, kv.pool.options());
+  torch::Tensor o = out.has_value() ? *out
+                                    : empty({plan.T, plan.nq, a.g.hd}, kv.pool.scalar_type(), kv.pool.device());
   check_heads(o, plan.T, plan.nq, a.g.hd, kv.pool, "out");
   KUS_CHECK(heads_on_16(o), "out's heads must start on 16 bytes");
   a.layer = kv.checked_layer(layer);
@@ -284,9 +306,9 @@ torch::Tensor cached_attention_op(const torch::Tensor& q, const PagedKV& kv, int
   const bool weighted = weights.has_value();
   const int64_t n_o = plan.part_rows * a.g.hd, n_s = weighted ? plan.score_cols * plan.nq : 0,
                 n_st = weighted ? 2LL * plan.T * plan.nq : 0;
-  torch::Tensor scratch = torch::empty({n_o + n_s + 2 * plan.part_rows + n_st},
-                                       torch::TensorOptions().dtype(torch::kFloat32).device(kv.pool.device()));
-  a.part_o = scratch.data_ptr<float>();
+  const c10::DataPtr scratch =
+      c10::cuda::CUDACachingAllocator::get()->allocate(4 * (n_o + n_s + 2 * plan.part_rows + n_st));
+  a.part_o = static_cast<float*>(scratch.get());
   a.part_ml = reinterpret_cast<float2*>(a.part_o + n_o + n_s);
   if (weighted) {
     KUS_CHECK(plan.n_reqs > 0 || plan.T == 0, "weights need a decode plan");
@@ -314,9 +336,8 @@ std::tuple<torch::Tensor, torch::Tensor> select_evictions_op(const torch::Tensor
               ") must fit in keep (", keep, ")");
   kv.check_side(weights, torch::kFloat32, "weights");
   kv.check_side(slot_positions, torch::kInt32, "slot_positions");
-  auto i32 = torch::TensorOptions().dtype(torch::kInt32).device(kv.pool.device());
-  torch::Tensor moves = torch::empty({plan.n_reqs, kv.g.kvh, cap, 2}, i32);
-  torch::Tensor counts = torch::empty({plan.n_reqs, kv.g.kvh}, i32);
+  torch::Tensor moves = empty({plan.n_reqs, kv.g.kvh, cap, 2}, torch::kInt32, kv.pool.device());
+  torch::Tensor counts = empty({plan.n_reqs, kv.g.kvh}, torch::kInt32, kv.pool.device());
   EvictSelect a{};
   a.weights = weights.data_ptr<float>();
   a.slot_positions = slot_positions.data_ptr<int>();
@@ -337,8 +358,8 @@ std::tuple<torch::Tensor, torch::Tensor> select_evictions_op(const torch::Tensor
 }
 
 void compact_cache_op(const PagedKV& kv, int64_t layer, const CachePlan& plan, const torch::Tensor& moves,
-                      const torch::Tensor& counts, c10::optional<torch::Tensor> weights,
-                      c10::optional<torch::Tensor> slot_positions) {
+                      const torch::Tensor& counts, const c10::optional<torch::Tensor>& weights,
+                      const c10::optional<torch::Tensor>& slot_positions) {
   plan.use(kv);
   c10::cuda::CUDAGuard guard(kv.pool.device());
   CacheCompact a{};
@@ -382,6 +403,7 @@ void bind_cache_ops(py::module& m) {
       .def_property_readonly("pool", [](const PagedKV& k) { return k.pool; });
   py::class_<CachePlan>(m, "CachePlan")
       .def(py::init<const torch::Tensor&, const PagedKV&, const std::map<std::string, int64_t>&>());
+  py::class_<RotaryTable>(m, "RotaryTable").def(py::init<torch::Tensor, double, int64_t, bool>());
   m.def("rotary_apply", &rotary_apply_op);
   m.def("rotary_append_scaled", &rotary_append_op);
   m.def("cached_attention", &cached_attention_op);

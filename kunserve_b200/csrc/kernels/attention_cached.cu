@@ -460,25 +460,12 @@ __global__ void __launch_bounds__(kJoinThreads, 8) weights_kernel(CachedAttn a) 
   add_weights(a, c, kh, sh_m, sh_l);
 }
 
-// Launch whose grid may start while the previous one of the stream ends.
-template <typename... KArgs, typename... Args>
-void launch_behind(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, Args... args) {
-  bool& pdl = pdl_flag();
-  const bool was = pdl;
-  pdl = true;
-  launch_k(kern, dim3(grid), dim3(block), smem, s, args...);
-  pdl = was;
-}
-
 template <typename T, int HD, bool SCORES>
 void launch_rows(const CachedAttn& a, bool second, cudaStream_t s) {
   constexpr int smem = RowCfg<HD>::kSmem;
   ensure_smem_attr(reinterpret_cast<const void*>(rows_kernel<T, HD, SCORES>), smem);
   const unsigned grid = (unsigned)(((long long)a.n_row_units * a.g.kvh + kWarps - 1) / kWarps);
-  if (second)
-    launch_behind(rows_kernel<T, HD, SCORES>, grid, kWarps * 32, smem, s, a, a.scale * kLog2e, true);
-  else
-    launch_k(rows_kernel<T, HD, SCORES>, dim3(grid), dim3(kWarps * 32), smem, s, a, a.scale * kLog2e, false);
+  launch_k(rows_kernel<T, HD, SCORES>, dim3(grid), dim3(kWarps * 32), smem, s, a, a.scale * kLog2e, second);
 }
 
 template <typename T, int HD>
@@ -493,15 +480,13 @@ void launch(const CachedAttn& a, const CUtensorMap* map, int type, cudaStream_t 
   const bool wide = a.most_parts > 32;
   const unsigned joins = (unsigned)(wide ? rows : (rows + 3) / 4);
   const unsigned chunks = a.scores ? (unsigned)a.n_chunks * a.g.kvh : 0u;
-  if (!tiles && a.n_row_units == 0) {   // no part at all: zeros
-    launch_k(join_kernel<T, HD, 1>, dim3(joins), dim3(kJoinThreads), 0, s, a, joins);
-  } else if (!wide) {
+  if (!wide) {
     CachedAttn b = a;
     b.stats = nullptr;
-    launch_behind(join_kernel<T, HD, 1>, joins + chunks, kJoinThreads, 0, s, b, joins);
+    launch_k(join_kernel<T, HD, 1>, dim3(joins + chunks), dim3(kJoinThreads), 0, s, b, joins);
   } else {
-    launch_behind(join_kernel<T, HD, 8>, joins, 256, 0, s, a, joins);
-    if (chunks) launch_behind(weights_kernel, chunks, kJoinThreads, 0, s, a);
+    launch_k(join_kernel<T, HD, 8>, dim3(joins), dim3(256), 0, s, a, joins);
+    if (chunks) launch_k(weights_kernel, dim3(chunks), dim3(kJoinThreads), 0, s, a);
   }
 }
 
@@ -509,6 +494,7 @@ void launch(const CachedAttn& a, const CUtensorMap* map, int type, cudaStream_t 
 
 void cached_attention(const CachedAttn& a, const CUtensorMap* map, int type, cudaStream_t s) {
   if (a.T <= 0) return;
+  const LaunchBehind behind;
   if (type == kTypeBF16) {
     a.hd == 128 ? cat::launch<__nv_bfloat16, 128>(a, map, type, s) : cat::launch<__nv_bfloat16, 64>(a, map, type, s);
   } else {

@@ -52,4 +52,14 @@ KUS_DEVICE float ex2(float x) {
   return y;
 }
 
+// While one lives, this thread's launches carry programmatic serialization:
+// a grid is set up while the one before it ends.  Every kernel of the cache
+// operators waits for the one before (pdl_wait) ahead of its first access to
+// what others write; only plans, which no kernel writes, are read earlier.
+struct LaunchBehind {
+  const bool was = pdl_flag();
+  LaunchBehind() { pdl_flag() = true; }
+  ~LaunchBehind() { pdl_flag() = was; }
+};
+
 }  // namespace kus

@@ -8,6 +8,7 @@
 // must, no destination is another move's source, and the order of keys does
 // not matter to attention.
 #include "../common.cuh"
+#include "cache_elem.cuh"
 #include "cache_ops.h"
 
 namespace kus {
@@ -333,6 +334,7 @@ __global__ void __launch_bounds__(kCompactWarps * 32, CH ? 8 : 4) compact_kernel
 void evict_select(const EvictSelect& a, cudaStream_t s) {
   const int rows = a.n_reqs * a.g.kvh;
   if (rows <= 0) return;
+  const LaunchBehind behind;
   // Few long rows: several CTAs share one, down to 2048 slots each, while the
   // grid stays within eight CTAs an SM.  Small blocks pay less for each of the
   // search's barriers (8 rows of 6001-20000 slots and 8 heads: 21 us, blocks of
@@ -350,6 +352,7 @@ void evict_select(const EvictSelect& a, cudaStream_t s) {
 void cache_compact(const CacheCompact& a, cudaStream_t s) {
   const int rows = a.n_reqs * a.g.kvh;
   if (rows <= 0 || a.cap <= 0) return;
+  const LaunchBehind behind;
   const int per_row = (a.cap + evict::kMoves - 1) / evict::kMoves;
   const long long warps = (long long)rows * per_row;
   const dim3 grid((unsigned)((warps + evict::kCompactWarps - 1) / evict::kCompactWarps));

@@ -185,6 +185,7 @@ void launch(const RotaryArgs& a, cudaStream_t s) {
 
 void rotary(const RotaryArgs& a, int type, cudaStream_t s) {
   if (a.T <= 0 || a.nq + a.nkv == 0) return;
+  const LaunchBehind behind;
   if (type == kTypeBF16) {
     a.interleaved ? rot::launch<__nv_bfloat16, true>(a, s) : rot::launch<__nv_bfloat16, false>(a, s);
   } else {

@@ -7,7 +7,6 @@ calls the operators with it for every layer.  All of them run on the current
 CUDA stream of the cache's device and allocate their scratch from it.
 """
 import functools
-import math
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
@@ -76,8 +75,6 @@ def shared_prefix_attention(q: torch.Tensor, kv, layer: int, plan: SharedPrefixP
     their group's prefix and their request's own tokens in ``layer`` of the
     cache, the keys of a prefix read once for all its requests.  Queries that
     see no key give zeros.  ``scale`` defaults to head_dim ** -0.5."""
-    if scale is None:
-        scale = 1.0 / math.sqrt(kv.head_dim)
     return native().cached_attention(q, kv, layer, plan._native, scale, out, None)
 
 
@@ -125,8 +122,6 @@ def weighted_decode_attention(q: torch.Tensor, kv, layer: int, plan: DecodePlan,
     over its cached tokens; ``weights`` gains, at each token's slot and KV
     head, the softmax weight that the head's query group gave it (summed over
     the group, fp32).  Requests without tokens give zeros."""
-    if scale is None:
-        scale = 1.0 / math.sqrt(kv.head_dim)
     return native().cached_attention(q, kv, layer, plan._native, scale, out, weights)
 
 

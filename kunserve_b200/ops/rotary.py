@@ -99,6 +99,9 @@ class Rotary:
         turns = [round(f / (2 * math.pi) * 2 ** 64) % 2 ** 64 for f in self.frequencies.tolist()]
         signed = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns]
         self.steps = torch.tensor(signed, dtype=torch.int64, device=device)
+        self._native = None
+        if self.steps.is_cuda:
+            self._native = native().RotaryTable(self.steps, self.scale, self.head_dim, self.interleaved)
 
 
 def rotary_apply(x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, out: Optional[torch.Tensor] = None,
@@ -109,10 +112,7 @@ def rotary_apply(x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, out: 
     ``out`` may be ``x``.  ``inverse`` turns back; with the factor on cos and
     sin kept, that is the gradient: if y = rotary_apply(x), the gradient of x
     is rotary_apply(gradient of y, inverse=True)."""
-    if x.dim() != 3 or x.shape[2] != rotary.head_dim:
-        raise ValueError(f"x must be [T, heads, {rotary.head_dim}], got {tuple(x.shape)}")
-    return native().rotary_apply(x, positions, rotary.steps, rotary.scale, rotary.rotary_dim, rotary.interleaved, out,
-                                 inverse)
+    return native().rotary_apply(x, positions, rotary._native, out, inverse)
 
 
 def rotary_append(qkv: torch.Tensor, positions: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor,
@@ -127,7 +127,4 @@ def rotary_append(qkv: torch.Tensor, positions: torch.Tensor, pages: torch.Tenso
     ``slot_positions`` (see ``DecodePlan``) get the new slots' zero weight and
     their token's position.  A page or slot outside the cache is not written;
     ``check_error`` reports it."""
-    if rotary.head_dim != kv.head_dim:
-        raise ValueError(f"rotary head_dim {rotary.head_dim}, cache head_dim {kv.head_dim}")
-    native().rotary_append_scaled(qkv, positions, pages, slots, rotary.steps, rotary.scale, rotary.rotary_dim,
-                                  rotary.interleaved, kv, layer, out, weights, slot_positions)
+    native().rotary_append_scaled(qkv, positions, pages, slots, rotary._native, kv, layer, out, weights, slot_positions)
