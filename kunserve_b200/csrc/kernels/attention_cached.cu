@@ -14,7 +14,11 @@
 // Stages of 32 keys (K and V rows, 16-byte cp.async, ends filled with zeros)
 // run through a ring in shared memory; S = Q K^T and O += P V are m16n8k16
 // tensor products with the unit's rows as M, so a key costs the same HBM
-// bytes for 1 to 16 rows: bound by HBM.
+// bytes for 1 to 16 rows: bound by HBM (30 requests of 300-2300 tokens, 40
+// heads: 812 MB in 130 us, 6.2 TB/s).  Six warps an SM hold 32 KB each; with
+// few stages a warp's own latency counts: 3500 clk to its first stage, 2900 a
+// stage, of which 1400 issue the next loads (TMA boxes instead gained nothing
+// here, three stages neither: fewer warps then fit).
 #include "../common.cuh"
 #include "cache_elem.cuh"
 #include "cache_ops.h"
@@ -22,7 +26,6 @@
 namespace kus {
 namespace cat {
 
-constexpr int kWarps = 1;
 constexpr int kKeys = 32;       // keys per stage
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -31,7 +34,7 @@ struct RowCfg {
   static constexpr int kTile = kKeys * HD * 2;        // K or V of a stage
   static constexpr int kStage = 2 * kTile;
   static constexpr int kStages = HD == 128 ? 2 : 4;   // 32 KB a warp
-  static constexpr int kSmem = kWarps * kStages * kStage;
+  static constexpr int kSmem = kStages * kStage;
 };
 
 KUS_DEVICE void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -95,26 +98,24 @@ KUS_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
 // so that the join (which waits for this kernel) finds both done.  (A block
 // that waits keeps its place on the SM: the others leave it to the next.)
 template <typename T, int HD, bool SCORES>
-__global__ void __launch_bounds__(kWarps * 32) rows_kernel(CachedAttn a, float scale_log2, bool second) {
+__global__ void __launch_bounds__(32) rows_kernel(CachedAttn a, float scale_log2, bool second) {
   using Cf = RowCfg<HD>;
   constexpr int kStages = Cf::kStages;
   constexpr int kCh = HD / 8;              // 16-byte chunks of a row
   constexpr int kRowsPer = 32 / kCh;       // rows that one load of the warp covers
   extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int lane = threadIdx.x;
   const int kvh = a.g.kvh, G = a.nq / kvh;
   if (!second) pdl_wait();
   pdl_trigger();
-  const int item = blockIdx.x * kWarps + warp;
-  if (item >= a.n_row_units * kvh) return;
-  const int u = item / kvh, kh = item - u * kvh;   // heads fastest: neighbours read the same cache rows
+  const int u = blockIdx.x / kvh, kh = blockIdx.x - u * kvh;   // heads fastest: neighbours read the same cache rows
   const int4 u0 = __ldg(reinterpret_cast<const int4*>(a.row_units) + 2 * u);
   const int4 u1 = __ldg(reinterpret_cast<const int4*>(a.row_units) + 2 * u + 1);
   const int tok0 = u0.x, ntok = u0.y & 255, ng = (u0.y >> 8) & 255, g0 = u0.y >> 16;
   const int key_lo = u0.z, key_hi = u0.w, lim0 = u1.x;
   const int* table = a.pages + u1.y;
   const int rows = ntok * ng;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * Cf::kStage;
+  const uint32_t ring = smem_u32(smem);
   const int nst = (key_hi - key_lo + kKeys - 1) / kKeys;
   const long long layer_elems = a.g.layer_stride / (int)sizeof(T);
 
@@ -464,8 +465,8 @@ template <typename T, int HD, bool SCORES>
 void launch_rows(const CachedAttn& a, bool second, cudaStream_t s) {
   constexpr int smem = RowCfg<HD>::kSmem;
   ensure_smem_attr(reinterpret_cast<const void*>(rows_kernel<T, HD, SCORES>), smem);
-  const unsigned grid = (unsigned)(((long long)a.n_row_units * a.g.kvh + kWarps - 1) / kWarps);
-  launch_k(rows_kernel<T, HD, SCORES>, dim3(grid), dim3(kWarps * 32), smem, s, a, a.scale * kLog2e, second);
+  launch_k(rows_kernel<T, HD, SCORES>, dim3((unsigned)a.n_row_units * a.g.kvh), dim3(32), smem, s, a,
+           a.scale * kLog2e, second);
 }
 
 template <typename T, int HD>

