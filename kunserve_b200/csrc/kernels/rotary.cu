@@ -12,8 +12,9 @@
 // Bound by HBM: each element is read once and written once.  A block takes
 // one token (its cos and sin computed once, into shared memory, for all
 // heads, while the first items' loads are under way); a thread turns 16
-// elements of a head as two 16-byte vectors.  16384 tokens of 64 + 8 heads of
-// 128: 672 MB in 119-124 us, 5.4-5.6 TB/s.
+// elements of a head as two 16-byte vectors.  Full SMs (32 registers a thread)
+// move more than several items in flight a thread: 16384 tokens of 64 + 8
+// heads of 128, 672 MB, take 103 us, with three items at 62 registers 117.
 #include "../common.cuh"
 #include "cache_elem.cuh"
 #include "cache_ops.h"
@@ -23,13 +24,12 @@ namespace kus {
 namespace rot {
 
 constexpr int kThreads = 256;   // at most; a block has what its items divide into
-constexpr int kItems = 3;        // items (16 elements of a head) whose loads a thread has in flight
 
 // VEC: 16-byte vectors (bases and strides of 16 bytes, hd and rot multiples
 // of 16, interleaved rot of 8); otherwise single elements, one pair or one
 // unrotated element a thread.
 template <typename T, bool INTER, bool VEC>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) rotary_kernel(RotaryArgs a) {
   extern __shared__ float2 cs[];   // (cos, sin) of the token's rot / 2 pairs
   pdl_wait();
   pdl_trigger();
@@ -56,19 +56,15 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
     it.d1 = (!INTER && it.turn) ? it.d0 + half : it.d0 + 8;
     return it;
   };
-  uint4 v0[kItems], v1[kItems];
-  auto load = [&](int u0) {
-#pragma unroll
-    for (int k = 0; k < kItems; ++k)
-      if (u0 + k * step < items) {
-        const Item it = item_at(u0 + k * step);
-        const T* src = xrow + it.h * a.xh;
-        v0[k] = *reinterpret_cast<const uint4*>(src + it.d0);
-        v1[k] = *reinterpret_cast<const uint4*>(src + it.d1);
-      }
+  uint4 v0, v1;
+  auto load = [&](int u) {
+    const Item it = item_at(u);
+    const T* src = xrow + it.h * a.xh;
+    v0 = *reinterpret_cast<const uint4*>(src + it.d0);
+    v1 = *reinterpret_cast<const uint4*>(src + it.d1);
   };
-  // the data's loads run beside the angles
-  if (VEC) load(first);
+  // the first item's loads run beside the angles
+  if (VEC && first < items) load(first);
 
   const long long pos = a.positions[t];
   for (int i = threadIdx.x; i < half; i += threads) {
@@ -104,43 +100,39 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
     return h < a.nq + a.nkv ? krow + (long long)(h - a.nq) * a.hd : vrow + (long long)(h - a.nq - a.nkv) * a.hd;
   };
   if (VEC) {
-    for (int u0 = first; u0 < items; u0 += kItems * step) {
-      if (u0 != first) load(u0);
+    for (int u = first; u < items; u += step) {
+      if (u != first) load(u);
+      const Item it = item_at(u);
+      T* dst = dest(it.h);
+      if (!dst) continue;
+      if (it.turn) {
+        float x0[8], x1[8];
+        unpack8<T>(v0, x0);
+        unpack8<T>(v1, x1);
+        if (INTER) {
 #pragma unroll
-      for (int k = 0; k < kItems; ++k) {
-        if (u0 + k * step >= items) break;
-        const Item it = item_at(u0 + k * step);
-        T* dst = dest(it.h);
-        if (!dst) continue;
-        if (it.turn) {
-          float x0[8], x1[8];
-          unpack8<T>(v0[k], x0);
-          unpack8<T>(v1[k], x1);
-          if (INTER) {
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float2 p = cs[it.d0 / 2 + e / 2], r = cs[it.d1 / 2 + e / 2];
-              const float a0 = x0[e], a1 = x1[e];
-              x0[e] = a0 * p.x - x0[e + 1] * p.y;
-              x0[e + 1] = x0[e + 1] * p.x + a0 * p.y;
-              x1[e] = a1 * r.x - x1[e + 1] * r.y;
-              x1[e + 1] = x1[e + 1] * r.x + a1 * r.y;
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 p = cs[it.d0 + e];
-              const float a0 = x0[e];
-              x0[e] = a0 * p.x - x1[e] * p.y;
-              x1[e] = x1[e] * p.x + a0 * p.y;
-            }
+          for (int e = 0; e < 8; e += 2) {
+            const float2 p = cs[it.d0 / 2 + e / 2], r = cs[it.d1 / 2 + e / 2];
+            const float a0 = x0[e], a1 = x1[e];
+            x0[e] = a0 * p.x - x0[e + 1] * p.y;
+            x0[e + 1] = x0[e + 1] * p.x + a0 * p.y;
+            x1[e] = a1 * r.x - x1[e + 1] * r.y;
+            x1[e + 1] = x1[e + 1] * r.x + a1 * r.y;
           }
-          v0[k] = pack8<T>(x0);
-          v1[k] = pack8<T>(x1);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 p = cs[it.d0 + e];
+            const float a0 = x0[e];
+            x0[e] = a0 * p.x - x1[e] * p.y;
+            x1[e] = x1[e] * p.x + a0 * p.y;
+          }
         }
-        *reinterpret_cast<uint4*>(dst + it.d0) = v0[k];
-        *reinterpret_cast<uint4*>(dst + it.d1) = v1[k];
+        v0 = pack8<T>(x0);
+        v1 = pack8<T>(x1);
       }
+      *reinterpret_cast<uint4*>(dst + it.d0) = v0;
+      *reinterpret_cast<uint4*>(dst + it.d1) = v1;
     }
   } else {
     const int pairs = half + (a.hd - a.rot);
