@@ -50,20 +50,20 @@ class SharedPrefixPlan:
     order of the groups, their requests and their queries."""
 
     def __init__(self, groups: Sequence[PrefixGroup], kv, num_q_heads: int):
-        bs, total = kv.block_size, kv.pages_total
+        bs = kv.block_size
         prefix, own, pages, t = [], [], [], 0
         for i, g in enumerate(groups):
             first, at = t, len(pages)
-            pages += plans.check_pages(g.pages, g.length, bs, total, f"prefix {i}")
+            pages += plans.take_pages(g.pages, g.length, bs, f"prefix {i}")
             for j, (p, n, q) in enumerate(g.requests):
                 if q < 0 or q > n:
                     raise ValueError(f"group {i}, request {j}: {q} queries of {n} own tokens")
                 own.append(plans.Span(t, q, n, n - q + 1, len(pages)))
-                pages += plans.check_pages(p, n, bs, total, f"group {i}, request {j}")
+                pages += plans.take_pages(p, n, bs, f"group {i}, request {j}")
                 t += q
             prefix.append(plans.Span(first, t - first, g.length, plans.NO_LIMIT, at))
         self.tokens, self.num_q_heads = t, int(num_q_heads)
-        blob, table = plans.build(prefix + own, np.array(pages, dtype=np.int64), t, self.num_q_heads,
+        blob, table = plans.build(prefix + own, plans.page_array(pages, kv.pages_total), t, self.num_q_heads,
                                   kv.num_kv_heads, _sms(kv.pool.device.index), tiles=kv.tiles)
         blob = plans.append_sections(blob, table, chunks=np.zeros(0), requests=np.zeros(0))
         self._native = native().CachePlan(torch.from_numpy(blob), kv, table)
@@ -74,7 +74,11 @@ def shared_prefix_attention(q: torch.Tensor, kv, layer: int, plan: SharedPrefixP
     """softmax(scale q K^T) V of queries ``q`` [tokens, q heads, head_dim] over
     their group's prefix and their request's own tokens in ``layer`` of the
     cache, the keys of a prefix read once for all its requests.  Queries that
-    see no key give zeros.  ``scale`` defaults to head_dim ** -0.5."""
+    see no key give zeros.  ``scale`` (positive) defaults to head_dim ** -0.5.
+
+    Cache slots past a request's tokens may hold anything; the values of a
+    request's asked tokens must be finite, since queries of one call that come
+    before a token meet its values with weight zero."""
     return native().cached_attention(q, kv, layer, plan._native, scale, out, None)
 
 
@@ -93,10 +97,10 @@ class DecodePlan:
                  newest: Optional[Sequence[int]] = None):
         if len(tables) != len(lengths) or (newest is not None and len(newest) != len(lengths)):
             raise ValueError("tables, lengths and newest must have one entry per request")
-        spans, pages, chunks, reqs, cols, col = [], [], [], [], [], 0
+        spans, pages, chunks, reqs, cols, col, bs = [], [], [], [], [], 0, kv.block_size
         for i, (table, n) in enumerate(zip(tables, lengths)):
             at = len(pages)
-            pages += plans.check_pages(table, n, kv.block_size, kv.pages_total, f"request {i}")
+            pages += plans.take_pages(table, n, bs, f"request {i}")
             spans.append(plans.Span(i, 1, n, n, at))
             last = n - 1 if newest is None else int(newest[i])
             reqs.append((n, at, last, 0))
@@ -108,7 +112,7 @@ class DecodePlan:
         self.lengths: List[int] = list(lengths)
         self.longest = max(self.lengths, default=0)
         self.num_q_heads = int(num_q_heads)
-        blob, table = plans.build(spans, np.array(pages, dtype=np.int64), len(spans), self.num_q_heads,
+        blob, table = plans.build(spans, plans.page_array(pages, kv.pages_total), len(spans), self.num_q_heads,
                                   kv.num_kv_heads, _sms(kv.pool.device.index), score_cols=cols)
         blob = plans.append_sections(blob, table, chunks=np.array(chunks), requests=np.array(reqs))
         table.update(chunks=len(chunks), requests=len(reqs), most_tokens=self.longest, score_cols=col)
@@ -121,7 +125,9 @@ def weighted_decode_attention(q: torch.Tensor, kv, layer: int, plan: DecodePlan,
     """Attention of one query per request, ``q`` [requests, q heads, head_dim],
     over its cached tokens; ``weights`` gains, at each token's slot and KV
     head, the softmax weight that the head's query group gave it (summed over
-    the group, fp32).  Requests without tokens give zeros."""
+    the group, fp32; one writer a slot, so that a repeat gives the same bits).
+    Requests without tokens give zeros.  ``scale`` (positive) defaults to
+    head_dim ** -0.5."""
     return native().cached_attention(q, kv, layer, plan._native, scale, out, weights)
 
 

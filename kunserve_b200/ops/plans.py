@@ -54,10 +54,10 @@ def _row_tiles(spans: Sequence[Span], group: int, rows: int) -> np.ndarray:
     return np.array(out, dtype=np.int64).reshape(-1, 8)
 
 
-def _parts(stages: np.ndarray, share: int) -> np.ndarray:
-    """Equal ranges of at most ``share`` stages per tile."""
+def _parts(stages: np.ndarray, share: np.ndarray) -> np.ndarray:
+    """Equal ranges of at most ``share`` stages per tile (of one stage at least)."""
     parts = -(-stages // share)
-    return -(-stages // np.maximum(-(-stages // np.maximum(parts, 1)), 1))   # no empty range at the end
+    return -(-stages // -(-stages // parts))         # no empty range at the end
 
 
 def _cut(tiles: np.ndarray, kv_heads: int, slots: int, stage: int, least: int, start: float) -> np.ndarray:
@@ -75,17 +75,12 @@ def _cut(tiles: np.ndarray, kv_heads: int, slots: int, stage: int, least: int, s
     most, total = int(stages.max()), int(stages.sum()) * kv_heads
     extra = start + tiles[:, 1] * tiles[:, 2] / 8.0 * STAGE_KEYS / stage
     tries = {-(-most // k) for k in range(1, 49)} | {-(-total * k // (slots * 8)) for k in range(1, 17)}
-    best = None
-    for c in sorted({max(least, t) for t in tries}):
-        parts = _parts(stages, c)
-        each = -(-stages // parts) + extra
-        n = int(parts.sum()) * kv_heads
-        cost = float(each.max()) + int(parts.max()) / 32.0
-        if n > slots:
-            cost += float((each * parts).sum()) * kv_heads / slots
-        if best is None or cost < best[0]:
-            best = (cost, parts)
-    parts = best[1]
+    parts = _parts(stages, np.array(sorted({max(least, t) for t in tries}))[:, None])   # [tries, tiles]
+    each = -(-stages // parts) + extra
+    units = parts.sum(axis=1) * kv_heads
+    cost = each.max(axis=1) + parts.max(axis=1) / 32.0 + np.where(
+        units > slots, (each * parts).sum(axis=1) * kv_heads / slots, 0.0)
+    parts = parts[int(cost.argmin())]
     each = -(-stages // parts)
     idx = np.repeat(np.arange(len(tiles)), parts)
     k = np.arange(len(idx)) - np.repeat(np.cumsum(parts) - parts, parts)
@@ -163,16 +158,20 @@ def append_sections(blob: np.ndarray, table: Dict[str, int], **sections: np.ndar
     return np.concatenate([blob, more])
 
 
-def check_pages(pages: Sequence[int], tokens: int, block_size: int, pages_total: int, what: str) -> List[int]:
-    """The pages that hold ``tokens`` tokens, checked against the cache."""
-    if tokens < 0:
+def take_pages(pages: Sequence[int], tokens: int, block_size: int, what: str) -> List[int]:
+    """The pages that hold ``tokens`` tokens, first of a page list."""
+    if not 0 <= tokens < NO_LIMIT:
         raise ValueError(f"{what}: {tokens} tokens")
-    if tokens >= NO_LIMIT:
-        raise ValueError(f"{what}: {tokens} tokens are too many")
     need = -(-tokens // block_size)
-    pages = list(pages)[:need]
+    pages = list(pages[:need])
     if len(pages) < need:
         raise ValueError(f"{what}: {tokens} tokens need {need} pages of {block_size}, got {len(pages)}")
-    if pages and (min(pages) < 0 or max(pages) >= pages_total):
-        raise ValueError(f"{what}: page ids must lie in [0, {pages_total}), got {min(pages)} to {max(pages)}")
     return pages
+
+
+def page_array(pages: Sequence[int], pages_total: int) -> np.ndarray:
+    """All page lists of a plan, every id checked against the cache."""
+    a = np.array(pages, dtype=np.int64)
+    if a.size and not (0 <= int(a.min()) and int(a.max()) < pages_total):
+        raise ValueError(f"page ids must lie in [0, {pages_total}), got {int(a.min())} to {int(a.max())}")
+    return a

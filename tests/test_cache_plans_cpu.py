@@ -97,11 +97,15 @@ def test_long_contexts_spread_over_the_gpu():
 
 
 def test_page_checks():
-    assert plans.check_pages([3, 4, 5], 17, 16, 6, "x") == [3, 4]
-    assert plans.check_pages([], 0, 16, 6, "x") == []
-    for pages, n in (([3], 17), ([6], 1), ([-1], 1), ([0], -1), ([0], 1 << 31)):
+    assert plans.take_pages([3, 4, 5], 17, 16, "x") == [3, 4]
+    assert plans.take_pages([], 0, 16, "x") == []
+    for pages, n in (([3], 17), ([0], -1), ([0], 1 << 31)):
         with pytest.raises(ValueError):
-            plans.check_pages(pages, n, 16, 6, "x")
+            plans.take_pages(pages, n, 16, "x")
+    assert plans.page_array([0, 5, 5], 6).tolist() == [0, 5, 5] and plans.page_array([], 6).size == 0
+    for pages in ([6], [-1], [0, 7, 2]):
+        with pytest.raises(ValueError):
+            plans.page_array(pages, 6)
     with pytest.raises(ValueError):
         plans.build([], np.zeros(0), 0, 5, 2, 148)
     with pytest.raises(ValueError):
