@@ -86,7 +86,8 @@ def _cut(tiles: np.ndarray, kv_heads: int, slots: int, stage: int, least: int, s
     k = np.arange(len(idx)) - np.repeat(np.cumsum(parts) - parts, parts)
     lo = k * each[idx] * stage
     hi = np.minimum(lo + each[idx] * stage, tiles[idx, 4])
-    return np.concatenate([tiles[idx], lo[:, None], hi[:, None]], axis=1)
+    cut = np.concatenate([tiles[idx], lo[:, None], hi[:, None]], axis=1)
+    return cut[np.argsort(lo - hi, kind="stable")]   # the longest start first
 
 
 def build(spans: Sequence[Span], pages: np.ndarray, tokens: int, num_q_heads: int, kv_heads: int, sms: int,
