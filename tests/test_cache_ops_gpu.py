@@ -375,6 +375,18 @@ def test_attention_across_32_bit_offsets():
     _within(got[0], o, tol)
     want = p.view(nkv, 2, n).sum(1)
     _within(w[pages].transpose(0, 1).reshape(nkv, -1)[:, :n], want, rel * want)
+    # the same pages as a prefix of 15 requests: 30 rows, the tile kernel
+    from kunserve_b200.ops import PrefixGroup, SharedPrefixPlan, shared_prefix_attention
+    own = [68000 + i for i in range(15)]
+    for i, page in enumerate(own):
+        _fill(pool, lay, [page], 3, 0, 1, 50 + i)
+    q = torch.randn(15, 16, hd, device="cuda").to(BF)
+    plan = SharedPrefixPlan([PrefixGroup(pages, n, [([page], 3, 1) for page in own])], kv, 16)
+    got = shared_prefix_attention(q, kv, 0, plan)
+    for i, page in enumerate(own):
+        ok, ov = (_rows(pool, lay, [page], 3, 0, 1, x) for x in (False, True))
+        o, tol, _, _ = _attend(q[i], torch.cat([k, ok]), torch.cat([v, ov]), 1 / math.sqrt(hd), U[BF])
+        _within(got[i], o, tol)
 
 
 # ------------------------------------------------ weighted decode attention
