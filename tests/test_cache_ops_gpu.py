@@ -52,12 +52,16 @@ def _rows(pool, lay, pages, n, layer, fusion, value):
     return torch.cat(got)[:n] if got else pool.new_zeros(0, lay.num_kv_heads, lay.head_dim)
 
 
-def _fill(pool, lay, pages, n, layer, fusion, seed):
-    """Random keys and values in the first n slots behind a page list."""
+def _fill(pool, lay, pages, n, layer, fusion, seed, ramp=False):
+    """Random keys and values in the first n slots behind a page list; with
+    ``ramp`` the keys grow along the list."""
     g = torch.Generator(device="cuda").manual_seed(seed)
     bs, per = lay.block_size, lay.num_kv_heads * lay.head_dim
     for value in (False, True):
-        x = torch.randn(n, per, generator=g, device="cuda").to(pool.dtype)
+        x = torch.randn(n, per, generator=g, device="cuda")
+        if ramp and not value:
+            x *= torch.linspace(0.2, 8.0, n, device="cuda")[:, None]
+        x = x.to(pool.dtype)
         for i in range(-(-n // bs) if n else 0):
             o = lay.kv_offset(pages[i], layer, fusion, value) // 2
             part = x[i * bs:(i + 1) * bs]
@@ -265,7 +269,8 @@ def _allot(lens, block, total, seed):
     return out
 
 
-def _shared_case(groups, nq, nkv, hd, dtype, block, fusion=1, extend=0, amp=1.0, strided=False, seed=0):
+def _shared_case(groups, nq, nkv, hd, dtype, block, fusion=1, extend=0, amp=1.0, strided=False, seed=0,
+                 ramp=False):
     """groups: [(prefix length, [(own tokens, queries), ...]), ...].  Runs the
     operator on a cache whose every other slot is NaN and checks every row."""
     from kunserve_b200.ops import PrefixGroup, SharedPrefixPlan, shared_prefix_attention
@@ -276,7 +281,7 @@ def _shared_case(groups, nq, nkv, hd, dtype, block, fusion=1, extend=0, amp=1.0,
     pages = _allot(lens, block, kv.pages_total, seed)
     layer = 1
     for i, (p, n) in enumerate(zip(pages, lens)):
-        _fill(pool, lay, p, n, layer, fusion, 100 + i)
+        _fill(pool, lay, p, n, layer, fusion, 100 + i, ramp)
     it = iter(pages)
     plan_groups = []
     for p, reqs in groups:
@@ -338,6 +343,19 @@ def test_shared_prefix_query_chunks(queries):
 
 def test_shared_prefix_fused_page_ids():
     _shared_case(ODD, 8, 2, 128, BF, 16, fusion=2, extend=4)
+    _shared_case([(300, [(1 + i, 1) for i in range(9)])], 8, 2, 64, FP, 16, fusion=2, extend=9)   # the tile kernel
+
+
+@pytest.mark.parametrize("hd,dtype", [(128, BF), (64, FP)])
+def test_shared_prefix_growing_scores(hd, dtype):
+    """Each block of keys outgrows the maxima of the ones before, in both kernels."""
+    _shared_case([(1000, [(5, 1)] * 12), (900, [(150, 1)])], 8, 2, hd, dtype, 16, amp=4.0, ramp=True)
+
+
+def test_shared_prefix_many_units():
+    """More tile units than SMs: each CTA takes several, of ragged ends."""
+    _shared_case([(650 + 17 * i, [(1 + j % 3, 1) for j in range(6)]) for i in range(12)], 32, 8, 128, FP, 16)
+    _shared_case([(130 + 61 * i, [(2, 1 + j % 2) for j in range(20)]) for i in range(25)], 8, 8, 64, BF, 8, amp=3.0)
 
 
 @pytest.mark.parametrize("amp", [0.0, 30.0])
