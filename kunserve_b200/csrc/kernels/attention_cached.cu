@@ -276,10 +276,12 @@ __global__ void __launch_bounds__(32) rows_kernel(CachedAttn a, float scale_log2
 }
 
 // ------------------------------------------------------------------ joins
-// (M, L) of two parts: the larger max, the sums brought to it.
+// (M, L) of two parts: the larger max, the sums brought to it.  The maxima
+// skip NaN scores; the sums hold them, and keep what they hold here: a row
+// with a NaN score has no softmax, its output is NaN.
 KUS_DEVICE float2 join2(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x);
-  if (m == -INFINITY) return make_float2(m, 0.f);
+  if (m == -INFINITY) return make_float2(m, a.y + b.y);   // zeros or NaN
   return make_float2(m, a.y * ex2(a.x - m) + b.y * ex2(b.x - m));
 }
 KUS_DEVICE float2 warp_join(float2 s) {
@@ -288,6 +290,9 @@ KUS_DEVICE float2 warp_join(float2 s) {
     s = join2(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, off), __shfl_xor_sync(0xffffffffu, s.y, off)));
   return s;
 }
+
+// 1 / L; zero for a row without keys.
+KUS_DEVICE float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // Partial row of list entry p for a KV head and a head of its group.
 KUS_DEVICE long long part_row(int2 p, int kh, int g) { return p.x + (long long)kh * p.y + g; }
@@ -412,7 +417,7 @@ __global__ void __launch_bounds__(32 * (W > 4 ? W : 4), W > 4 ? 4 : 8) join_kern
       st = all;
     }
     if (!have) return;
-    const float inv = st.y > 0.f ? 1.f / st.y : 0.f;
+    const float inv = inverse_sum(st.y);
     T* dst = reinterpret_cast<T*>(a.out) + t * a.ot + h * a.oh + lane * kPer;
 #pragma unroll
     for (int i = 0; i < kPer; i += 2)
