@@ -293,6 +293,8 @@ KUS_DEVICE float2 warp_join(float2 s) {
 
 // 1 / L; zero for a row without keys.
 KUS_DEVICE float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
+// What scores are taken against: M, or zero where all of them are -inf.
+KUS_DEVICE float score_ref(float m) { return m == -INFINITY ? 0.f : m; }
 
 // Partial row of list entry p for a KV head and a head of its group.
 KUS_DEVICE long long part_row(int2 p, int kh, int g) { return p.x + (long long)kh * p.y + g; }
@@ -440,8 +442,8 @@ __global__ void __launch_bounds__(32 * (W > 4 ? W : 4), W > 4 ? 4 : 8) join_kern
       }
       st = warp_join(st);
       if (lane == 0) {
-        sh_m[g] = st.x;
-        sh_l[g] = 1.f / st.y;
+        sh_m[g] = score_ref(st.x);
+        sh_l[g] = inverse_sum(st.y);
       }
     }
   pdl_wait();
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(kJoinThreads, 8) weights_kernel(CachedAttn a) 
   pdl_wait();
   if (threadIdx.x < G) {
     const float2 st = __ldcg(a.stats + (long long)t * a.nq + kh * G + threadIdx.x);
-    sh_m[threadIdx.x] = st.x;
+    sh_m[threadIdx.x] = score_ref(st.x);
     sh_l[threadIdx.x] = st.y;
   }
   __syncthreads();

@@ -126,8 +126,8 @@ def weighted_decode_attention(q: torch.Tensor, kv, layer: int, plan: DecodePlan,
     over its cached tokens; ``weights`` gains, at each token's slot and KV
     head, the softmax weight that the head's query group gave it (summed over
     the group, fp32; one writer a slot, so that a repeat gives the same bits).
-    Requests without tokens give zeros.  ``scale`` (positive) defaults to
-    head_dim ** -0.5."""
+    Requests without tokens, and rows whose scores are all -inf, give zeros and
+    add no weight.  ``scale`` (positive) defaults to head_dim ** -0.5."""
     return native().cached_attention(q, kv, layer, plan._native, scale, out, weights)
 
 

@@ -134,3 +134,21 @@ def test_weighted_rows_without_a_softmax(n, where):
         p = want[i][2].view(NKV, G, m).sum(1)
         assert added[lost].isnan().all()
         _within(added[~lost], p[~lost], (want[i][3] + 2.0 ** -23) * p[~lost])
+
+
+@pytest.mark.parametrize("n", [5, 3000])
+def test_all_scores_minus_infinity(n):
+    """No key of finite score: zeros, and no weight is added."""
+    from kunserve_b200.ops import DecodePlan, weighted_decode_attention
+    hd = 64
+    pool, kv, lay = _cache(-(-n // BS) + 1, BS, NKV, hd, BF, poison=True)
+    pages = _allot([n], BS, kv.pages_total, 1)
+    _fill(pool, lay, pages[0], n, 1, 1, 0)
+    for page in pages[0]:
+        o = lay.kv_offset(page, 1, 1, False) // 2
+        pool[o:o + BS * NKV * hd].view(BS, NKV, hd)[:, 0, 2] = -math.inf
+    q = torch.rand(1, NQ, hd, device="cuda").to(BF) + 1.0
+    w = torch.ones(kv.pages_total, NKV, BS, device="cuda")
+    got = weighted_decode_attention(q, kv, 1, DecodePlan(pages, [n], kv, NQ), w)
+    assert (got[0, :G] == 0).all() and torch.isfinite(got.float()).all()
+    assert (w[:, 0] == 1).all() and torch.isfinite(w).all()
