@@ -86,6 +86,12 @@ KUS_DEVICE uint32_t swz(int r, int ch) {
 // Rounded part and remainder of two values as packed 16-bit pairs: hi + lo
 // carries about 16 bits of P, so the product with V loses nothing that shows
 // in a 16-bit output.  The second product is free where HBM is the bound.
+// In fp16 the probabilities are taken 2^15 times too large (P <= 2^15, the
+// sum with it): its exponents end at 2^-24, and many light keys together may
+// hold weight that a long context's output shows.  What is below 2^-40 of the
+// row's largest still vanishes.
+template <typename T>
+constexpr float kUpLog2 = std::is_same<T, __half>::value ? 15.f : 0.f;
 template <typename T>
 KUS_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = pack2<T>(a, b);
@@ -172,7 +178,7 @@ __global__ void __launch_bounds__(32) rows_kernel(CachedAttn a, float scale_log2
   float o[HD / 8][4];
 #pragma unroll
   for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};   // m: the max so far, less kUpLog2
   float* srow = nullptr;
   long long spitch = 0;
   if (SCORES) {
@@ -221,7 +227,7 @@ __global__ void __launch_bounds__(32) rows_kernel(CachedAttn a, float scale_log2
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[hi], mx);
+      const float mn = fmaxf(m[hi], mx - kUpLog2<T>);
       const float ref = mn == -INFINITY ? 0.f : mn;   // no key seen yet
       alpha[hi] = ex2(m[hi] - ref);
       m[hi] = mn;

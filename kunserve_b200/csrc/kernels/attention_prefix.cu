@@ -19,9 +19,9 @@
 // QK(i + 1) and PV(i - 1) run while block i's softmax does, which is what
 // bounds an iteration.  Blocks of 128 keys and not 64: the tensor core reads
 // Q from shared memory once per block, which at N = 64 takes longer than the
-// products.  Probabilities are taken against a row's max so far; only where
-// the block's is more than 2^8 times as large are they taken again and O
-// rescaled (the sum and O share the stale max).
+// products.  Probabilities are taken against a row's reference, at most a
+// range above which they are taken again and O rescaled (the sum and O share
+// the reference, whatever it is): struct Range.
 //
 // A block of 128 rows and keys takes about 1950 clk: 1024 of exponentials (16
 // a clk), the rest waits around them; the products take 1400 beside that.
@@ -51,7 +51,21 @@ constexpr int kThreads = kSoftmax + 128;
 constexpr uint32_t kCols = 512;          // S0, S1 [0, 256), P0, P1 [256, 384), O [384, 384 + HD)
 constexpr uint32_t kColP = 256;
 constexpr uint32_t kColO = 384;
-constexpr float kRescaleLog2 = 8.0f;
+
+// Probabilities P = 2^(s - m) of 16 bits, by element type: m is set kUp below
+// a row's max, and again once a P would exceed 2^kMost.  bf16 has fp32's
+// exponents: m is the max, and P up to 2^8 leaves it be.  fp16's end at
+// 2^-24: P of up to 2^15 let a weight of 2^-36 of the row's largest still
+// count (many light keys hold what a long context's output shows), and a max
+// may grow 2^4 times before m follows.
+template <typename T>
+struct Range {
+  static constexpr float kUp = 0.f, kMost = 8.f;
+};
+template <>
+struct Range<__half> {
+  static constexpr float kUp = 11.f, kMost = 15.f;
+};
 
 template <int HD>
 struct Cfg {
@@ -401,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           for (int e = 0; e < 64; ++e)
             if (e >= left) v[e] = 0xff800000u;   // -inf
         }
-        // Probabilities against the max so far, the block's own max beside
+        // Probabilities against the reference so far, the block's own max beside
         // them: it is only seldom needed, and the exponentials bound this loop.
         uint32_t pk[32];
         float sum;
@@ -425,14 +439,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           mx[1] = max3(mx[1], __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
         }
         const float top = fmaxf(mx[0], mx[1]) * scale_log2;
-        if (barrier_any(1 + (warp & 3), 64, top > m + kRescaleLog2)) {
-          // some row of this pair of warps outgrew its max
+        if (barrier_any(1 + (warp & 3), 64, top > m + Range<T>::kMost)) {
+          // some row of this pair of warps outgrew its reference
           float* mine = maxima + r;
           mine[half * kRows] = top;
           named_barrier(1 + (warp & 3), 64);
           const float both = fmaxf(top, mine[(half ^ 1) * kRows]);
-          const bool grow = both > m + kRescaleLog2;
-          const float mn = grow ? both : m;
+          const bool grow = both > m + Range<T>::kMost;
+          const float mn = grow ? both - Range<T>::kUp : m;
           const float alpha = grow ? ex2(m - mn) : 1.f;
           probabilities(mn == -INFINITY ? 0.f : mn);   // no key seen yet: zeros
           if (i > 0) {

@@ -74,11 +74,11 @@ struct CachedAttn {
   int head_chunks;
   int most_parts;                // longest of those lists
   float* part_o;                 // [partial rows, hd]
-  float2* part_ml;               // [partial rows] running max (log2 units), sum
+  float2* part_ml;               // [partial rows] reference of the sums (log2 units, near the max), sum
   // weighted plans: scores [request][nq][keys rounded up to 16] fp32, the
   // weights [pages, kvh, block_size] that each key's attention is added to
   float* scores;
-  float2* stats;                 // [T, nq] (max, 1 / sum) of weighted plans
+  float2* stats;                 // [T, nq] (reference, 1 / sum) of weighted plans
   float* weights;
   const int* chunks;             // [n_chunks, kChunkInts]
   int n_chunks;
