@@ -91,7 +91,9 @@ class DecodePlan:
     length less one; more once tokens were evicted).  Weights (fp32) and slot
     positions (int32) of a layer are [``kv.pages_total``, kv heads,
     block_size]: after evictions every KV head holds other tokens in a
-    request's slots."""
+    request's slots.  The pages that hold tokens must be the request's own:
+    a page listed twice is refused, since both its weights and its slots would
+    change under two requests at once."""
 
     def __init__(self, tables: Sequence[Sequence[int]], lengths: Sequence[int], kv, num_q_heads: int,
                  newest: Optional[Sequence[int]] = None):
@@ -109,11 +111,13 @@ class DecodePlan:
             col += -(-n // plans.STAGE_KEYS) * plans.STAGE_KEYS
         if reqs and not -2 ** 31 <= min(r[2] for r in reqs) <= max(r[2] for r in reqs) < 2 ** 31:
             raise ValueError("newest positions must fit 32 bits")
+        page_ids = plans.page_array(pages, kv.pages_total)
+        plans.check_distinct(page_ids)
         self.lengths: List[int] = list(lengths)
         self.longest = max(self.lengths, default=0)
         self.num_q_heads = int(num_q_heads)
-        blob, table = plans.build(spans, plans.page_array(pages, kv.pages_total), len(spans), self.num_q_heads,
-                                  kv.num_kv_heads, _sms(kv.pool.device.index), score_cols=cols)
+        blob, table = plans.build(spans, page_ids, len(spans), self.num_q_heads, kv.num_kv_heads,
+                                  _sms(kv.pool.device.index), score_cols=cols)
         blob = plans.append_sections(blob, table, chunks=np.array(chunks), requests=np.array(reqs))
         table.update(chunks=len(chunks), requests=len(reqs), most_tokens=self.longest, score_cols=col)
         self._native = native().CachePlan(torch.from_numpy(blob), kv, table)

@@ -176,3 +176,11 @@ def page_array(pages: Sequence[int], pages_total: int) -> np.ndarray:
     if a.size and not (0 <= int(a.min()) and int(a.max()) < pages_total):
         raise ValueError(f"page ids must lie in [0, {pages_total}), got {int(a.min())} to {int(a.max())}")
     return a
+
+
+def check_distinct(pages: np.ndarray) -> None:
+    """Every page of the plan's lists is listed once."""
+    ids, times = np.unique(pages, return_counts=True)
+    if ids.size < pages.size:
+        raise ValueError(f"page {int(ids[times.argmax()])} is listed {int(times.max())} times; slots that gain "
+                         "weight and move must belong to one request")
