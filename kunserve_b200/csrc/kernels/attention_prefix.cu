@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
           const int c = half * kEach + e;
-          const uint4 v = valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+          const uint4 v = valid ? src[c] : make_uint4(0, 0, 0, 0);
           *reinterpret_cast<uint4*>(smem + (c >> 3) * Cf::kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

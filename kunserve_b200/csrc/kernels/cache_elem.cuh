@@ -56,6 +56,8 @@ KUS_DEVICE float ex2(float x) {
 // a grid is set up while the one before it ends.  Every kernel of the cache
 // operators waits for the one before (pdl_wait) ahead of its first access to
 // what others write; only plans, which no kernel writes, are read earlier.
+// They alone may be read with __ldg: it takes memory for read-only while the
+// grid lives, and the grid before may still be writing when this one starts.
 struct LaunchBehind {
   const bool was = pdl_flag();
   LaunchBehind() { pdl_flag() = true; }

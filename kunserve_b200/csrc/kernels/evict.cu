@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(NT) select_kernel(EvictSelect a, int ctas, int
   const int lo = min(n, rank * slice), hi = min(n, lo + slice);
   auto read_key = [&](int i) {
     const long long at = side_at(a.g, __ldg(table + kv_page_col(a.g, i)), kh, i);
-    return rank_key(__ldg(a.weights + at), __ldg(a.slot_positions + at), a.sinks, rq.z, a.recent);
+    return rank_key(a.weights[at], a.slot_positions[at], a.sinks, rq.z, a.recent);
   };
   auto key_of = [&](int i) { return CACHED ? keys[i - lo] : read_key(i); };
 
@@ -116,8 +116,8 @@ __global__ void __launch_bounds__(NT) select_kernel(EvictSelect a, int ctas, int
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         const long long at = side_at(a.g, max(page[b], 0), kh, i0 + b * NT);
-        w[b] = page[b] >= 0 ? __ldg(a.weights + at) : 0.f;
-        pos[b] = page[b] >= 0 ? __ldg(a.slot_positions + at) : 0;
+        w[b] = page[b] >= 0 ? a.weights[at] : 0.f;
+        pos[b] = page[b] >= 0 ? a.slot_positions[at] : 0;
       }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b)
