@@ -19,7 +19,8 @@
 
 namespace kus {
 
-// Error codes written to g_kus_error (first writer wins).
+// Error codes written to g_kus_error: the first wait that ran out, else the
+// first bad index.
 enum : int {
   kErrNone = 0,
   kErrWaitFull = 1,     // producer->consumer smem stage never filled
@@ -36,10 +37,19 @@ __device__ int g_kus_error = 0;
 __device__ int g_kus_error_info = 0;
 
 KUS_DEVICE void set_error(int code, int info = 0) {
-  if (atomicCAS(&g_kus_error, 0, code) == 0) g_kus_error_info = info;
+  const int was = atomicCAS(&g_kus_error, 0, code);
+  if (was == 0 || (was == kErrBounds && code != kErrBounds &&
+                   atomicCAS(&g_kus_error, kErrBounds, code) == kErrBounds))
+    g_kus_error_info = info;
 }
 
-KUS_DEVICE bool error_set() { return *(volatile int*)&g_kus_error != 0; }
+// Whether some wait ran out: the others then give up early, since what they
+// wait for may never come.  A bad index is no reason to (its access was left
+// out, everything else goes on).
+KUS_DEVICE bool wait_failed() {
+  const int e = *(volatile int*)&g_kus_error;
+  return e != 0 && e != kErrBounds;
+}
 
 // A legitimate wait in this library lasts microseconds (a pipeline stage) to
 // milliseconds (a peer rank's kernel); two seconds means a lost arrival.
@@ -179,7 +189,7 @@ KUS_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity, int err_code) {
   for (uint32_t i = 1; i < kSpinLimit; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 255u) == 0) {
-      if (error_set()) return false;
+      if (wait_failed()) return false;
       if (global_ns() - t0 > kWaitNs) break;
     }
   }
@@ -246,7 +256,7 @@ KUS_DEVICE bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int err_code) 
   for (uint32_t i = 1; i < kSpinLimit; ++i) {
     if (mbar_try_wait_cluster(bar, parity)) return true;
     if ((i & 255u) == 0) {
-      if (error_set()) return false;
+      if (wait_failed()) return false;
       if (global_ns() - t0 > kWaitNs) break;
     }
   }

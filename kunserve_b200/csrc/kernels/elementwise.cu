@@ -480,7 +480,7 @@ __global__ void tp_reduce_rmsnorm_kernel(const __nv_bfloat16* __restrict__ rb, i
         asm volatile("ld.acquire.sys.global.u32 %0, [%1];" : "=r"(v) : "l"(flags + p) : "memory");
         if ((int)(v - epoch) >= 0) break;
         if (i >= (kSpinLimit >> 6) ||
-            ((i & 255u) == 255u && (error_set() || global_ns() - t0 > kWaitNs))) {
+            ((i & 255u) == 255u && (wait_failed() || global_ns() - t0 > kWaitNs))) {
           set_error(kErrPeerFlag, p);
           ok = 0;
           break;

@@ -109,7 +109,7 @@ __device__ __forceinline__ bool tail_arrive(const GemmArgs& a, int lt, int et, i
   named_barrier(1, 128);
   if (et == 0) {
     int last = 0;
-    if (!error_set()) {
+    if (!wait_failed()) {
       const int prev = atomicAdd(&a.tile_counters[lt], 1);
       last = (prev + 1 == a.tail_splits);
       if (last) a.tile_counters[lt] = 0;   // ready for the next GEMM
@@ -131,7 +131,7 @@ __device__ __forceinline__ bool sk_arrive(const GemmArgs& a, int sk, int kbs, in
   named_barrier(1, 128);
   if (et == 0) {
     int last = 0;
-    if (!error_set()) {
+    if (!wait_failed()) {
       const int prev = atomicAdd(&a.tile_counters[sk], kbs);
       last = (prev + kbs == a.num_kb);
       if (last) a.tile_counters[sk] = 0;   // ready for the next GEMM

@@ -259,7 +259,7 @@ KUS_DEVICE void ag_gather_slices(const GemmArgs& a, int gt) {
         unsigned v;
         asm volatile("ld.acquire.sys.global.u32 %0, [%1];" : "=r"(v) : "l"(a.ag_flags + q) : "memory");
         if ((int)(v - a.ag_epoch) >= 0) break;
-        if ((i & 255u) == 255u && (error_set() || global_ns() - t0 > kWaitNs)) {
+        if ((i & 255u) == 255u && (wait_failed() || global_ns() - t0 > kWaitNs)) {
           set_error(kErrPeerFlag, q);
           ok = false;
           break;
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kThreads + 32 * GW, 1)
           int v;
           asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(args.ag_ready + m) : "memory");
           if ((int)((unsigned)v - ready_target) >= 0) break;
-          if ((i & 255u) == 255u && (error_set() || global_ns() - t0 > kWaitNs)) {
+          if ((i & 255u) == 255u && (wait_failed() || global_ns() - t0 > kWaitNs)) {
             set_error(kErrPeerFlag, 100 + m);
             break;
           }
