@@ -182,14 +182,18 @@ KUS_DEVICE bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 }
 
 // Bounded wait: true when the phase with `parity` completed.  On a timeout
-// the error info holds (blockIdx.x << 8) | (warp << 1) | parity.
+// the error info holds (blockIdx.x << 8) | (warp << 1) | parity.  With DRAIN
+// it is a wait for what this CTA itself has in flight (copies, products),
+// which must end before the CTA does: bounded by time alone, whatever other
+// waits ran out.
+template <bool DRAIN = false>
 KUS_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity, int err_code) {
   if (mbar_try_wait(bar, parity)) return true;
   const unsigned long long t0 = global_ns();
   for (uint32_t i = 1; i < kSpinLimit; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 255u) == 0) {
-      if (wait_failed()) return false;
+      if (!DRAIN && wait_failed()) return false;
       if (global_ns() - t0 > kWaitNs) break;
     }
   }

@@ -88,8 +88,10 @@ struct Bars {
   uint64_t k_full[Cfg<HD>::kKStages], k_empty[Cfg<HD>::kKStages];
   uint64_t v_full[Cfg<HD>::kVStages], v_empty[Cfg<HD>::kVStages];
   uint64_t s_full[2], s_empty[2], p_full[2], pv_done[2];
+  uint64_t drained[2];   // all products of the issuers of QK, PV
   uint32_t tmem;
 };
+static_assert(sizeof(Bars<64>) <= 256 && sizeof(Bars<128>) <= 256, "they lie before the maxima");
 
 KUS_DEVICE void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
   asm volatile(
@@ -232,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       mbar_init(&bars->s_empty[b], kSoftmax);
       mbar_init(&bars->p_full[b], kSoftmax);
       mbar_init(&bars->pv_done[b], 1);
+      mbar_init(&bars->drained[b], 1);
     }
     fence_barrier_init();
   }
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     }
     // every load has landed before the CTA may leave
     for (int i = max(0, loaded - stages); i < loaded; ++i)
-      mbar_wait(&full[i % stages], (uint32_t)(i / stages) & 1u, kErrWaitFull);
+      mbar_wait<true>(&full[i % stages], (uint32_t)(i / stages) & 1u, kErrWaitFull);
     __syncwarp();
   } else if (warp == 10) {
     // ------------------------------------------------------- S = Q K^T
@@ -322,6 +325,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           }
         }
       }
+      // shared memory and TMEM stay until every product is done, whatever
+      // wait ran out (here or in the softmax)
+      umma_commit(&bars->drained[0]);
+      mbar_wait<true>(&bars->drained[0], 0, kErrWaitTmemFull);
     }
     __syncwarp();
   } else if (warp == 11) {
@@ -365,6 +372,11 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
       }
     }
+    if (lane == 0) {
+      umma_commit(&bars->drained[1]);
+      mbar_wait<true>(&bars->drained[1], 0, kErrWaitTmemFull);
+    }
+    __syncwarp();
   } else {
     // --------------------------------------------------- Q, softmax, output
     const int half = warp >> 2, r = threadIdx.x & (kRows - 1);   // TMEM lane of warp w: 32 (w % 4) + lane
