@@ -4,7 +4,8 @@ and eviction by those weights.
 
 A step makes one plan from the lengths and page lists the scheduler holds, and
 calls the operators with it for every layer.  All of them run on the current
-CUDA stream of the cache's device and allocate their scratch from it.
+CUDA stream of the cache's device and allocate their scratch from it.  They
+serve: their results carry no gradient.
 """
 import functools
 from typing import List, NamedTuple, Optional, Sequence, Tuple

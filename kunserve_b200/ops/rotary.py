@@ -104,6 +104,25 @@ class Rotary:
             self._native = native().RotaryTable(self.steps, self.scale, self.head_dim, self.interleaved)
 
 
+class _Turn(torch.autograd.Function):
+    """The rotation of a tensor whose gradient is asked for: a gradient turns
+    back (the map is linear, its transpose the rotation by the opposite angle
+    with the same factor)."""
+
+    @staticmethod
+    def forward(ctx, x, positions, rotary, inverse):
+        ctx.save_for_backward(positions)
+        ctx.rotary, ctx.inverse = rotary, inverse
+        return native().rotary_apply(x, positions, rotary._native, None, inverse)
+
+    @staticmethod
+    def backward(ctx, grad):
+        positions, = ctx.saved_tensors
+        if grad.stride(-1) != 1:          # broadcast from a sum, say
+            grad = grad.contiguous()
+        return rotary_apply(grad, positions, ctx.rotary, inverse=not ctx.inverse), None, None, None
+
+
 def rotary_apply(x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, out: Optional[torch.Tensor] = None,
                  inverse: bool = False) -> torch.Tensor:
     """``x`` [T, heads, head_dim] (bf16 or fp16, any strides between heads and
@@ -111,7 +130,12 @@ def rotary_apply(x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, out: 
 
     ``out`` may be ``x``.  ``inverse`` turns back; with the factor on cos and
     sin kept, that is the gradient: if y = rotary_apply(x), the gradient of x
-    is rotary_apply(gradient of y, inverse=True)."""
+    is rotary_apply(gradient of y, inverse=True).  Autograd does so where ``x``
+    requires a gradient; ``out`` is refused there."""
+    if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
+        if out is not None:
+            raise ValueError("rotary_apply: results written to out= carry no gradient, but an argument requires one")
+        return _Turn.apply(x, positions, rotary, inverse)
     return native().rotary_apply(x, positions, rotary._native, out, inverse)
 
 
@@ -126,5 +150,5 @@ def rotary_append(qkv: torch.Tensor, positions: torch.Tensor, pages: torch.Tenso
     ``qkv``.  For a cache that evicts by weight, ``weights`` and
     ``slot_positions`` (see ``DecodePlan``) get the new slots' zero weight and
     their token's position.  A page or slot outside the cache is not written;
-    ``check_error`` reports it."""
+    ``check_error`` reports it.  Nothing here carries a gradient."""
     native().rotary_append_scaled(qkv, positions, pages, slots, rotary._native, kv, layer, out, weights, slot_positions)
