@@ -180,17 +180,28 @@ bool heads_on_16(const torch::Tensor& t) {
 // The frequencies of a model's rotary positions (kunserve_b200/ops/rotary.py).
 struct RotaryTable {
   torch::Tensor steps;
+  c10::cuda::CUDAStream made_on;
   float scale;
   int hd, rot;
   bool interleaved;
 
   RotaryTable(torch::Tensor s, double scale_, int64_t hd_, bool interleaved_)
-      : steps(std::move(s)), scale((float)scale_), hd((int)hd_), rot(0), interleaved(interleaved_) {
+      : steps(std::move(s)),
+        made_on(c10::cuda::getCurrentCUDAStream(steps.is_cuda() ? steps.get_device() : -1)),
+        scale((float)scale_),
+        hd((int)hd_),
+        rot(0),
+        interleaved(interleaved_) {
     KUS_CHECK(steps.is_cuda() && steps.scalar_type() == torch::kInt64 && steps.is_contiguous() && steps.dim() == 1,
               "rotary steps must be a contiguous int64 CUDA tensor");
     const int64_t r = 2 * steps.numel();
     KUS_CHECK(r > 0 && r <= hd_ && r <= 4096, "rotary_dim ", r, " of head_dim ", hd_);
     rot = (int)r;
+  }
+  // The frequencies outlive the work queued on the current stream.
+  void use() const {
+    const auto st = at::cuda::getCurrentCUDAStream(steps.get_device());
+    if (st != made_on) steps.record_stream(st);
   }
 };
 
@@ -200,6 +211,7 @@ RotaryArgs rotary_args(const RotaryTable* table, const torch::Tensor& x, const t
   const int64_t hd = x.size(2);
   KUS_CHECK(hd == table->hd, "head_dim ", hd, ", the rotary frequencies have ", (int64_t)table->hd);
   check_index(positions, x.size(0), x, "positions");
+  table->use();
   KUS_CHECK(x.size(0) < (1LL << 31) && x.size(1) * hd < (1 << 23), "too many tokens or heads");
   RotaryArgs a{};
   a.x = x.data_ptr();
