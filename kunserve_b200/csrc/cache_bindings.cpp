@@ -344,7 +344,7 @@ std::tuple<torch::Tensor, torch::Tensor> select_evictions_op(const torch::Tensor
   c10::cuda::CUDAGuard guard(kv.pool.device());
   KUS_CHECK(plan.n_reqs > 0 || plan.T == 0, "eviction needs a decode plan");
   KUS_CHECK(keep > 0 && keep < (1LL << 31) && cap >= 0 && cap <= keep, "keep must be positive, got ", keep);
-  KUS_CHECK(sinks >= 0 && recent >= 0 && sinks + recent <= keep, "sinks (", sinks, ") and recent (", recent,
+  KUS_CHECK(sinks >= 0 && recent >= 0 && sinks <= keep && recent <= keep - sinks, "sinks (", sinks, ") and recent (", recent,
               ") must fit in keep (", keep, ")");
   kv.check_side(weights, torch::kFloat32, "weights");
   kv.check_side(slot_positions, torch::kInt32, "slot_positions");
