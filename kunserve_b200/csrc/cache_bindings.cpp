@@ -421,7 +421,14 @@ void bind_cache_ops(py::module& m) {
   m.def("cached_attention", &cached_attention_op);
   m.def("select_evictions", &select_evictions_op);
   m.def("compact_cache", &compact_cache_op);
-  m.attr("UNIT_INTS") = kUnitInts;
-  m.attr("ROW_UNIT_ROWS") = kRowUnitRows;
-  m.attr("TILE_UNIT_ROWS") = kTileUnitRows;
+  // what ops/plans.py lays plans out by
+  py::dict c;
+  c["UNIT_INTS"] = kUnitInts;
+  c["ROW_UNIT_ROWS"] = kRowUnitRows;
+  c["TILE_UNIT_ROWS"] = kTileUnitRows;
+  c["STAGE_KEYS"] = kStageKeys;
+  c["TILE_KEYS"] = kTileKeys;
+  c["CHUNK_KEYS"] = kChunkKeys;
+  c["NO_LIMIT"] = kNoLimit;
+  m.attr("PLAN_CONSTANTS") = c;
 }

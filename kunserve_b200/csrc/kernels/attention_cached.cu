@@ -26,7 +26,7 @@
 namespace kus {
 namespace cat {
 
-constexpr int kKeys = 32;       // keys per stage
+constexpr int kKeys = kStageKeys;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int HD>
@@ -314,7 +314,7 @@ KUS_DEVICE void add_weights(const CachedAttn& a, const int* c, int kh, const flo
   const long long pitch = (len + kKeys - 1) / kKeys * kKeys;
   const int key = c[1] + 4 * threadIdx.x;
   if (key >= key1) return;
-  // the rows of scores run on to a multiple of 16 keys
+  // the rows of scores run on to a multiple of kKeys
   const float* src = a.scores + (long long)col * a.nq + kh * G * pitch + key;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -347,6 +347,7 @@ KUS_DEVICE void add_weights(const CachedAttn& a, const int* c, int kh, const flo
 }
 
 constexpr int kJoinThreads = 128;
+static_assert(4 * kJoinThreads == kChunkKeys, "add_weights takes a chunk, four keys a thread");
 
 // Blocks [0, joins): W warps per (token, head) row join its parts, 4 / W rows
 // a block; with a.stats the row's M and 1 / L are kept.  Blocks after them

@@ -45,7 +45,7 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn();
 namespace cpt {
 
 constexpr int kRows = kTileUnitRows;
-constexpr int kKeys = 128;
+constexpr int kKeys = kTileKeys;
 constexpr int kSoftmax = 256;            // softmax threads: two a row
 constexpr int kThreads = kSoftmax + 128;
 constexpr uint32_t kCols = 512;          // S0, S1 [0, 256), P0, P1 [256, 384), O [384, 384 + HD)

@@ -48,10 +48,12 @@ void rotary(const RotaryArgs& a, int type, cudaStream_t s);
 constexpr int kUnitInts = 8;
 constexpr int kRowUnitRows = 16;     // most rows of a unit of the row kernel
 constexpr int kTileUnitRows = 128;   // most rows of a unit of the tile kernel
+constexpr int kStageKeys = 32;       // keys per stage of the row kernel; ranges and rows of scores are multiples
+constexpr int kTileKeys = 128;       // keys per block of the tile kernel; its ranges start on multiples
 constexpr int kNoLimit = 1 << 30;    // unit int 4 of keys without a causal limit
 // Ints of a weight chunk: token row, first key, end, first page, keys of the request, first score column.
 constexpr int kChunkInts = 6;
-constexpr int kChunkKeys = 512;
+constexpr int kChunkKeys = 512;      // keys of a chunk, at most
 
 struct CachedAttn {
   const void* q;                 // [T, nq, hd]
@@ -75,7 +77,7 @@ struct CachedAttn {
   int most_parts;                // longest of those lists
   float* part_o;                 // [partial rows, hd]
   float2* part_ml;               // [partial rows] reference of the sums (log2 units, near the max), sum
-  // weighted plans: scores [request][nq][keys rounded up to 16] fp32, the
+  // weighted plans: scores [request][nq][keys rounded up to kStageKeys] fp32, the
   // weights [pages, kvh, block_size] that each key's attention is added to
   float* scores;
   float2* stats;                 // [T, nq] (reference, 1 / sum) of weighted plans

@@ -26,8 +26,8 @@ namespace rot {
 constexpr int kThreads = 256;   // at most; a block has what its items divide into
 
 // VEC: 16-byte vectors (bases and strides of 16 bytes, hd and rot multiples
-// of 16, interleaved rot of 8); otherwise single elements, one pair or one
-// unrotated element a thread.
+// of 16); otherwise single elements, one pair or one unrotated element a
+// thread.
 template <typename T, bool INTER, bool VEC>
 __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(RotaryArgs a) {
   extern __shared__ float2 cs[];   // (cos, sin) of the token's rot / 2 pairs

@@ -5,7 +5,8 @@ query rows (the tokens behind a shared prefix, or one request's tokens) into
 row tiles, and the keys they see into ranges, so that the units spread over
 the GPU whatever the mix of lengths; and it lists for every (token, head)
 which partial rows to join.  ``csrc/kernels/cache_ops.h`` describes the
-records; everything the kernels index with is checked here.
+records; everything the kernels index with is checked here.  The constants up
+to ``NO_LIMIT`` are the kernels' (``PLAN_CONSTANTS`` of the extension).
 """
 from typing import Dict, List, NamedTuple, Sequence, Tuple
 
@@ -16,9 +17,9 @@ ROW_UNIT_ROWS = 16
 STAGE_KEYS = 32          # keys per stage of the row kernel
 TILE_UNIT_ROWS = 128
 TILE_KEYS = 128          # keys per block of the tile kernel
-TILE_MIN_ROWS = 17       # fewest query rows (tokens x group heads) the tile kernel takes
 CHUNK_KEYS = 512         # keys per block that adds up weights
-NO_LIMIT = 1 << 30
+NO_LIMIT = 1 << 30       # limit of keys that every query sees
+TILE_MIN_ROWS = 17       # fewest query rows (tokens x group heads) the tile kernel takes
 ROW_SLOTS = 6            # warps of the row kernel an SM takes at once
 ROW_MIN_STAGES = 2       # shortest range of a row unit, in stages
 ROW_START = 1            # what starting and ending a unit takes, in stages
