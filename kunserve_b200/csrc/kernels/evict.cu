@@ -244,19 +244,14 @@ __global__ void __launch_bounds__(NT) select_kernel(EvictSelect a, int ctas, int
   if (ctas > 1) cluster_sync();   // no CTA leaves while another reads its shared memory
 }
 
-template <int NT, int BITS>
+constexpr int kMostSmem = 200 * 1024;
+template <int NT, int BITS, bool CACHED>
 void launch_select(const EvictSelect& a, int ctas, int slice, cudaStream_t s) {
   constexpr int kHist = (31 + BITS) / BITS * (1 << BITS) * 4;
-  constexpr int kMost = 200 * 1024;
-  const unsigned grid = (unsigned)a.n_reqs * a.g.kvh * ctas;
-  const bool cached = kHist + slice * 4 <= kMost;
-  if (cached) {
-    const int smem = kHist + slice * 4;
-    ensure_smem_attr(reinterpret_cast<const void*>(select_kernel<NT, BITS, true>), kMost);
-    launch_kc(select_kernel<NT, BITS, true>, dim3(grid), dim3(NT), smem, s, ctas, a, ctas, slice);
-  } else {
-    launch_kc(select_kernel<NT, BITS, false>, dim3(grid), dim3(NT), kHist, s, ctas, a, ctas, slice);
-  }
+  const int smem = kHist + (CACHED ? slice * 4 : 0);
+  if (CACHED) ensure_smem_attr(reinterpret_cast<const void*>(select_kernel<NT, BITS, CACHED>), kMostSmem);
+  launch_kc(select_kernel<NT, BITS, CACHED>, dim3((unsigned)a.n_reqs * a.g.kvh * ctas), dim3(NT), smem, s, ctas, a,
+            ctas, slice);
 }
 
 // A warp moves kMoves tokens of a row: K and V as 16-byte vectors, weights and
@@ -344,9 +339,11 @@ void evict_select(const EvictSelect& a, cudaStream_t s) {
   while (ctas < evict::kMostCtas && rows * ctas * 2 <= 8 * 148 && a.most_tokens > 2048 * ctas) ctas *= 2;
   const int slice = ((a.most_tokens + ctas - 1) / ctas + 31) / 32 * 32;
   if (slice <= 4096)
-    evict::launch_select<256, 8>(a, ctas, slice, s);
+    evict::launch_select<256, 8, true>(a, ctas, slice, s);
+  else if (slice <= (evict::kMostSmem - 8 * 1024) / 4)   // beside four histograms of 512 bins
+    evict::launch_select<512, 9, true>(a, ctas, slice, s);
   else
-    evict::launch_select<512, 9>(a, ctas, slice, s);
+    evict::launch_select<512, 9, false>(a, ctas, slice, s);
 }
 
 void cache_compact(const CacheCompact& a, cudaStream_t s) {
