@@ -181,7 +181,9 @@ def page_array(pages: Sequence[int], pages_total: int) -> np.ndarray:
 
 def check_distinct(pages: np.ndarray) -> None:
     """Every page of the plan's lists is listed once."""
-    ids, times = np.unique(pages, return_counts=True)
-    if ids.size < pages.size:
-        raise ValueError(f"page {int(ids[times.argmax()])} is listed {int(times.max())} times; slots that gain "
-                         "weight and move must belong to one request")
+    seen = np.zeros(int(pages.max()) + 1 if pages.size else 0, dtype=bool)
+    seen[pages] = True
+    if np.count_nonzero(seen) < pages.size:
+        times = np.bincount(pages)
+        raise ValueError(f"page {int(times.argmax())} is listed {int(times.max())} times; slots that gain weight and "
+                         "move must belong to one request")
