@@ -198,20 +198,19 @@ struct RotaryTable {
     KUS_CHECK(r > 0 && r <= hd_ && r <= 4096, "rotary_dim ", r, " of head_dim ", hd_);
     rot = (int)r;
   }
-  // The frequencies outlive the work queued on the current stream.
-  void use() const {
-    const auto st = at::cuda::getCurrentCUDAStream(steps.get_device());
+  // The frequencies outlive the work queued on `st`.
+  void use(const c10::cuda::CUDAStream& st) const {
     if (st != made_on) steps.record_stream(st);
   }
 };
 
 RotaryArgs rotary_args(const RotaryTable* table, const torch::Tensor& x, const torch::Tensor& positions,
-                       const torch::Tensor& out, bool inverse) {
+                       const torch::Tensor& out, bool inverse, const c10::cuda::CUDAStream& st) {
   KUS_CHECK(table && table->steps.device() == x.device(), "the rotary frequencies must be on ", x.device());
   const int64_t hd = x.size(2);
   KUS_CHECK(hd == table->hd, "head_dim ", hd, ", the rotary frequencies have ", (int64_t)table->hd);
   check_index(positions, x.size(0), x, "positions");
-  table->use();
+  table->use(st);
   KUS_CHECK(x.size(0) < (1LL << 31) && x.size(1) * hd < (1 << 23), "too many tokens or heads");
   RotaryArgs a{};
   a.x = x.data_ptr();
@@ -232,15 +231,22 @@ RotaryArgs rotary_args(const RotaryTable* table, const torch::Tensor& x, const t
   return a;
 }
 
-torch::Tensor rotary_apply_op(const torch::Tensor& x, const torch::Tensor& positions, const RotaryTable* table,
-                              const c10::optional<torch::Tensor>& out, bool inverse) {
+// None: a gradient is asked for, the caller goes through autograd.
+c10::optional<torch::Tensor> rotary_apply_op(const torch::Tensor& x, const torch::Tensor& positions,
+                                             const RotaryTable* table, const c10::optional<torch::Tensor>& out,
+                                             bool inverse) {
   KUS_CHECK(x.is_cuda() && x.dim() == 3, "x must be a CUDA tensor [T, heads, head_dim]");
+  if ((x.requires_grad() || (out.has_value() && out->requires_grad())) && at::GradMode::is_enabled()) {
+    TORCH_CHECK_VALUE(!out.has_value(), "results written to out= carry no gradient, but an argument requires one");
+    return c10::nullopt;
+  }
   const int type = elem_type(x, "x");
   c10::cuda::CUDAGuard guard(x.device());
   check_heads(x, x.size(0), x.size(1), x.size(2), x, "x");
   torch::Tensor o = out.has_value() ? *out : empty(x.sizes(), x.scalar_type(), x.device());
   check_heads(o, x.size(0), x.size(1), x.size(2), x, "out");
-  rotary(rotary_args(table, x, positions, o, inverse), type, at::cuda::getCurrentCUDAStream());
+  const auto st = at::cuda::getCurrentCUDAStream();
+  rotary(rotary_args(table, x, positions, o, inverse, st), type, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return o;
 }
@@ -257,7 +263,8 @@ void rotary_append_op(const torch::Tensor& qkv, const torch::Tensor& positions, 
   check_heads(qkv, T, nq + 2 * g.kvh, g.hd, kv.pool, "qkv");
   // without `out` the queries turn in place: they lie first in qkv
   if (out.has_value()) check_heads(*out, T, nq, g.hd, kv.pool, "out");
-  RotaryArgs a = rotary_args(table, qkv, positions, out.has_value() ? *out : qkv, false);
+  const auto st = at::cuda::getCurrentCUDAStream();
+  RotaryArgs a = rotary_args(table, qkv, positions, out.has_value() ? *out : qkv, false, st);
   check_index(pages, T, qkv, "pages");
   check_index(slots, T, qkv, "slots");
   KUS_CHECK(weights.has_value() == slot_positions.has_value(), "weights and slot_positions come together");
@@ -273,7 +280,7 @@ void rotary_append_op(const torch::Tensor& qkv, const torch::Tensor& positions, 
     a.weights = weights->data_ptr<float>();
     a.slot_positions = slot_positions->data_ptr<int>();
   }
-  rotary(a, kv.type, at::cuda::getCurrentCUDAStream());
+  rotary(a, kv.type, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 

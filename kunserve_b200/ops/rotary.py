@@ -132,11 +132,8 @@ def rotary_apply(x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, out: 
     sin kept, that is the gradient: if y = rotary_apply(x), the gradient of x
     is rotary_apply(gradient of y, inverse=True).  Autograd does so where ``x``
     requires a gradient; ``out`` is refused there."""
-    if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
-        if out is not None:
-            raise ValueError("rotary_apply: results written to out= carry no gradient, but an argument requires one")
-        return _Turn.apply(x, positions, rotary, inverse)
-    return native().rotary_apply(x, positions, rotary._native, out, inverse)
+    y = native().rotary_apply(x, positions, rotary._native, out, inverse)
+    return y if y is not None else _Turn.apply(x, positions, rotary, inverse)
 
 
 def rotary_append(qkv: torch.Tensor, positions: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor,
