@@ -25,8 +25,14 @@
 //
 // A block of 128 rows and keys takes about 1950 clk: 1024 of exponentials (16
 // a clk), the rest waits around them; the products take 1400 beside that.
-// 128 requests, 8 rows each per KV head, behind four prefixes of 16384: 73 us
-// for 70 GFLOP and 268 MB.
+// 128 requests, 8 rows each per KV head, behind four prefixes of 16384: 73-85
+// us for 70 GFLOP and 268 MB.
+//
+// P is rounded once to the element type on its way to O += P V; sums, maxima
+// and O are fp32.  Its remainder would take a second product with V: some 2100
+// clk of products a block, above what bounds it now.  Outputs are so off by 0.0023 (bf16) and 0.00029 (fp16) of
+// their norm against 64 bits, where their own rounding makes 0.0017 and
+// 0.00021, which is all that the row kernel is off by.
 //
 // The keys a unit covers end inside a page or a block: boxes past the end
 // are not loaded, the tail rows of V are zeroed (a stale NaN times a zero

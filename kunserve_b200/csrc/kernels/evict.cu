@@ -257,7 +257,7 @@ void launch_select(const EvictSelect& a, int ctas, int slice, cudaStream_t s) {
 // A warp moves kMoves tokens of a row: K and V as 16-byte vectors, weights and
 // positions, all loads in flight before the first store.  Bound by the latency
 // of index, page and row loads in turn, so by the warps an SM holds: all
-// 64, at 32 registers a thread: 166,000 moves of 1 KB read and written in 36 us.
+// 64, at 32 registers a thread: 166,000 moves of 1 KB read and written in 33-36 us.
 constexpr int kMoves = 4;
 constexpr int kCompactWarps = 8;
 

@@ -14,7 +14,8 @@
 // heads, while the first items' loads are under way); a thread turns 16
 // elements of a head as two 16-byte vectors.  Full SMs (32 registers a thread)
 // move more than several items in flight a thread: 16384 tokens of 64 + 8
-// heads of 128, 672 MB, take 102 us, with three items at 62 registers 117.
+// heads of 128, 672 MB, take 104-111 us in a steady run (102 in the first
+// 100 ms); with three items at 62 registers 117 where these took 102.
 #include "../common.cuh"
 #include "cache_elem.cuh"
 #include "cache_ops.h"

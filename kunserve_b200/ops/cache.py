@@ -3,7 +3,10 @@ share prefixes, single-token attention that accumulates each key's weight,
 and eviction by those weights.
 
 A step makes one plan from the lengths and page lists the scheduler holds, and
-calls the operators with it for every layer.  All of them run on the current
+calls the operators with it for every layer.  (Making one takes 0.2 ms for one
+or two requests, 0.4 to 0.8 ms for 30 to 130, on the host; its copy to the
+device waits for what is queued on the current stream.  A captured graph holds
+for the lengths of its plan alone, and needs it alive.)  All of them run on the current
 CUDA stream of the cache's device and allocate their scratch from it.  They
 serve: their results carry no gradient.
 """
@@ -79,7 +82,17 @@ def shared_prefix_attention(q: torch.Tensor, kv, layer: int, plan: SharedPrefixP
 
     Cache slots past a request's tokens may hold anything; the values of a
     request's asked tokens must be finite, since queries of one call that come
-    before a token meet its values with weight zero."""
+    before a token meet its values with weight zero.  Rows with a NaN score or
+    one of +inf give NaN; keys of score -inf count for nothing, and rows of no
+    other keys give zeros.
+
+    Sums and statistics are fp32.  Keys that 17 or more query rows (queries
+    times heads of a KV head's group) see together, as the requests behind one
+    prefix do, meet their values with probabilities rounded to the cache's type:
+    outputs are then off by 0.0023 (bf16) or 0.0003 (fp16) of their norm, of
+    which 0.0017 and 0.0002 are their own rounding; with fewer rows the rounding
+    of the output is all.  In fp16 a weight below 2^-36 of its row's largest may
+    count as zero."""
     return native().cached_attention(q, kv, layer, plan._native, scale, out, None)
 
 

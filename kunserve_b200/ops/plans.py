@@ -19,7 +19,13 @@ TILE_UNIT_ROWS = 128
 TILE_KEYS = 128          # keys per block of the tile kernel
 CHUNK_KEYS = 512         # keys per block that adds up weights
 NO_LIMIT = 1 << 30       # limit of keys that every query sees
-TILE_MIN_ROWS = 17       # fewest query rows (tokens x group heads) the tile kernel takes
+# Fewest query rows (tokens x group heads) of a span that the tile kernel takes.
+# Prefixes: at 16 rows both take the same (40 heads, 2048 keys: 20.7 us), at 24
+# the tile kernel 53 us, row tiles 90 (8 heads, four prefixes of 16384).  Own
+# spans of 96 rows (24 requests, 8 heads, us, tile / row kernel): 2048 keys 63 /
+# 165, 512 keys 31 / 54, 128 keys 25 / 25, 40 keys 25 / 19; of 20 to 24 rows the
+# two meet at 512 keys and the row kernel takes half as long at 40.
+TILE_MIN_ROWS = 17
 ROW_SLOTS = 6            # warps of the row kernel an SM takes at once
 ROW_MIN_STAGES = 2       # shortest range of a row unit, in stages
 ROW_START = 1            # what starting and ending a unit takes, in stages

@@ -31,7 +31,11 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
     ``linear`` (positions divided by the factor), ``dynamic`` (a larger base
     once ``max_position`` exceeds the original context), ``llama3`` (low
     frequencies divided, high ones kept, a linear mix between) or ``yarn``
-    (the same by rotation counts, and a factor on cos and sin)."""
+    (the same by rotation counts, and a factor on cos and sin).  Other kinds and
+    keys (``longrope``, yarn's ``mscale`` and ``truncate``, a ``rope_theta``
+    among them) are refused, and so is an original context left to the model's
+    other settings: ``original_max_position_embeddings`` must be given where the
+    kind needs it."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be a positive even number, got {rotary_dim}")
     if not theta > 0:
