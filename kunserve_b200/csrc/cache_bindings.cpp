@@ -9,31 +9,12 @@
 #include <cmath>
 
 #include "kernels/cache_ops.h"
+#include "messages.h"
 
 namespace py = pybind11;
 using namespace kus;
 
 namespace {
-
-// Text of an error message's parts.  Numbers are formatted with to_string:
-// streaming them needs the locale tables of one C++ runtime, and the
-// extension may be linked with another than the libraries it is loaded into.
-std::string text(const char* s) { return s; }
-std::string text(int64_t v) { return std::to_string(v); }
-std::string text(torch::ScalarType t) { return c10::toString(t); }
-std::string text(const torch::Device& d) { return d.str(); }
-std::string text(at::IntArrayRef v) {
-  std::string s = "[";
-  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
-  return s + "]";
-}
-template <typename... A>
-std::string say(const A&... a) {
-  std::string s;
-  ((s += text(a)), ...);
-  return s;
-}
-#define KUS_CHECK(cond, ...) TORCH_CHECK(cond, say(__VA_ARGS__))
 
 int elem_type(const torch::Tensor& t, const char* what) {
   KUS_CHECK(t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat16, what,

@@ -13,6 +13,8 @@
 #include "attention_prefix.cu"
 #include "attention_cached.cu"
 #include "evict.cu"
+#include "int8_rows.cu"
+#include "int8_gemm.cu"
 
 namespace kus {
 void set_pdl(bool on) { pdl_flag() = on; }
