@@ -88,9 +88,23 @@ torch::Tensor empty_rows8(int64_t rows, int64_t columns, const torch::Device& de
   return wide == columns ? t : t.narrow(1, 0, columns);
 }
 
+// Such rows and their scales, behind them in one block of memory: a second
+// allocation takes as long as a small call has.
+std::tuple<torch::Tensor, torch::Tensor> empty_quantized(int64_t rows, int64_t columns, const torch::Device& device) {
+  const int64_t wide = (columns + 15) / 16 * 16;
+  const torch::Tensor block = empty({rows * wide + 4 * rows}, torch::kInt8, device);
+  auto view = [&](torch::ScalarType type, at::IntArrayRef sizes, at::IntArrayRef strides, int64_t offset) {
+    torch::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(block.storage()),
+                                                               c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                               c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides, offset);
+    return t;
+  };
+  return {view(torch::kInt8, {rows, columns}, {wide, 1}, 0), view(torch::kFloat32, {rows}, {1}, rows * wide / 4)};
+}
+
 std::tuple<torch::Tensor, torch::Tensor> run_rows(Int8Rows a, const torch::Tensor& x) {
-  torch::Tensor q = empty_rows8(x.size(0), x.size(1), x.device());
-  torch::Tensor scales = empty({x.size(0)}, torch::kFloat32, x.device());
+  auto [q, scales] = empty_quantized(x.size(0), x.size(1), x.device());
   a.x = x.data_ptr();
   a.xs = x.stride(0);
   a.q = q.data_ptr<int8_t>();

@@ -24,6 +24,13 @@ KUS_DEVICE float max_nan(float a, float b) {
   return r;
 }
 
+// 1 / x to one step
+KUS_DEVICE float rcp(float x) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // 8 elements from 16-byte vectors
 template <typename T>
 KUS_DEVICE void load8(const T* p, float (&f)[8]) {
@@ -116,38 +123,58 @@ struct Row {
     }
     if (OP == kRowsSilu) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = y[e] / (1.f + expf(-y[e])) * o[e];
+      for (int e = 0; e < 8; ++e) y[e] = y[e] * rcp(1.f + expf(-y[e])) * o[e];
     }
   }
 };
 
-// One row a group of LANES threads.  HELD: vectors of 8 a thread keeps
-// between the two passes over its row; 0: the row is read again.
-template <typename T, int OP, int LANES, int HELD, bool VEC>
-__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) rows_kernel(Int8Rows a) {
-  constexpr int kThreads = LANES < 256 ? 256 : LANES;
-  constexpr int kRows = kThreads / LANES, kWarps = LANES / 32;
-  __shared__ float2 part[kThreads / 32];
+// The integers nearest to 127 v / top, two's complement, in the low bytes.
+// The quotient is that of a product with 1 / top, put right by its remainder
+// once (Markstein 1990): where 127 v / top is a float, a half say, the result
+// is that float, and halves go to even.  Adding 1.5 * 2^23 rounds to a whole
+// number and leaves it in the low bits; a conversion runs at a quarter of the
+// rate.
+struct Quotient {
+  float times, over, inverse;
+  KUS_DEVICE Quotient(float top, bool sound) {
+    const float small = top > 1e36f ? 0x1p-10f : top < 1e-30f ? 0x1p60f : 1.f;   // 127 v and 1 / top stay in range
+    over = sound && top > 0.f ? top * small : 1.f;
+    times = sound ? 127.f * small : 0.f;
+    inverse = 1.f / over;
+  }
+  KUS_DEVICE uint32_t operator()(float v) const {
+    const float t = v * times, r = t * inverse;
+    return __float_as_uint(fmaf(fmaf(-r, over, t), inverse, r) + 12582912.f);
+  }
+};
+
+// One row a warp (WARPS == 1; eight warps a block) or a block.  HELD: vectors
+// of 8 a thread keeps between the two passes over its row; 0: the row is read
+// again.
+template <typename T, int OP, bool ONE_WARP, int HELD, bool VEC>
+__global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_kernel(Int8Rows a) {
+  __shared__ float2 part[32];
   pdl_wait();
   pdl_trigger();
-  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
-  const long long t = (long long)blockIdx.x * kRows + group;
-  if (kRows > 1 && t >= a.T) return;      // whole groups leave; those of several warps are their block's only one
+  const int lanes = ONE_WARP ? 32 : blockDim.x;
+  const int lane = ONE_WARP ? threadIdx.x % 32 : threadIdx.x;
+  const long long t = ONE_WARP ? (long long)blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x;
+  if (ONE_WARP && t >= a.T) return;
   const Row<T, OP> row(a, t);
-  const int vectors = (a.K + 8 * LANES - 1) / (8 * LANES);
+  const int vectors = HELD > 0 ? HELD : (a.K + 8 * lanes - 1) / (8 * lanes);
 
   float y[HELD > 0 ? HELD : 1][8];
   float sum = 0.f, top = 0.f;
   if (HELD > 0) {
 #pragma unroll
-    for (int j = 0; j < HELD; ++j) row.template values<VEC>(j, lane, LANES, true, y[j], sum);
+    for (int j = 0; j < HELD; ++j) row.template values<VEC>(j, lane, lanes, true, y[j], sum);
 #pragma unroll
     for (int j = 0; j < HELD; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(y[j][e]));
   } else {
     for (int j = 0; j < vectors; ++j) {
-      row.template values<VEC>(j, lane, LANES, false, y[0], sum);
+      row.template values<VEC>(j, lane, lanes, false, y[0], sum);
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(y[0][e]));
     }
@@ -157,20 +184,17 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) rows_kernel(Int8Row
     if (OP == kRowsNorm) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   }
-  if (kWarps > 1) {
-    const int w0 = group * kWarps;
-    if (lane % 32 == 0) part[threadIdx.x / 32] = make_float2(sum, top);
-    if (kRows > 1)
-      named_barrier(1 + group, LANES);
-    else
-      __syncthreads();
-    sum = 0.f;
-    top = 0.f;
+  if (!ONE_WARP) {
+    const int warps = blockDim.x / 32, l = threadIdx.x % 32;
+    if (l == 0) part[threadIdx.x / 32] = make_float2(sum, top);
+    __syncthreads();
+    const float2 p = l < warps ? part[l] : make_float2(0.f, 0.f);
+    sum = p.x;
+    top = p.y;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float2 p = part[w0 + w];
-      if (OP == kRowsNorm) sum += p.x;
-      top = max_nan(top, p.y);
+    for (int o = 16; o > 0; o >>= 1) {
+      if (OP == kRowsNorm) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
   }
 
@@ -182,25 +206,22 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) rows_kernel(Int8Row
     sound = sound && sum < INFINITY;
   }
   if (lane == 0) a.scales[t] = sound ? top / 127.f * factor : NAN;
-  const float small = top > 1e36f ? 0x1p-10f : 1.f;     // keeps 127 y in range
-  const float times = sound ? 127.f * small : 0.f, over = sound && top > 0.f ? top * small : 1.f;
+  const Quotient quotient(top, sound);
   int8_t* q = a.q + t * a.qs;
   auto write = [&](int j, const float (&v)[8]) {
-    int r[8];
+    uint32_t r[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = sound ? __float2int_rn(v[e] * times / over) : 0;
+    for (int e = 0; e < 8; ++e) r[e] = sound ? quotient(v[e]) : 0;
+    const int c = column(j, lane, lanes);
     if (VEC) {
-      const int c = column(j, lane, LANES);
       uint2 u;
       u.x = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
       u.y = __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410);
       if (c < a.K) *reinterpret_cast<uint2*>(q + c) = u;
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = column(j, lane, LANES) + e;
-        if (c < a.K) q[c] = (int8_t)r[e];
-      }
+      for (int e = 0; e < 8; ++e)
+        if (c + e < a.K) q[c + e] = (int8_t)r[e];
     }
   };
   if (HELD > 0) {
@@ -210,20 +231,23 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) rows_kernel(Int8Row
     // the sum x + residual is written in the second pass: it may lie over either of them
     for (int j = 0; j < vectors; ++j) {
       float unused = 0.f;
-      row.template values<VEC>(j, lane, LANES, true, y[0], unused);
+      row.template values<VEC>(j, lane, lanes, true, y[0], unused);
       write(j, y[0]);
     }
   }
 }
 
-template <typename T, int OP, int LANES, int HELD>
+template <typename T, int OP, bool ONE_WARP, int HELD>
 void launch(const Int8Rows& a, bool vec, cudaStream_t s) {
-  constexpr int kThreads = LANES < 256 ? 256 : LANES;
-  const dim3 grid((unsigned)((a.T + kThreads / LANES - 1) / (kThreads / LANES)));
+  const int vectors = (a.K + 7) / 8;
+  const int each = HELD > 0 ? HELD : 4;
+  int threads = ONE_WARP ? 256 : ((vectors + each - 1) / each + 31) / 32 * 32;
+  if (threads > 1024) threads = 1024;
+  const dim3 grid((unsigned)(ONE_WARP ? (a.T + 7) / 8 : a.T));
   if (vec)
-    launch_k(rows_kernel<T, OP, LANES, HELD, true>, grid, dim3(kThreads), 0, s, a);
+    launch_k(rows_kernel<T, OP, ONE_WARP, HELD, true>, grid, dim3(threads), 0, s, a);
   else
-    launch_k(rows_kernel<T, OP, LANES, HELD, false>, grid, dim3(kThreads), 0, s, a);
+    launch_k(rows_kernel<T, OP, ONE_WARP, HELD, false>, grid, dim3(threads), 0, s, a);
 }
 
 bool on16(const void* p, long long stride, int bytes, int rows) {
@@ -236,55 +260,61 @@ void launch_op(const Int8Rows& a, cudaStream_t s) {
   const bool vec = a.K % 8 == 0 && on16(a.x, a.xs, el, a.T) && (!a.other || on16(a.other, a.os, el, a.T)) &&
                    (!a.weight || on16(a.weight, 0, el, 1)) && (!a.total || on16(a.total, a.ts, el, a.T));
   const int n = (a.K + 7) / 8;
-  if (n <= 32) return launch<T, OP, 32, 1>(a, vec, s);
-  if (n <= 64) return launch<T, OP, 32, 2>(a, vec, s);
-  if (n <= 128) return launch<T, OP, 64, 2>(a, vec, s);
-  if (n <= 256) return launch<T, OP, 128, 2>(a, vec, s);
-  if (n <= 512) return launch<T, OP, 256, 2>(a, vec, s);
-  if (n <= 768) return launch<T, OP, 256, 3>(a, vec, s);
-  if (n <= 1024) return launch<T, OP, 512, 2>(a, vec, s);
-  if (n <= 2048) return launch<T, OP, 512, 4>(a, vec, s);
-  if (n <= 4096) return launch<T, OP, 1024, 4>(a, vec, s);
-  return launch<T, OP, 1024, 0>(a, vec, s);
+  if (n <= 32) return launch<T, OP, true, 1>(a, vec, s);
+  if (n <= 64) return launch<T, OP, true, 2>(a, vec, s);
+  if (n <= 256) return launch<T, OP, false, 1>(a, vec, s);
+  if (n <= 1024) return launch<T, OP, false, 2>(a, vec, s);
+  if (n <= 4096) return launch<T, OP, false, 4>(a, vec, s);
+  return launch<T, OP, false, 0>(a, vec, s);
 }
 
+// The float of byte i of u, whose bytes are integers with their top bit
+// turned over: 2^23 + 128 + q, less 2^23 + 128.  (A conversion runs at a
+// quarter of the rate.)
+KUS_DEVICE float value(uint32_t u, int i) { return __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + i)) - 8388736.f; }
+
+// A row a block; VEC: 16 elements a thread and step.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) values_kernel(Int8Values a) {
+__global__ void __launch_bounds__(512) values_kernel(Int8Values a) {
   pdl_wait();
   pdl_trigger();
   const long long t = blockIdx.x;
   const int8_t* q = a.q + t * a.qs;
   T* out = reinterpret_cast<T*>(a.out) + t * a.os;
   const float s = a.scales[t];
+  const int at = blockIdx.y * blockDim.x + threadIdx.x, step = gridDim.y * blockDim.x;
   if (VEC) {
-    for (int c = (blockIdx.y * 256 + threadIdx.x) * 8; c < a.K; c += gridDim.y * 256 * 8) {
-      const uint2 u = *reinterpret_cast<const uint2*>(q + c);
-      float f[8];
+    for (int c = at * 16; c < a.K; c += step * 16) {
+      const uint4 u = *reinterpret_cast<const uint4*>(q + c);
+      const uint32_t w[4] = {u.x ^ 0x80808080u, u.y ^ 0x80808080u, u.z ^ 0x80808080u, u.w ^ 0x80808080u};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)((e < 4 ? u.x : u.y) >> (8 * (e % 4))) * s;
-      if constexpr (std::is_same<T, float>::value) {
-        reinterpret_cast<float4*>(out + c)[0] = make_float4(f[0], f[1], f[2], f[3]);
-        reinterpret_cast<float4*>(out + c)[1] = make_float4(f[4], f[5], f[6], f[7]);
-      } else {
-        *reinterpret_cast<uint4*>(out + c) = pack8<T>(f);
+      for (int h = 0; h < 2; ++h) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = value(w[2 * h + e / 4], e % 4) * s;
+        if constexpr (std::is_same<T, float>::value) {
+          reinterpret_cast<float4*>(out + c + 8 * h)[0] = make_float4(f[0], f[1], f[2], f[3]);
+          reinterpret_cast<float4*>(out + c + 8 * h)[1] = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+          *reinterpret_cast<uint4*>(out + c + 8 * h) = pack8<T>(f);
+        }
       }
     }
   } else {
-    for (int c = blockIdx.y * 256 + threadIdx.x; c < a.K; c += gridDim.y * 256) out[c] = from_float<T>((float)q[c] * s);
+    for (int c = at; c < a.K; c += step) out[c] = from_float<T>((float)q[c] * s);
   }
 }
 
 template <typename T>
 void launch_values(const Int8Values& a, cudaStream_t s) {
-  const bool vec = a.K % 8 == 0 && on16(a.out, a.os, sizeof(T), a.T) &&
-                   reinterpret_cast<uintptr_t>(a.q) % 8 == 0 && (a.T <= 1 || a.qs % 8 == 0);
-  const int per = vec ? 8 * 256 : 256;
-  const int y = (a.K + per - 1) / per;
+  const bool vec = a.K % 16 == 0 && on16(a.out, a.os, sizeof(T), a.T) && on16(a.q, a.qs, 1, a.T);
+  const int items = vec ? a.K / 16 : a.K;
+  const int y = (items + 511) / 512, threads = ((items + y - 1) / y + 31) / 32 * 32;
   const dim3 grid((unsigned)a.T, (unsigned)(y < 64 ? y : 64));
   if (vec)
-    launch_k(values_kernel<T, true>, grid, dim3(256), 0, s, a);
+    launch_k(values_kernel<T, true>, grid, dim3(threads), 0, s, a);
   else
-    launch_k(values_kernel<T, false>, grid, dim3(256), 0, s, a);
+    launch_k(values_kernel<T, false>, grid, dim3(threads), 0, s, a);
 }
 
 }  // namespace i8rows

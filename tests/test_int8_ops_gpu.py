@@ -130,8 +130,9 @@ def test_silu(k, dtype):
     gate, up = wide[:, :k], wide[:, k:]
     q, s = silu_mul_int8(gate, up)
     g = gate.double()
-    # y: e^-g one step (two U), the sum, the quotient and the product: 5 U, of element and maximum
-    check_rows(q, s, g / (1 + torch.exp(-g)) * up.double(), 12, 8)
+    # y: e^-g one step (two U), the sum one U, its reciprocal a step, two products: 7 U, of element and maximum;
+    # the product with 127 and the quotient two more
+    check_rows(q, s, g / (1 + torch.exp(-g)) * up.double(), 16, 8)
 
 
 def test_silu_large_gates():
