@@ -6,7 +6,6 @@
 #include <torch/extension.h>
 #include <cmath>
 
-#include "kernels/gemm.h"
 #include "kernels/int8_ops.h"
 #include "messages.h"
 
@@ -216,6 +215,22 @@ struct Int8Weight {
   c10::cuda::CUDAStream made_on;
   CUtensorMap map;
   int N, K;
+  // plans of the numbers of tokens met last (choosing one takes 1 to 3 us)
+  struct Recent {
+    int M = -1, element = 0;
+    Int8Plan plan;
+  };
+  mutable Recent recent[32];
+
+  const Int8Plan& plan_of(int M, int element) const {
+    Recent& r = recent[M % 32];
+    if (r.M != M || r.element != element) {
+      r.plan = int8_plan(M, N, K, element, int8_slots());
+      r.M = M;
+      r.element = element;
+    }
+    return r.plan;
+  }
 
   static c10::cuda::CUDAStream stream_of(const torch::Tensor& q, const torch::Tensor& s) {
     check_quantized(q, s);
@@ -285,9 +300,9 @@ torch::Tensor int8_linear_op(const torch::Tensor& q, const torch::Tensor& scales
   a.out = o.data_ptr();
   a.ldc = o.stride(0);
   KUS_CHECK(int8_blocks(M) * int8_blocks(N) < (1LL << 28), "the product is too large for one launch");
-  const Int8Plan plan = int8_plan(a.M, a.N, a.K, num_sms());
+  const Int8Plan& plan = weight->plan_of(a.M, (int)o.element_size());
   CUtensorMap tokens;
-  KUS_CHECK(int8_token_map(&tokens, x.data_ptr<int8_t>(), stride, a.M, a.K, plan.width), "q cannot be mapped");
+  KUS_CHECK(int8_token_map(&tokens, x.data_ptr<int8_t>(), stride, a.M, a.K, plan), "q cannot be mapped");
   int8_gemm(a, plan, weight->map, tokens, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return o;
@@ -307,15 +322,17 @@ void bind_int8_ops(py::module& m) {
   m.def("silu_mul_int8", &silu_mul_int8_op);
   m.def("dequantize_int8", &dequantize_int8_op);
   m.def("int8_linear", &int8_linear_op);
-  m.def("int8_plan", [](int M, int N, int K, int sms) {
-    const Int8Plan p = int8_plan(M, N, K, sms);
-    py::dict d;
-    d["width"] = p.width;
-    d["token_tiles"] = p.token_tiles;
-    d["channel_tiles"] = p.channel_tiles;
-    d["splits"] = p.splits;
-    d["group"] = p.group;
-    d["grid"] = p.grid;
-    return d;
+  m.def("int8_slots", [] {
+    const Int8Slots s = int8_slots();
+    return std::vector<int>(s.clusters, s.clusters + 9);
+  });
+  m.def("int8_plan", [](int M, int N, int K, int element, const std::vector<int>& slots) {
+    Int8Slots s{};
+    for (int c = 0; c < 9; ++c) s.clusters[c] = slots.at(c);
+    const Int8Plan p = int8_plan(M, N, K, element, s);
+    return std::map<std::string, int>{{"pair", p.pair},     {"width", p.width}, {"token_tiles", p.token_tiles},
+                                      {"channel_tiles", p.channel_tiles},       {"splits", p.splits}, {"alone", p.alone},
+                                      {"group", p.group},   {"grid", p.grid},   {"stages", p.stages},
+                                      {"tmem_columns", p.tmem_columns}};
   });
 }

@@ -6,6 +6,10 @@
 // of tokens, the tokens its N side (a tile of 16 to 256): a decode step pads
 // its few tokens to 16 and no further.  A k-block is 128 bytes of K, 32 a
 // product.
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+
 #include "../common.cuh"
 #include "cache_elem.cuh"
 #include "int8_ops.h"
@@ -13,29 +17,58 @@
 namespace kus {
 namespace i8gemm {
 
-constexpr int kThreads = 192;          // producer, issuer, four epilogue warps
+constexpr int kThreads = 320;          // producer, issuer, two groups of four epilogue warps
 constexpr int kBK = kInt8Block;        // bytes of K per stage
 constexpr int kWBytes = kInt8Block * kBK;
 
-// CAP: most tokens of a tile.  64: two CTAs an SM.
-template <int CAP>
-struct Cfg {
-  static constexpr int kXBytes = CAP * kBK;
-  static constexpr int kStageBytes = kWBytes + kXBytes;
-  static constexpr int kStages = 4;
-  static constexpr int kTmemCols = 2 * CAP;             // two accumulators
-  static constexpr int kScaleBytes = 2 * CAP * 4;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kScaleBytes + 1024 + 256;
-  static constexpr int kPerSm = CAP <= 64 ? 2 : 1;
-};
+constexpr int kMostStages = 8;
+constexpr int kBarriers = 2 * kMostStages + 5;
+// Shared memory of a CTA: alone on its SM, or one of two.
+constexpr int kSmemAlone = 232448, kSmemHalf = 115712;
 
-// D(tmem, s32) (+)= A(smem, s8) * B(smem, s8)^T
+// Results go through shared memory, so that whole lines are written: each
+// group of epilogue warps has two buffers of 16 tokens x 128 channels, the
+// tokens 272 bytes apart in 16 bits (stmatrix writes eight of them at once).
+constexpr int kChunk = 16;
+KUS_HOST_DEVICE constexpr int token_bytes(int element) { return kInt8Block * element + (element == 2 ? 16 : 0); }
+KUS_HOST_DEVICE constexpr int out_bytes(int element) { return 4 * kChunk * token_bytes(element); }
+
+KUS_HOST_DEVICE int x_rows(const Int8Plan& p) { return p.pair ? p.width / 2 : p.width; }   // tokens a CTA loads
+KUS_HOST_DEVICE int stage_bytes(const Int8Plan& p) { return kWBytes + x_rows(p) * kBK; }
+int smem_bytes(const Int8Plan& p, int element) {
+  return p.stages * stage_bytes(p) + out_bytes(element) + 2 * p.width * 4 + kBarriers * 8 + 16 + 1024;
+}
+
+// D(tmem, s32) (+)= A(smem, s8) * B(smem, s8)^T; of a pair: A rows 128 and
+// up and the second half of B's rows are the other CTA's (umma_f16_pair).
+template <bool PAIR>
 KUS_DEVICE void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
+  if (PAIR)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrive on `bar` (PAIR: of both CTAs of the pair whose even rank is `lead`)
+// once the products issued so far have ended.
+template <bool PAIR>
+KUS_DEVICE void commit(uint64_t* bar, uint32_t lead) {
+  if (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)(3u << lead))
+        : "memory");
+  else
+    umma_commit(bar);
 }
 
 // Instruction descriptor: kind::i8, A and B signed and K-major, D s32, M x N.
@@ -74,6 +107,90 @@ KUS_DEVICE float float_of(O x) { return Elem<O>::to_f(x); }
 template <>
 KUS_DEVICE float float_of<float>(float x) { return x; }
 
+// 16 lanes (channels) x 16 columns (tokens) of TMEM as the fragments of two
+// 16 x 8 products: v[4 g + 2 s + i] is lane t / 4 + 8 s, column 8 g + 2 (t % 4) + i.
+KUS_DEVICE void tmem_ld_frag(uint32_t taddr, int (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
+}
+KUS_DEVICE void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Four 8 x 8 matrices of 16 bits, each written with its columns as rows of 16
+// bytes; lane 8 i + j gives the address of row j of matrix i.
+KUS_DEVICE void stmatrix4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
+}
+
+// Results of 16 tokens x the warp's 32 channels, from TMEM to a buffer of
+// tokens x 128 channels.
+template <typename O>
+KUS_DEVICE void stage_chunk(uint32_t taddr, const float* xs, const float (&ws)[4], const float (&b)[4], uint8_t* to,
+                            int quarter, int lane) {
+  if constexpr (sizeof(O) == 2) {
+    int v[2][8];
+    tmem_ld_frag(taddr, v[0]);
+    tmem_ld_frag(taddr + (16u << 16), v[1]);
+    float2 x[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) x[g] = *reinterpret_cast<const float2*>(xs + 8 * g + 2 * (lane % 4));
+    tmem_ld_wait();
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {      // channels 8 i .. of the warp's 32
+        const int* w = &v[i / 2][4 * g + 2 * (i % 2)];
+        m[i] = pack2<O>(fmaf((float)w[0] * x[g].x, ws[i], b[i]), fmaf((float)w[1] * x[g].y, ws[i], b[i]));
+      }
+      const int token = 8 * g + lane % 8, channel = quarter * 32 + lane / 8 * 8;
+      stmatrix4_trans(smem_u32(to + token * token_bytes(2) + channel * 2), m[0], m[1], m[2], m[3]);
+    }
+  } else {
+    int v[16];
+    tmem_ld16(taddr, v);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      reinterpret_cast<float*>(to + i * token_bytes(4))[quarter * 32 + lane] = fmaf((float)v[i] * xs[i], ws[0], b[0]);
+  }
+}
+
+// Where results go.
+template <typename O>
+struct Results {
+  O* out;
+  long long ldc;
+  int N;
+  bool aligned;      // whole vectors of 16 bytes
+
+  KUS_DEVICE explicit Results(const Int8Gemm& a)
+      : out(reinterpret_cast<O*>(a.out)),
+        ldc(a.ldc),
+        N(a.N),
+        aligned((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldc * sizeof(O))) % 16 == 0) {}
+
+  // `tokens` rows of 128 channels, `stride` bytes apart, by 128 threads.
+  KUS_DEVICE void write(const uint8_t* from, int stride, int t0, int tokens, int n0, int thread) const {
+    constexpr int kVec = 16 / sizeof(O), kPerRow = kInt8Block / kVec, kRows = 128 / kPerRow;
+    if (aligned && n0 + kInt8Block <= N) {
+      const int r = thread / kPerRow, e = thread % kPerRow * kVec;
+      O* dst = out + (t0 + r) * ldc + n0 + e;
+      from += r * stride + e * sizeof(O);
+#pragma unroll
+      for (int t = 0; t < kChunk; t += kRows) {
+        if (t + r < tokens) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(from);
+        dst += kRows * ldc;
+        from += kRows * stride;
+      }
+    } else if (n0 + thread < N) {
+      for (int t = 0; t < tokens; ++t)
+        out[(t0 + t) * ldc + n0 + thread] = reinterpret_cast<const O*>(from + t * stride)[thread];
+    }
+  }
+};
+
 // Unit u of a plan: channel tile, token tile.  Token tiles run fastest within
 // groups of `group`, so that a group's tokens stay in L2 while the weights
 // stream past them once.
@@ -90,19 +207,23 @@ KUS_DEVICE Unit unit_at(const Int8Plan& p, int u) {
   return x;
 }
 
-template <int CAP, typename O, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, Cfg<CAP>::kPerSm)
+// PAIR: clusters of pairs of CTAs; a unit is 256 channels, CTA rank r of the
+// pair stages channels 128 r.. and half of the tile's tokens, the even CTA
+// issues cta_group::2 products over both, and each CTA holds and writes its
+// own 128 channels.  SPLIT: the p.splits CTAs (pairs) of a cluster share one
+// unit's K; else each walks whole units.
+template <typename O, bool PAIR, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 2)
     gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, Int8Gemm a,
                 Int8Plan p) {
-  using C = Cfg<CAP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* smem_w = smem;
-  uint8_t* smem_x = smem + C::kStages * kWBytes;
-  float* scales = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(scales + 2 * CAP);
-  uint64_t* empty = full + C::kStages;
-  uint64_t* tfull = empty + C::kStages;
+  const int stages = p.stages, stage_size = stage_bytes(p);
+  uint8_t* staged = smem + stages * stage_size;
+  float* scales = reinterpret_cast<float*>(staged + out_bytes(sizeof(O)));
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + 2 * p.width);
+  uint64_t* empty = full + kMostStages;
+  uint64_t* tfull = empty + kMostStages;
   uint64_t* tempty = tfull + 2;
   uint64_t* drained = tempty + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
@@ -110,139 +231,192 @@ __global__ void __launch_bounds__(kThreads, Cfg<CAP>::kPerSm)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int blocks = (a.K + kBK - 1) / kBK;
   const int units = p.channel_tiles * p.token_tiles;
-  // SPLIT: a cluster per unit, CTA `rank` takes a range of its K; else each
-  // CTA walks whole units
-  const int rank = SPLIT ? (int)cluster_rank() : 0;
+  constexpr int kCtas = PAIR ? 2 : 1;                    // of a unit (of a part of its K)
+  const uint32_t rank = PAIR || SPLIT ? cluster_rank() : 0u;
+  const int half = PAIR ? (int)(rank & 1) : 0;           // which of the pair
+  const uint32_t lead = PAIR ? rank & ~1u : rank;
+  const bool leads = rank == lead;
+  const int part = SPLIT ? (int)rank / kCtas : 0;
   const int each = SPLIT ? (blocks + p.splits - 1) / p.splits : blocks;
-  const int kb0 = rank * each, kb1 = min(blocks, kb0 + each);
-  const int first = SPLIT ? (int)blockIdx.x / p.splits : (int)blockIdx.x;
-  const int step = SPLIT ? units : (int)gridDim.x;
+  const int kb0 = part * each, kb1 = min(blocks, kb0 + each);
+  const int first = (int)blockIdx.x / (SPLIT ? kCtas * p.splits : kCtas);
+  const int step = SPLIT ? units : (int)gridDim.x / kCtas;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 128);
+      mbar_init(&tempty[b], 2 * kCtas);      // each group of epilogue warps
     }
     mbar_init(drained, 1);
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(tmem_holder, C::kTmemCols);
+  if (warp == 1) PAIR ? tmem_alloc_pair(tmem_holder, p.tmem_columns) : tmem_alloc(tmem_holder, p.tmem_columns);
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();    // both CTAs' barriers are ready before the other arrives on them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
 
-  pdl_wait();
-  pdl_trigger();
+  if (warp != 0) {
+    pdl_wait();
+    pdl_trigger();
+  }
 
   if (warp == 0) {
     if (elect_one_sync()) {
       prefetch_tmap(&tmW);
       prefetch_tmap(&tmX);
-      const uint32_t bytes = kWBytes + p.width * kBK;
-      int fills = 0;
+      const uint32_t bytes = (uint32_t)stage_size * kCtas;    // both CTAs' count on the leader's barrier
+      const uint32_t lead_full = PAIR ? mapa_shared(smem_u32(full), lead) : 0u;
+      auto load_w = [&](int st, const Unit& at, int kb) {
+        uint8_t* to = smem + st * stage_size;
+        const int row = ((at.n * kCtas + half) * blocks + kb) * kInt8Block;
+        if (leads) mbar_arrive_expect_tx(&full[st], bytes);
+        if (PAIR)
+          tma_load_2d_pair(to, &tmW, lead_full + 8u * st, 0, row);
+        else
+          tma_load_2d(to, &tmW, &full[st], 0, row);
+      };
+      auto load_x = [&](int st, const Unit& at, int kb) {
+        uint8_t* to = smem + st * stage_size + kWBytes;
+        const int row = at.t * p.width + half * x_rows(p);
+        if (PAIR)
+          tma_load_2d_pair(to, &tmX, lead_full + 8u * st, kb * kBK, row);
+        else
+          tma_load_2d(to, &tmX, &full[st], kb * kBK, row);
+      };
+      // the first stages' weights are on their way while the kernel before
+      // ends: none but pack_kernel writes weights, and nothing starts before
+      // that one has ended
+      const Unit start = unit_at(p, first);
+      const int early = first < units ? min(stages, kb1 - kb0) : 0;
+      for (int j = 0; j < early; ++j) load_w(j, start, kb0 + j);
+      pdl_wait();
+      pdl_trigger();
+      for (int j = 0; j < early; ++j) load_x(j, start, kb0 + j);
+      int fills = early, st = early == stages ? 0 : early;
+      uint32_t phase = early == stages ? 1u : 0u;
       bool ok = true;
+      int kb = kb0 + early;
       for (int u = first; ok && u < units; u += step) {
         const Unit at = unit_at(p, u);
-        for (int kb = kb0; kb < kb1; ++kb, ++fills) {
-          const int st = fills % C::kStages;
-          if (!mbar_wait(&empty[st], ((fills / C::kStages) & 1) ^ 1, kErrWaitEmpty)) {
+        for (; kb < kb1; ++kb) {
+          if (!mbar_wait(&empty[st], phase ^ 1, kErrWaitEmpty)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full[st], bytes);
-          tma_load_2d(smem_w + st * kWBytes, &tmW, &full[st], 0, (at.n * blocks + kb) * kInt8Block);
-          tma_load_2d(smem_x + st * C::kXBytes, &tmX, &full[st], kb * kBK, at.t * p.width);
+          load_w(st, at, kb);
+          load_x(st, at, kb);
+          ++fills;
+          if (++st == stages) {
+            st = 0;
+            phase ^= 1;
+          }
         }
+        kb = kb0;
       }
-      // every copy has landed before the CTA ends
-      for (int f = max(0, fills - C::kStages); f < fills; ++f)
-        mbar_wait<true>(&full[f % C::kStages], (f / C::kStages) & 1, kErrWaitFull);
+      // every copy has landed before the CTA ends (a pair's, before the
+      // leader meets the other CTA at the end)
+      if (leads)
+        for (int f = max(0, fills - stages); f < fills; ++f)
+          mbar_wait<true>(&full[f % stages], (f / stages) & 1, kErrWaitFull);
     }
   } else if (warp == 1) {
-    if (elect_one_sync()) {
-      const uint32_t idesc = idesc_s8(kInt8Block, p.width);
-      int used = 0, acc = 0;
-      uint32_t acc_phase = 0;
+    if (leads && elect_one_sync()) {
+      const uint32_t idesc = idesc_s8(kInt8Block * kCtas, p.width);
+      int st = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int u = first; ok && u < units; u += step) {
-        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, kErrWaitTmemEmpty)) break;
+        const bool freed = PAIR ? mbar_wait_cluster(&tempty[acc], acc_phase ^ 1, kErrWaitTmemEmpty)
+                                : mbar_wait(&tempty[acc], acc_phase ^ 1, kErrWaitTmemEmpty);
+        if (!freed) break;
         tc_fence_after();
-        const uint32_t d = tmem_base + acc * CAP;
-        for (int kb = kb0; kb < kb1; ++kb, ++used) {
-          const int st = used % C::kStages;
-          if (!mbar_wait(&full[st], (used / C::kStages) & 1, kErrWaitFull)) {
+        const uint32_t d = tmem_base + acc * p.width;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&full[st], phase, kErrWaitFull)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t dw = umma_desc_sw128(smem_u32(smem_w + st * kWBytes));
-          const uint64_t dx = umma_desc_sw128(smem_u32(smem_x + st * C::kXBytes));
+          const uint64_t dw = umma_desc_sw128(smem_u32(smem + st * stage_size));
+          const uint64_t dx = umma_desc_sw128(smem_u32(smem + st * stage_size + kWBytes));
 #pragma unroll
           for (int k = 0; k < kBK / 32; ++k)
-            umma_i8(d, dw + (uint64_t)(2 * k), dx + (uint64_t)(2 * k), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
-          umma_commit(&empty[st]);
+            umma_i8<PAIR>(d, dw + (uint64_t)(2 * k), dx + (uint64_t)(2 * k), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+          commit<PAIR>(&empty[st], lead);
+          if (++st == stages) {
+            st = 0;
+            phase ^= 1;
+          }
         }
-        umma_commit(&tfull[acc]);
+        commit<PAIR>(&tfull[acc], lead);
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1;
         }
       }
       // every product has ended before the CTA does
-      umma_commit(drained);
+      commit<PAIR>(drained, lead);
+      mbar_wait<true>(drained, 0, kErrWaitTmemFull);
+    } else if (!leads && elect_one_sync()) {
       mbar_wait<true>(drained, 0, kErrWaitTmemFull);
     }
   } else {
-    const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;     // channel within the tile
-    const int et = threadIdx.x - 64;
-    O* out = reinterpret_cast<O*>(a.out);
-    const O* bias = reinterpret_cast<const O*>(a.bias);
-    int acc = 0;
+    const int quarter = warp & 3, group = (warp - 2) / 4;
+    const int row = quarter * 32 + lane;     // channel within the CTA's 128
+    const int gt = (threadIdx.x - 64) % 128;
+    const uint32_t lead_tempty = PAIR ? mapa_shared(smem_u32(tempty), lead) : 0u;
+    const Results<O> results(a);
+    int acc = 0, buffer = 0;
     uint32_t acc_phase = 0;
     for (int u = first; u < units; u += step) {
       const Unit at = unit_at(p, u);
       const int t0 = at.t * p.width, tokens = min(p.width, a.M - t0);
-      const int n = at.n * kInt8Block + row;
+      const int n0 = (at.n * kCtas + half) * kInt8Block;
+      float* xs = scales + acc * p.width;
+      float ws[4], b[4];
       if (!SPLIT) {
-        // this unit's token scales; the other half may still be read
-        for (int i = et; i < p.width; i += 128) scales[acc * CAP + i] = i < tokens ? a.x_scales[t0 + i] : 0.f;
-        named_barrier(2, 128);
+        // this unit's token scales; the other accumulator's may still be read
+        for (int i = threadIdx.x - 64; i < p.width; i += 256) xs[i] = i < tokens ? a.x_scales[t0 + i] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // of 16-bit results a thread has the channels lane / 4 + 8 i of its warp's 32, of 32-bit ones channel `lane`
+          const int n = n0 + (sizeof(O) == 2 ? quarter * 32 + 8 * i + lane / 4 : row);
+          ws[i] = n < a.N ? a.w_scales[n] : 0.f;
+          b[i] = a.bias && n < a.N ? float_of<O>(reinterpret_cast<const O*>(a.bias)[n]) : 0.f;
+          if (sizeof(O) == 4) break;
+        }
+        named_barrier(2, 256);
       }
       const bool ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, kErrWaitTmemFull));
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * CAP);
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * p.width);
       if (!SPLIT) {
-        const float ws = n < a.N ? a.w_scales[n] : 0.f;
-        const float b = bias && n < a.N ? float_of<O>(bias[n]) : 0.f;
-        if (ok) {
 #pragma unroll 1
-          for (int c = 0; c < tokens; c += 16) {
-            int v[16];
-            tmem_ld16(taddr + c, v);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float y = fmaf((float)v[i] * scales[acc * CAP + c + i], ws, b);
-              if (c + i < tokens && n < a.N) out[(long long)(t0 + c + i) * a.ldc + n] = out_of<O>(y);
-            }
-          }
+        for (int c = group * kChunk; c < tokens; c += 2 * kChunk) {
+          uint8_t* to = staged + (group * 2 + buffer) * kChunk * token_bytes(sizeof(O));
+          buffer ^= 1;
+          if (ok) stage_chunk<O>(taddr + c, xs + c, ws, b, to, quarter, lane);
+          named_barrier(3 + group, 128);      // the group's other buffer has been read by now
+          if (ok) results.write(to, token_bytes(sizeof(O)), t0 + c, min(kChunk, tokens - c), n0, gt);
         }
         tc_fence_before();
-        mbar_arrive(&tempty[acc]);
+        named_barrier(3 + group, 128);
+        if (gt == 0) PAIR ? mbar_arrive_remote(lead_tempty + 8u * acc) : mbar_arrive(&tempty[acc]);
       } else if (ok) {
         // this CTA's part of the sums, over the stages: all of them are used up
-        int* part = reinterpret_cast<int*>(smem);
+        int* sums = reinterpret_cast<int*>(smem);
 #pragma unroll 1
-        for (int c = 0; c < tokens; c += 16) {
+        for (int c = group * kChunk; c < tokens; c += 2 * kChunk) {
           int v[16];
           tmem_ld16(taddr + c, v);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) part[(c + i) * kInt8Block + row] = v[i];
+          for (int i = 0; i < 16; ++i) sums[(c + i) * kInt8Block + row] = v[i];
         }
       }
       if (++acc == 2) {
@@ -253,17 +427,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<CAP>::kPerSm)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem_base, C::kTmemCols);
+  if (PAIR || SPLIT) cluster_sync();     // the cluster's sums are written; a pair is done with both TMEMs and barriers
+  if (warp == 1) PAIR ? tmem_dealloc_pair(tmem_base, p.tmem_columns) : tmem_dealloc(tmem_base, p.tmem_columns);
   if (SPLIT) {
-    // the cluster's CTAs share the tile's tokens: each adds up all parts of
-    // its own (integers: any order gives the same)
-    cluster_sync();
+    // the CTAs that hold parts of the same sums share the tile's tokens: each
+    // adds up all parts of its own (integers: any order gives the same)
     const Unit at = unit_at(p, first);
     const int t0 = at.t * p.width, tokens = min(p.width, a.M - t0);
     const int share = (tokens + p.splits - 1) / p.splits;
-    const int n = at.n * kInt8Block + lane * 4;
-    const uint32_t part = smem_u32(smem);
-    O* out = reinterpret_cast<O*>(a.out);
+    const int n = (at.n * kCtas + half) * kInt8Block + lane * 4;
+    const uint32_t sums = smem_u32(smem);
+    const Results<O> results(a);
     const O* bias = reinterpret_cast<const O*>(a.bias);
     float ws[4], b[4];
 #pragma unroll
@@ -271,24 +445,34 @@ __global__ void __launch_bounds__(kThreads, Cfg<CAP>::kPerSm)
       ws[i] = n + i < a.N ? a.w_scales[n + i] : 0.f;
       b[i] = bias && n + i < a.N ? float_of<O>(bias[n + i]) : 0.f;
     }
-    for (int c = rank * share + warp; c < min(tokens, (rank + 1) * share); c += kThreads / 32) {
+    for (int c = part * share + warp; c < min(tokens, (part + 1) * share); c += kThreads / 32) {
       const float xs = a.x_scales[t0 + c];
-      const uint32_t at_c = part + (uint32_t)(c * kInt8Block + lane * 4) * 4;
+      const uint32_t at_c = sums + (uint32_t)(c * kInt8Block + lane * 4) * 4;
       int s[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
+      for (int r = 0; r < 8 / kCtas; ++r) {
         if (r < p.splits) {
-          const int4 v = ld_cluster(mapa_shared(at_c, r));
+          const int4 v = ld_cluster(mapa_shared(at_c, r * kCtas + half));
           s[0] += v.x;
           s[1] += v.y;
           s[2] += v.z;
           s[3] += v.w;
         }
       }
-      O* dst = out + (long long)(t0 + c) * a.ldc + n;
+      O* dst = results.out + (t0 + c) * results.ldc + n;
+      alignas(16) O y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < a.N) dst[i] = out_of<O>(fmaf((float)s[i] * xs, ws[i], b[i]));
+      for (int i = 0; i < 4; ++i) y[i] = out_of<O>(fmaf((float)s[i] * xs, ws[i], b[i]));
+      if (results.aligned && n + 4 <= a.N) {
+        if constexpr (sizeof(O) == 2)
+          *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+        else
+          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < a.N) dst[i] = y[i];
+      }
     }
     cluster_sync();    // no CTA ends while others read its part
   }
@@ -331,24 +515,19 @@ bool byte_map(CUtensorMap* map, const void* base, long long rows, int cols, long
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int CAP, typename O>
+template <typename O, bool PAIR, bool SPLIT>
 void launch(const Int8Gemm& a, const Int8Plan& p, const CUtensorMap& w, const CUtensorMap& x, cudaStream_t s) {
-  using C = Cfg<CAP>;
-  if (p.splits > 1) {
-    ensure_smem_attr(reinterpret_cast<const void*>(gemm_kernel<CAP, O, true>), C::kSmemBytes);
-    launch_kc(gemm_kernel<CAP, O, true>, dim3(p.grid), dim3(kThreads), C::kSmemBytes, s, p.splits, w, x, a, p);
-  } else {
-    ensure_smem_attr(reinterpret_cast<const void*>(gemm_kernel<CAP, O, false>), C::kSmemBytes);
-    launch_k(gemm_kernel<CAP, O, false>, dim3(p.grid), dim3(kThreads), C::kSmemBytes, s, w, x, a, p);
-  }
+  const auto kernel = gemm_kernel<O, PAIR, SPLIT>;
+  ensure_smem_attr(reinterpret_cast<const void*>(kernel), kSmemAlone);
+  launch_kc(kernel, dim3(p.grid), dim3(kThreads), smem_bytes(p, sizeof(O)), s, (PAIR ? 2 : 1) * p.splits, w, x, a, p);
 }
 
 template <typename O>
-void launch_cap(const Int8Gemm& a, const Int8Plan& p, const CUtensorMap& w, const CUtensorMap& x, cudaStream_t s) {
-  if (p.width <= 64)
-    launch<64, O>(a, p, w, x, s);
+void launch_as(const Int8Gemm& a, const Int8Plan& p, const CUtensorMap& w, const CUtensorMap& x, cudaStream_t s) {
+  if (p.pair)
+    p.splits > 1 ? launch<O, true, true>(a, p, w, x, s) : launch<O, true, false>(a, p, w, x, s);
   else
-    launch<256, O>(a, p, w, x, s);
+    p.splits > 1 ? launch<O, false, true>(a, p, w, x, s) : launch<O, false, false>(a, p, w, x, s);
 }
 
 }  // namespace i8gemm
@@ -362,28 +541,127 @@ void int8_pack(const int8_t* w, long long stride, int N, int K, int8_t* packed, 
                                                                                  vectors, on16);
 }
 
-Int8Plan int8_plan(int M, int N, int K, int sms) {
-  Int8Plan p{};
-  const int blocks = (int)int8_blocks(K);
-  p.token_tiles = (M + 255) / 256;
-  p.width = ((M + p.token_tiles - 1) / p.token_tiles + 15) / 16 * 16;
-  p.token_tiles = (M + p.width - 1) / p.width;
-  p.channel_tiles = (int)int8_blocks(N);
-  const long long units = (long long)p.token_tiles * p.channel_tiles;
-  const int slots = sms * (p.width <= 64 ? 2 : 1);
-  p.splits = 1;
-  if (units < slots) {
-    p.splits = (int)(slots / units);
-    if (p.splits > 8) p.splits = 8;
-    if (p.splits > blocks) p.splits = blocks;
-    const int each = (blocks + p.splits - 1) / p.splits;
-    p.splits = (blocks + each - 1) / each;
+Int8Slots int8_slots() {
+  using namespace i8gemm;
+  constexpr int kMaxDev = 64;
+  static std::mutex mu;
+  static Int8Slots known[kMaxDev];
+  static bool done[kMaxDev] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  if (dev >= 0 && dev < kMaxDev && done[dev]) return known[dev];
+  Int8Slots s{};
+  const auto kernel = gemm_kernel<float, true, true>;
+  ensure_smem_attr(reinterpret_cast<const void*>(kernel), kSmemAlone);
+  for (int c = 1; c <= 8; ++c) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c);
+    cfg.blockDim = dim3(i8gemm::kThreads);
+    cfg.dynamicSmemBytes = kSmemAlone;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = c;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+    s.clusters[c] = n;
   }
+  if (dev >= 0 && dev < kMaxDev) {
+    known[dev] = s;
+    done[dev] = true;
+  }
+  return s;
+}
+
+namespace i8gemm {
+
+// What a cut is expected to take, in us (less what every cut takes).  Of its
+// products, stage by stage: the loads (104 bytes a clock of a CTA alone on its
+// SM, 60 of each of two), 2 clocks a token, at least 290 clocks (145) of
+// latency; of the results 20 ns a token and tile to write; of the bytes that
+// HBM moves.  Each hides some of the others: their root of squares.  The last
+// tile is written when nothing is left to hide it, a round takes 0.63 us to
+// fill the stages, and adding up parts of K 2 us.  The numbers were fitted to
+// 863 cuts of 75 products (1 to 12000 tokens, 64 to 28672 channels, K 64 to
+// 16384): times are off by 10 % on average, and the cut that is cheapest by
+// this takes 1.4 % longer than the best, 12 % at most.
+double cost(const Int8Plan& p, int M, int N, int K, int element, const Int8Slots& slots) {
+  const int ctas = p.pair ? 2 : 1, blocks = (int)int8_blocks(K), units = p.token_tiles * p.channel_tiles;
+  const int each = (blocks + p.splits - 1) / p.splits;
+  // times that one CTA after another runs on an SM; two at once share it
+  const int waves = p.splits > 1 ? 1 : (units + slots.clusters[ctas] - 1) / slots.clusters[ctas];
+  const int rounds = p.splits > 1 && !p.alone ? 2 : waves;
+  const double stage = std::max({stage_bytes(p) / (p.alone ? 104.0 : 60.0), 2.0 * p.width, p.alone ? 290.0 : 145.0});
+  const double write = 0.02 * p.width;
+  const double products = rounds * each * stage / 1.9e3, writes = p.splits > 1 ? 0 : rounds * write;
+  const double moved = ((double)N * K + (double)M * K + (double)M * N * element) / 7.2e6;
+  double t = std::sqrt(products * products + writes * writes + moved * moved) + write;
+  t += 0.63 * (p.alone ? waves : (waves + 1) / 2);
+  if (p.splits > 1) t += 2.0 + 0.005 * p.width * (p.splits - 1) / p.splits;
+  return t;
+}
+
+}  // namespace i8gemm
+
+// The cheapest of: single CTAs (up to 200 tokens; from there pairs, which load
+// half the tokens each, took less in every case) or pairs, tiles of 16 to 256
+// tokens, K whole or split over a cluster's CTAs, one CTA an SM or two.
+// Clusters of a split all run at once: a second wave would double the time
+// (40 tiles of 5120 x 5120: 8.7 us split over 6, 13.7 over 7).  Two CTAs an SM
+// only where one each would leave some out: they are placed two by two even
+// where SMs stay idle (306 x 13824 x 5120 in 120 CTAs: 44 us, alone 27).
+Int8Plan int8_plan(int M, int N, int K, int element, const Int8Slots& slots) {
+  using namespace i8gemm;
+  const int blocks = (int)int8_blocks(K);
+  Int8Plan best{};
+  double least = 0;
+  for (int pair = M > 200; pair < 2; ++pair) {
+    const int ctas = pair ? 2 : 1, step = 16 * ctas;
+    int last = 0;
+    for (int tile = step; tile <= 256; tile += tile < 32 ? 16 : 32) {
+      Int8Plan p{};
+      p.pair = pair;
+      p.token_tiles = (M + tile - 1) / tile;
+      if (p.token_tiles > 64 && tile < 256) continue;
+      p.width = ((M + p.token_tiles - 1) / p.token_tiles + step - 1) / step * step;
+      if (p.width == last) continue;
+      last = p.width;
+      p.token_tiles = (M + p.width - 1) / p.width;
+      p.channel_tiles = (int)((int8_blocks(N) + ctas - 1) / ctas);
+      const int units = p.token_tiles * p.channel_tiles;
+      for (int splits = 1; splits * ctas <= 8 && splits <= blocks; ++splits) {
+        const int each = (blocks + splits - 1) / splits, clusters = slots.clusters[splits * ctas];
+        if ((splits - 1) * each >= blocks) continue;      // the last would have nothing
+        if (splits > 1 && units > 2 * clusters) break;
+        p.splits = splits;
+        for (int alone = 0; alone < 2; ++alone) {
+          if (alone ? splits > 1 && units > clusters : p.width > 128 || units <= clusters) continue;
+          p.alone = alone;
+          const double t = cost(p, M, N, K, element, slots);
+          if (best.width == 0 || t < least) {
+            best = p;
+            least = t;
+          }
+        }
+      }
+    }
+  }
+  Int8Plan& p = best;
+  const int ctas = p.pair ? 2 : 1, units = p.token_tiles * p.channel_tiles;
+  const int most = (p.alone ? 1 : 2) * slots.clusters[ctas];
+  p.grid = ctas * (p.splits > 1 ? units * p.splits : std::min(units, most));
+  p.tmem_columns = 32;
+  while (p.tmem_columns < 2 * p.width) p.tmem_columns *= 2;
+  p.stages = kMostStages;
+  while (smem_bytes(p, element) > (p.alone ? kSmemAlone : kSmemHalf)) --p.stages;
   // the tokens of a group: at most 32 MB
-  const long long tile = (long long)p.width * K;
-  const long long group = (32ll << 20) / tile;
-  p.group = (int)(group < 1 ? 1 : group > p.token_tiles ? p.token_tiles : group);
-  p.grid = p.splits > 1 ? (int)units * p.splits : (int)(units < slots ? units : slots);
+  p.group = (int)std::max(1ll, std::min<long long>(p.token_tiles, (32ll << 20) / ((long long)p.width * K)));
   return p;
 }
 
@@ -392,17 +670,17 @@ bool int8_weight_map(CUtensorMap* map, const int8_t* packed, int N, int K) {
   return rows < (1ll << 31) && i8gemm::byte_map(map, packed, rows, kInt8Block, kInt8Block, kInt8Block);
 }
 
-bool int8_token_map(CUtensorMap* map, const int8_t* x, long long stride, int M, int K, int width) {
-  return i8gemm::byte_map(map, x, M, K, stride, width);
+bool int8_token_map(CUtensorMap* map, const int8_t* x, long long stride, int M, int K, const Int8Plan& p) {
+  return i8gemm::byte_map(map, x, M, K, stride, i8gemm::x_rows(p));
 }
 
 void int8_gemm(const Int8Gemm& a, const Int8Plan& p, const CUtensorMap& weights, const CUtensorMap& tokens,
                cudaStream_t s) {
   if (a.M == 0) return;
   LaunchBehind behind;
-  if (a.type == kInt8TypeBF16) return i8gemm::launch_cap<__nv_bfloat16>(a, p, weights, tokens, s);
-  if (a.type == kInt8TypeFP16) return i8gemm::launch_cap<__half>(a, p, weights, tokens, s);
-  return i8gemm::launch_cap<float>(a, p, weights, tokens, s);
+  if (a.type == kInt8TypeBF16) return i8gemm::launch_as<__nv_bfloat16>(a, p, weights, tokens, s);
+  if (a.type == kInt8TypeFP16) return i8gemm::launch_as<__half>(a, p, weights, tokens, s);
+  return i8gemm::launch_as<float>(a, p, weights, tokens, s);
 }
 
 }  // namespace kus

@@ -60,17 +60,26 @@ struct Int8Gemm {
 };
 // How the kernel cuts a product.
 struct Int8Plan {
-  int width;                 // tokens of a tile (a multiple of 16)
+  int pair;                  // pairs of CTAs share 256 channels; else a CTA has 128
+  int width;                 // tokens of a tile (a multiple of 16, of a pair 32)
   int token_tiles, channel_tiles;
-  int splits;                // CTAs of a cluster that share a tile's K
+  int splits;                // CTAs (pairs) of a cluster that share a tile's K
+  int alone;                 // one CTA an SM; else two
   int group;                 // token tiles walked before the next channel tile
-  int grid;
+  int grid;                  // CTAs
+  int stages, tmem_columns;
 };
-Int8Plan int8_plan(int M, int N, int K, int sms);
+// Clusters of 1 to 8 CTAs that the device holds at once, with one CTA an SM.
+struct Int8Slots {
+  int clusters[9];
+};
+Int8Slots int8_slots();
+// `element`: bytes of a result.
+Int8Plan int8_plan(int M, int N, int K, int element, const Int8Slots& slots);
 // Tensor maps of the packed weights (made once) and of the tokens (each call;
 // base and row stride are multiples of 16 bytes).
 bool int8_weight_map(CUtensorMap* map, const int8_t* packed, int N, int K);
-bool int8_token_map(CUtensorMap* map, const int8_t* x, long long stride, int M, int K, int width);
+bool int8_token_map(CUtensorMap* map, const int8_t* x, long long stride, int M, int K, const Int8Plan& p);
 void int8_gemm(const Int8Gemm& a, const Int8Plan& p, const CUtensorMap& weights, const CUtensorMap& tokens,
                cudaStream_t s);
 

@@ -5,7 +5,10 @@ import random
 import pytest
 import torch  # noqa: F401  (loads what the extension links)
 
-SMS = 148
+# clusters of 1 to 8 CTAs that a B200 holds at once, one CTA an SM; and a device of few
+B200 = [0, 148, 74, 45, 33, 26, 22, 15, 15]
+SMALL = [0, 10, 5, 3, 2, 1, 1, 1, 1]
+SHARED = {True: 232448, False: 115712}      # bytes a CTA may have, alone on its SM or one of two
 
 
 def _units(p):
@@ -16,24 +19,35 @@ def _units(p):
         yield r // wide, g * p["group"] + r % wide
 
 
-@pytest.mark.parametrize("seed", range(8))
-def test_every_tile_once(seed):
+@pytest.mark.parametrize("slots", [B200, SMALL])
+@pytest.mark.parametrize("seed", range(6))
+def test_every_tile_once(seed, slots):
     native = pytest.importorskip("kunserve_b200._C")
     rng = random.Random(seed)
     for _ in range(150):
-        m, n, k = (int(2 ** (rng.random() * b)) for b in (14, 17, 17))
-        p = native.int8_plan(m, n, min(k, 131071), SMS)
-        assert p["width"] % 16 == 0 and 16 <= p["width"] <= 256
+        m, n, k = (max(1, min(131071, int(2 ** (rng.random() * b)))) for b in (14, 17, 17))
+        element = rng.choice([2, 4])
+        p = native.int8_plan(m, n, k, element, slots)
+        ctas = 2 if p["pair"] else 1
+        assert p["width"] % (16 * ctas) == 0 and 16 * ctas <= p["width"] <= 256
         assert (p["token_tiles"] - 1) * p["width"] < m <= p["token_tiles"] * p["width"]
-        assert (p["channel_tiles"] - 1) * 128 < n <= p["channel_tiles"] * 128
-        blocks = -(-min(k, 131071) // 128)
+        assert (p["channel_tiles"] - 1) * 128 * ctas < n <= p["channel_tiles"] * 128 * ctas
+        blocks = -(-k // 128)
         each = -(-blocks // p["splits"])
-        assert 1 <= p["splits"] <= 8 and (p["splits"] - 1) * each < blocks <= p["splits"] * each
+        assert 1 <= p["splits"] <= 8 // ctas and (p["splits"] - 1) * each < blocks <= p["splits"] * each
         units = p["channel_tiles"] * p["token_tiles"]
+        assert p["grid"] % (ctas * p["splits"]) == 0
         if p["splits"] > 1:
-            assert p["grid"] == units * p["splits"]
+            assert p["grid"] == ctas * units * p["splits"]
         else:
-            assert 0 < p["grid"] <= units
+            assert 0 < p["grid"] <= ctas * units
+        # shared memory: stages, two buffers for each epilogue group, scales, barriers; the parts of a split lie over
+        # the stages.  TMEM: two accumulators, of each of two CTAs an SM
+        stage = 128 * 128 + p["width"] // ctas * 128
+        staged = 4 * 16 * (128 * element + (16 if element == 2 else 0))
+        assert 2 <= p["stages"] <= 8 and p["width"] * 512 <= p["stages"] * stage or p["splits"] == 1
+        assert p["stages"] * stage + staged + 8 * p["width"] + 21 * 8 + 16 + 1024 <= SHARED[bool(p["alone"])]
+        assert 2 * p["width"] <= p["tmem_columns"] <= (512 if p["alone"] else 256)
         if units < 20000:
             seen = set(_units(p))
             assert len(seen) == units
