@@ -8,6 +8,7 @@
 // The norm's factor is common to a row, so max|y| = rstd max|h w| and
 // q = rint(127 h w / max|h w|): sum h^2 and max|h w| come from one reduction
 // over registers, and each element is read once and written once.
+#include <algorithm>
 #include <type_traits>
 
 #include "../common.cuh"
@@ -24,24 +25,56 @@ KUS_DEVICE float max_nan(float a, float b) {
   return r;
 }
 
-// 1 / x to one step
-KUS_DEVICE float rcp(float x) {
+// 1 / (1 + e^-g) to five roundings: one step of each function, one of the
+// sum.  Zero from g < -87 on, where it leaves the normal range.
+KUS_DEVICE float sigmoid(float g) {
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + expf(-g)));
   return r;
 }
 
-// 8 elements from 16-byte vectors
+// The largest of non-negative floats, NaN above all: their bits' order.
+KUS_DEVICE float warp_top(float v) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+
+// 8 neighbours of a row as they lie in memory.
 template <typename T>
-KUS_DEVICE void load8(const T* p, float (&f)[8]) {
-  unpack8<T>(*reinterpret_cast<const uint4*>(p), f);
-}
+struct Raw8 {
+  using V2 = typename Elem<T>::V2;
+  uint4 u;
+  KUS_DEVICE void load(const T* p, bool there) {
+    u = there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+  }
+  KUS_DEVICE void values(float (&f)[8]) const { unpack8<T>(u, f); }
+  // largest magnitude, NaN above all
+  KUS_DEVICE float top() const {
+    const V2* v = reinterpret_cast<const V2*>(&u);
+    const V2 m = __hmax2_nan(__hmax2_nan(__habs2(v[0]), __habs2(v[1])), __hmax2_nan(__habs2(v[2]), __habs2(v[3])));
+    const float2 f = Elem<T>::to_f2(m);
+    return max_nan(f.x, f.y);
+  }
+};
 template <>
-KUS_DEVICE void load8<float>(const float* p, float (&f)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
+struct Raw8<float> {
+  float4 a, b;
+  KUS_DEVICE void load(const float* p, bool there) {
+    a = there ? reinterpret_cast<const float4*>(p)[0] : make_float4(0, 0, 0, 0);
+    b = there ? reinterpret_cast<const float4*>(p)[1] : make_float4(0, 0, 0, 0);
+  }
+  KUS_DEVICE void values(float (&f)[8]) const {
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+  KUS_DEVICE float top() const {
+    float f[8], m = 0.f;
+    values(f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(f[e]));
+    return m;
+  }
+};
+
 template <typename T>
 KUS_DEVICE float to_float(T x) { return Elem<T>::to_f(x); }
 template <>
@@ -71,183 +104,232 @@ struct Row {
         total(a.total ? reinterpret_cast<T*>(a.total) + t * a.ts : nullptr),
         K(a.K) {}
 
-  // The row's values (the norm's without its common factor) of 8 columns;
-  // `sum` gains h^2.  `keep`: write x + residual.
-  template <bool VEC>
-  KUS_DEVICE void values(int j, int lane, int lanes, bool keep, float (&y)[8], float& sum) const {
+  // y of 8 columns (the norm's without its common factor) from their inputs,
+  // y holding x; `sum` gains h^2.
+  KUS_DEVICE static void combine(float (&y)[8], const float (&w)[8], float& sum) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      sum = fmaf(y[e], y[e], sum);
+      y[e] *= w[e];
+    }
+  }
+  KUS_DEVICE static void gate(float (&y)[8], const float (&o)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = y[e] * sigmoid(y[e]) * o[e];
+  }
+
+  // Element by element; `keep`: write x + residual.
+  KUS_DEVICE void values(int c0, bool keep, float (&y)[8], float& sum) const {
     float o[8], w[8];
-    if (VEC) {
-      const int c = column(j, lane, lanes);
-      if (c >= K) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = 0.f;
-        return;
-      }
-      load8<T>(x + c, y);
-      if (OP == kRowsSilu || (OP == kRowsNorm && other)) load8<T>(other + c, o);
-      if (OP == kRowsNorm) load8<T>(weight + c, w);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = column(j, lane, lanes) + e;
-        y[e] = o[e] = w[e] = 0.f;
-        if (c >= K) continue;
-        y[e] = to_float<T>(x[c]);
-        if (OP == kRowsSilu || (OP == kRowsNorm && other)) o[e] = to_float<T>(other[c]);
-        if (OP == kRowsNorm) w[e] = to_float<T>(weight[c]);
+    for (int e = 0; e < 8; ++e) {
+      const int c = c0 + e;
+      y[e] = o[e] = w[e] = 0.f;
+      if (c >= K) continue;
+      y[e] = to_float<T>(x[c]);
+      if (OP == kRowsSilu || (OP == kRowsNorm && other)) o[e] = to_float<T>(other[c]);
+      if (OP == kRowsNorm) w[e] = to_float<T>(weight[c]);
+      if (OP == kRowsNorm && other) {
+        y[e] += o[e];
+        if (keep) total[c] = from_float<T>(y[e]);
       }
     }
-    if (OP == kRowsNorm) {
-      if (other) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] += o[e];
-        if (keep) {
-          if constexpr (!std::is_same<T, float>::value) {
-            if (VEC) {
-              *reinterpret_cast<uint4*>(total + column(j, lane, lanes)) = pack8<T>(y);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const int c = column(j, lane, lanes) + e;
-                if (c < K) total[c] = from_float<T>(y[e]);
-              }
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        sum = fmaf(y[e], y[e], sum);
-        y[e] *= w[e];
-      }
-    }
-    if (OP == kRowsSilu) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = y[e] * rcp(1.f + expf(-y[e])) * o[e];
-    }
+    if (OP == kRowsNorm) combine(y, w, sum);
+    if (OP == kRowsSilu) gate(y, o);
   }
 };
 
-// The integers nearest to 127 v / top, two's complement, in the low bytes.
-// The quotient is that of a product with 1 / top, put right by its remainder
-// once (Markstein 1990): where 127 v / top is a float, a half say, the result
-// is that float, and halves go to even.  Adding 1.5 * 2^23 rounds to a whole
-// number and leaves it in the low bits; a conversion runs at a quarter of the
-// rate.
+// The integers nearest to 127 v / top, two's complement, in the low bytes:
+// adding 1.5 * 2^23 rounds to a whole number and leaves it in the low bits (a
+// conversion runs at a quarter of the rate).  Of quantised inputs the quotient
+// is that of a product with 1 / top, put right by its remainder once
+// (Markstein 1990): where 127 v / top is a float, a half say, the result is
+// that float, and halves go to even.  Computed values have roundings of their
+// own: v times 127 / top does.
 struct Quotient {
-  float times, over, inverse;
-  KUS_DEVICE Quotient(float top, bool sound) {
+  float times, over, inverse, factor;
+  bool exact;
+  KUS_DEVICE Quotient(float top, bool sound, bool exact_) {
+    const bool range = top > 1e36f || top < 1e-30f;
     const float small = top > 1e36f ? 0x1p-10f : top < 1e-30f ? 0x1p60f : 1.f;   // 127 v and 1 / top stay in range
     over = sound && top > 0.f ? top * small : 1.f;
     times = sound ? 127.f * small : 0.f;
     inverse = 1.f / over;
+    factor = 127.f / over;
+    exact = exact_ || range;
   }
-  KUS_DEVICE uint32_t operator()(float v) const {
+  KUS_DEVICE uint32_t near(float v) const { return __float_as_uint(fmaf(v, factor, 12582912.f)); }
+  KUS_DEVICE uint32_t nearest(float v) const {
     const float t = v * times, r = t * inverse;
     return __float_as_uint(fmaf(fmaf(-r, over, t), inverse, r) + 12582912.f);
   }
 };
 
-// One row a warp (WARPS == 1; eight warps a block) or a block.  HELD: vectors
-// of 8 a thread keeps between the two passes over its row; 0: the row is read
-// again.
-template <typename T, int OP, bool ONE_WARP, int HELD, bool VEC>
+// Over the warp, and over the block through `part` (32 entries, not written
+// again before every thread has read them).
+KUS_DEVICE void reduce_warp(int op, float& sum, float& top) {
+  if (op == kRowsNorm) sum = warp_sum(sum);
+  top = warp_top(top);
+}
+KUS_DEVICE void reduce_block(int op, float& sum, float& top, float2* part) {
+  const int l = threadIdx.x % 32;
+  if (l == 0) part[threadIdx.x / 32] = make_float2(sum, top);
+  __syncthreads();
+  const float2 p = l < blockDim.x / 32 ? part[l] : make_float2(0.f, 0.f);
+  sum = p.x;
+  top = p.y;
+  reduce_warp(op, sum, top);
+}
+
+// A row's scale, and its integers.  A row without finite values has scale NaN.
+template <int OP>
+struct Writer {
+  int8_t* q;
+  int K;
+  bool sound;
+  Quotient quotient;
+
+  KUS_DEVICE Writer(const Int8Rows& a, long long t, float sum, float top, bool first)
+      : q(a.q + t * a.qs),
+        K(a.K),
+        sound(top < INFINITY && (OP != kRowsNorm || sum < INFINITY)),
+        quotient(top, sound, OP == kRowsQuantize) {
+    if (first) a.scales[t] = sound ? top / 127.f * (OP == kRowsNorm ? rsqrtf(sum / (float)a.K + a.eps) : 1.f) : NAN;
+  }
+  KUS_DEVICE void integers(const float (&v)[8], uint32_t (&r)[8]) const {
+    if (OP == kRowsQuantize || quotient.exact) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = quotient.nearest(v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = quotient.near(v[e]);
+    }
+  }
+  KUS_DEVICE void write_vec(int c, const float (&v)[8]) const {
+    if (c >= K) return;
+    uint32_t r[8];
+    integers(v, r);
+    uint2 u;
+    u.x = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+    u.y = __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410);
+    *reinterpret_cast<uint2*>(q + c) = sound ? u : make_uint2(0, 0);
+  }
+  KUS_DEVICE void write(int c, const float (&v)[8]) const {
+    uint32_t r[8];
+    integers(v, r);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < K) q[c + e] = sound ? (int8_t)r[e] : (int8_t)0;
+  }
+};
+
+// A row of whole vectors in a thread's registers: HELD vectors of 8, the
+// inputs of a quantisation as they came, else y.
+template <typename T, int OP, int HELD>
+struct Held {
+  Raw8<T> raw[OP == kRowsQuantize ? HELD : 1];
+  float y[OP == kRowsQuantize ? 1 : HELD][8];
+
+  KUS_DEVICE void read(const Row<T, OP>& row, int lane, int lanes, float& sum, float& top) {
+    constexpr int kOther = OP == kRowsQuantize ? 1 : HELD;
+    Raw8<T> x[HELD], o[kOther];
+    const bool two = OP == kRowsSilu || (OP == kRowsNorm && row.other);
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      const int c = column(j, lane, lanes);
+      x[j].load(row.x + c, c < row.K);
+      if (OP != kRowsQuantize) o[j % kOther].load(row.other + c, two && c < row.K);
+    }
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      if constexpr (OP == kRowsQuantize) {
+        raw[j] = x[j];
+        top = max_nan(top, x[j].top());
+      } else {
+        float f[8];
+        x[j].values(y[j]);
+        o[j].values(f);
+        if constexpr (OP == kRowsNorm) {
+          if (two) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[j][e] += f[e];
+            const int c = column(j, lane, lanes);
+            if (c < row.K) *reinterpret_cast<uint4*>(row.total + c) = pack8<T>(y[j]);
+          }
+          Raw8<T> w;
+          w.load(row.weight + column(j, lane, lanes), column(j, lane, lanes) < row.K);
+          w.values(f);
+          Row<T, OP>::combine(y[j], f, sum);
+        } else {
+          Row<T, OP>::gate(y[j], f);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(y[j][e]));
+      }
+    }
+  }
+  KUS_DEVICE void write(const Writer<OP>& writer, int lane, int lanes) const {
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      float v[8];
+      if constexpr (OP == kRowsQuantize) {
+        raw[j].values(v);
+        writer.write_vec(column(j, lane, lanes), v);
+      } else {
+        writer.write_vec(column(j, lane, lanes), y[j]);
+      }
+    }
+  }
+};
+
+// One row a warp (ONE_WARP; eight of them a block) or a block, in whole
+// vectors.
+template <typename T, int OP, bool ONE_WARP, int HELD>
 __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_kernel(Int8Rows a) {
   __shared__ float2 part[32];
   pdl_wait();
   pdl_trigger();
-  const int lanes = ONE_WARP ? 32 : blockDim.x;
-  const int lane = ONE_WARP ? threadIdx.x % 32 : threadIdx.x;
+  const int lanes = ONE_WARP ? 32 : blockDim.x, lane = ONE_WARP ? threadIdx.x % 32 : threadIdx.x;
   const long long t = ONE_WARP ? (long long)blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x;
   if (ONE_WARP && t >= a.T) return;
-  const Row<T, OP> row(a, t);
-  const int vectors = HELD > 0 ? HELD : (a.K + 8 * lanes - 1) / (8 * lanes);
-
-  float y[HELD > 0 ? HELD : 1][8];
   float sum = 0.f, top = 0.f;
-  if (HELD > 0) {
-#pragma unroll
-    for (int j = 0; j < HELD; ++j) row.template values<VEC>(j, lane, lanes, true, y[j], sum);
-#pragma unroll
-    for (int j = 0; j < HELD; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(y[j][e]));
-  } else {
-    for (int j = 0; j < vectors; ++j) {
-      row.template values<VEC>(j, lane, lanes, false, y[0], sum);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(y[0][e]));
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    if (OP == kRowsNorm) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-  }
-  if (!ONE_WARP) {
-    const int warps = blockDim.x / 32, l = threadIdx.x % 32;
-    if (l == 0) part[threadIdx.x / 32] = make_float2(sum, top);
-    __syncthreads();
-    const float2 p = l < warps ? part[l] : make_float2(0.f, 0.f);
-    sum = p.x;
-    top = p.y;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      if (OP == kRowsNorm) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
-  }
+  Held<T, OP, HELD> held;
+  held.read(Row<T, OP>(a, t), lane, lanes, sum, top);
+  reduce_warp(OP, sum, top);
+  if (!ONE_WARP) reduce_block(OP, sum, top, part);
+  held.write(Writer<OP>(a, t, sum, top, lane == 0), lane, lanes);
+}
 
-  // scale and the integers' factor; a row without finite values has scale NaN
-  float factor = 1.f;
-  bool sound = top < INFINITY;
-  if (OP == kRowsNorm) {
-    factor = rsqrtf(sum / (float)a.K + a.eps);
-    sound = sound && sum < INFINITY;
+// Any rows, read twice and element by element, a row a block.  The columns of
+// a thread are those of rows_kernel.
+template <typename T, int OP>
+__global__ void __launch_bounds__(1024) any_rows_kernel(Int8Rows a) {
+  __shared__ float2 part[32];
+  pdl_wait();
+  pdl_trigger();
+  const long long t = blockIdx.x;
+  const Row<T, OP> row(a, t);
+  float sum = 0.f, top = 0.f, y[8];
+  for (int c = threadIdx.x * 8; c < a.K; c += blockDim.x * 8) {
+    row.values(c, false, y, sum);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(y[e]));
   }
-  if (lane == 0) a.scales[t] = sound ? top / 127.f * factor : NAN;
-  const Quotient quotient(top, sound);
-  int8_t* q = a.q + t * a.qs;
-  auto write = [&](int j, const float (&v)[8]) {
-    uint32_t r[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = sound ? quotient(v[e]) : 0;
-    const int c = column(j, lane, lanes);
-    if (VEC) {
-      uint2 u;
-      u.x = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
-      u.y = __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410);
-      if (c < a.K) *reinterpret_cast<uint2*>(q + c) = u;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c + e < a.K) q[c + e] = (int8_t)r[e];
-    }
-  };
-  if (HELD > 0) {
-#pragma unroll
-    for (int j = 0; j < HELD; ++j) write(j, y[j]);
-  } else {
-    // the sum x + residual is written in the second pass: it may lie over either of them
-    for (int j = 0; j < vectors; ++j) {
-      float unused = 0.f;
-      row.template values<VEC>(j, lane, lanes, true, y[0], unused);
-      write(j, y[0]);
-    }
+  reduce_warp(OP, sum, top);
+  reduce_block(OP, sum, top, part);
+  const Writer<OP> writer(a, t, sum, top, threadIdx.x == 0);
+  // the sum x + residual is written in the second pass: it may lie over either of them
+  for (int c = threadIdx.x * 8; c < a.K; c += blockDim.x * 8) {
+    float unused = 0.f;
+    row.values(c, true, y, unused);
+    writer.write(c, y);
   }
 }
 
 template <typename T, int OP, bool ONE_WARP, int HELD>
-void launch(const Int8Rows& a, bool vec, cudaStream_t s) {
-  const int vectors = (a.K + 7) / 8;
-  const int each = HELD > 0 ? HELD : 4;
-  int threads = ONE_WARP ? 256 : ((vectors + each - 1) / each + 31) / 32 * 32;
-  if (threads > 1024) threads = 1024;
-  const dim3 grid((unsigned)(ONE_WARP ? (a.T + 7) / 8 : a.T));
-  if (vec)
-    launch_k(rows_kernel<T, OP, ONE_WARP, HELD, true>, grid, dim3(threads), 0, s, a);
-  else
-    launch_k(rows_kernel<T, OP, ONE_WARP, HELD, false>, grid, dim3(threads), 0, s, a);
+void launch(const Int8Rows& a, cudaStream_t s) {
+  const int threads = ONE_WARP ? 256 : ((a.K / 8 + HELD - 1) / HELD + 31) / 32 * 32;
+  launch_k(rows_kernel<T, OP, ONE_WARP, HELD>, dim3((unsigned)(ONE_WARP ? (a.T + 7) / 8 : a.T)), dim3(threads), 0, s, a);
 }
 
 bool on16(const void* p, long long stride, int bytes, int rows) {
@@ -260,12 +342,15 @@ void launch_op(const Int8Rows& a, cudaStream_t s) {
   const bool vec = a.K % 8 == 0 && on16(a.x, a.xs, el, a.T) && (!a.other || on16(a.other, a.os, el, a.T)) &&
                    (!a.weight || on16(a.weight, 0, el, 1)) && (!a.total || on16(a.total, a.ts, el, a.T));
   const int n = (a.K + 7) / 8;
-  if (n <= 32) return launch<T, OP, true, 1>(a, vec, s);
-  if (n <= 64) return launch<T, OP, true, 2>(a, vec, s);
-  if (n <= 256) return launch<T, OP, false, 1>(a, vec, s);
-  if (n <= 1024) return launch<T, OP, false, 2>(a, vec, s);
-  if (n <= 4096) return launch<T, OP, false, 4>(a, vec, s);
-  return launch<T, OP, false, 0>(a, vec, s);
+  if (!vec || n > 4096) {
+    const int threads = std::min(1024, ((n + 1) / 2 + 31) / 32 * 32);
+    launch_k(any_rows_kernel<T, OP>, dim3((unsigned)a.T), dim3(threads), 0, s, a);
+    return;
+  }
+  if (n <= 32) return launch<T, OP, true, 1>(a, s);
+  if (n <= 64) return launch<T, OP, true, 2>(a, s);
+  if (n <= (OP == kRowsNorm ? 1024 : 256)) return launch<T, OP, false, 2>(a, s);
+  return launch<T, OP, false, 4>(a, s);
 }
 
 // The float of byte i of u, whose bytes are integers with their top bit
