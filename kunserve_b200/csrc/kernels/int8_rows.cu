@@ -84,6 +84,71 @@ KUS_DEVICE T from_float(float x) { return Elem<T>::from_f(x); }
 template <>
 KUS_DEVICE float from_float<float>(float x) { return x; }
 
+// 16 bytes from byte `by` (even, below 16) of 32.
+KUS_DEVICE uint4 shifted(const uint4& a, const uint4& b, int by) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (by & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (by & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  const int bits = (by & 2) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// 8 neighbours from column c of a 16-bit row that starts anywhere: inside the
+// row from the two aligned vectors that hold them (both lie in the row), at
+// its ends one by one.
+template <typename T>
+KUS_DEVICE uint4 load_anywhere(const T* row, int c, int K) {
+  if (c >= 8 && c + 16 <= K) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + c);
+    const int by = (int)(at & 15);
+    const uint4* p = reinterpret_cast<const uint4*>(at - by);
+    const uint4 a = p[0];
+    return by ? shifted(a, p[1], by) : a;
+  }
+  uint32_t w[4] = {0, 0, 0, 0};
+  for (int e = 0; e < 8; ++e)
+    if (c + e < K) w[e / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(row)[c + e] << (16 * (e & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The same for writing, by a whole warp whose lanes hold neighbouring groups
+// of 8: a lane writes the aligned vector that its group and the next lane's
+// share; what is left at the warp's and the row's ends goes one by one.
+template <typename T>
+KUS_DEVICE void store_anywhere(T* row, int c, int K, const uint4& v) {
+  T* p = row + c;
+  const int by = (int)(reinterpret_cast<uintptr_t>(p) & 15), head = by ? 8 - by / 2 : 8;    // elements before the vector
+  const uint4 next = make_uint4(__shfl_down_sync(0xffffffffu, v.x, 1), __shfl_down_sync(0xffffffffu, v.y, 1),
+                                __shfl_down_sync(0xffffffffu, v.z, 1), __shfl_down_sync(0xffffffffu, v.w, 1));
+  const int lane = threadIdx.x % 32;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  auto one_by_one = [&](int from, int to) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e >= from && e < to && c + e < K)
+        reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+  };
+  if (by == 0) {
+    if (c + 8 <= K)
+      *reinterpret_cast<uint4*>(p) = v;
+    else
+      one_by_one(0, 8);
+    return;
+  }
+  if (lane == 0 || c + head > K) one_by_one(0, head);
+  if (lane < 31 && c + head + 8 <= K)
+    *reinterpret_cast<uint4*>(p + head) = shifted(v, next, 16 - by);
+  else
+    one_by_one(head, 8);
+}
+
 // First column of vector j of a thread.  Rows that start elsewhere than on 16
 // bytes are read element by element, but each by the same thread: the order
 // of the norm's sum, and so its bits, do not depend on strides.
@@ -205,31 +270,39 @@ struct Writer {
       for (int e = 0; e < 8; ++e) r[e] = quotient.near(v[e]);
     }
   }
-  KUS_DEVICE void write_vec(int c, const float (&v)[8]) const {
+  // 8 columns from c, a multiple of 8 (rows of q start on 16 bytes).
+  KUS_DEVICE void write(int c, const float (&v)[8]) const {
     if (c >= K) return;
     uint32_t r[8];
     integers(v, r);
     uint2 u;
     u.x = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
     u.y = __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410);
-    *reinterpret_cast<uint2*>(q + c) = sound ? u : make_uint2(0, 0);
-  }
-  KUS_DEVICE void write(int c, const float (&v)[8]) const {
-    uint32_t r[8];
-    integers(v, r);
+    if (!sound) u = make_uint2(0, 0);
+    if (c + 8 <= K) {
+      *reinterpret_cast<uint2*>(q + c) = u;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c + e < K) q[c + e] = sound ? (int8_t)r[e] : (int8_t)0;
+      for (int e = 0; e < 7; ++e)
+        if (c + e < K) q[c + e] = (int8_t)((e < 4 ? u.x : u.y) >> (8 * (e % 4)));
+    }
   }
 };
 
-// A row of whole vectors in a thread's registers: HELD vectors of 8, the
-// inputs of a quantisation as they came, else y.
-template <typename T, int OP, int HELD>
+// A row in registers: HELD vectors of 8 a thread, the inputs of a quantisation
+// as they came, else y.
+// ANYWHERE: rows that start on any element (16 bits).
+template <typename T, int OP, int HELD, bool ANYWHERE>
 struct Held {
   Raw8<T> raw[OP == kRowsQuantize ? HELD : 1];
   float y[OP == kRowsQuantize ? 1 : HELD][8];
 
+  KUS_DEVICE static void load(Raw8<T>& r, const T* row, int c, int K) {
+    if constexpr (ANYWHERE)
+      r.u = load_anywhere(row, c, K);
+    else
+      r.load(row + c, c < K);
+  }
   KUS_DEVICE void read(const Row<T, OP>& row, int lane, int lanes, float& sum, float& top) {
     constexpr int kOther = OP == kRowsQuantize ? 1 : HELD;
     Raw8<T> x[HELD], o[kOther];
@@ -237,8 +310,8 @@ struct Held {
 #pragma unroll
     for (int j = 0; j < HELD; ++j) {
       const int c = column(j, lane, lanes);
-      x[j].load(row.x + c, c < row.K);
-      if (OP != kRowsQuantize) o[j % kOther].load(row.other + c, two && c < row.K);
+      load(x[j], row.x, c, row.K);
+      if (OP != kRowsQuantize && two) load(o[j % kOther], row.other, c, row.K);
     }
 #pragma unroll
     for (int j = 0; j < HELD; ++j) {
@@ -248,16 +321,19 @@ struct Held {
       } else {
         float f[8];
         x[j].values(y[j]);
-        o[j].values(f);
+        if (two) o[j].values(f);
         if constexpr (OP == kRowsNorm) {
           if (two) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[j][e] += f[e];
             const int c = column(j, lane, lanes);
-            if (c < row.K) *reinterpret_cast<uint4*>(row.total + c) = pack8<T>(y[j]);
+            if constexpr (ANYWHERE)
+              store_anywhere(row.total, c, row.K, pack8<T>(y[j]));
+            else if (c < row.K)
+              *reinterpret_cast<uint4*>(row.total + c) = pack8<T>(y[j]);
           }
           Raw8<T> w;
-          w.load(row.weight + column(j, lane, lanes), column(j, lane, lanes) < row.K);
+          load(w, row.weight, column(j, lane, lanes), row.K);
           w.values(f);
           Row<T, OP>::combine(y[j], f, sum);
         } else {
@@ -274,17 +350,16 @@ struct Held {
       float v[8];
       if constexpr (OP == kRowsQuantize) {
         raw[j].values(v);
-        writer.write_vec(column(j, lane, lanes), v);
+        writer.write(column(j, lane, lanes), v);
       } else {
-        writer.write_vec(column(j, lane, lanes), y[j]);
+        writer.write(column(j, lane, lanes), y[j]);
       }
     }
   }
 };
 
-// One row a warp (ONE_WARP; eight of them a block) or a block, in whole
-// vectors.
-template <typename T, int OP, bool ONE_WARP, int HELD>
+// One row a warp (ONE_WARP; eight of them a block) or a block.
+template <typename T, int OP, bool ONE_WARP, int HELD, bool ANYWHERE>
 __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_kernel(Int8Rows a) {
   __shared__ float2 part[32];
   pdl_wait();
@@ -293,15 +368,15 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_kernel(Int8Rows a)
   const long long t = ONE_WARP ? (long long)blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x;
   if (ONE_WARP && t >= a.T) return;
   float sum = 0.f, top = 0.f;
-  Held<T, OP, HELD> held;
+  Held<T, OP, HELD, ANYWHERE> held;
   held.read(Row<T, OP>(a, t), lane, lanes, sum, top);
   reduce_warp(OP, sum, top);
   if (!ONE_WARP) reduce_block(OP, sum, top, part);
   held.write(Writer<OP>(a, t, sum, top, lane == 0), lane, lanes);
 }
 
-// Any rows, read twice and element by element, a row a block.  The columns of
-// a thread are those of rows_kernel.
+// Any row, read twice and element by element, a row a block: what is too long
+// for registers, and fp32 that does not start on 16 bytes.
 template <typename T, int OP>
 __global__ void __launch_bounds__(1024) any_rows_kernel(Int8Rows a) {
   __shared__ float2 part[32];
@@ -327,9 +402,14 @@ __global__ void __launch_bounds__(1024) any_rows_kernel(Int8Rows a) {
 }
 
 template <typename T, int OP, bool ONE_WARP, int HELD>
-void launch(const Int8Rows& a, cudaStream_t s) {
-  const int threads = ONE_WARP ? 256 : ((a.K / 8 + HELD - 1) / HELD + 31) / 32 * 32;
-  launch_k(rows_kernel<T, OP, ONE_WARP, HELD>, dim3((unsigned)(ONE_WARP ? (a.T + 7) / 8 : a.T)), dim3(threads), 0, s, a);
+void launch(const Int8Rows& a, bool vec, cudaStream_t s) {
+  const int threads = ONE_WARP ? 256 : ((a.K + 8 * HELD - 1) / (8 * HELD) + 31) / 32 * 32;
+  const dim3 grid((unsigned)(ONE_WARP ? (a.T + 7) / 8 : a.T));
+  if (vec) {
+    launch_k(rows_kernel<T, OP, ONE_WARP, HELD, false>, grid, dim3(threads), 0, s, a);
+  } else if constexpr (!std::is_same<T, float>::value) {
+    launch_k(rows_kernel<T, OP, ONE_WARP, HELD, true>, grid, dim3(threads), 0, s, a);
+  }
 }
 
 bool on16(const void* p, long long stride, int bytes, int rows) {
@@ -342,15 +422,18 @@ void launch_op(const Int8Rows& a, cudaStream_t s) {
   const bool vec = a.K % 8 == 0 && on16(a.x, a.xs, el, a.T) && (!a.other || on16(a.other, a.os, el, a.T)) &&
                    (!a.weight || on16(a.weight, 0, el, 1)) && (!a.total || on16(a.total, a.ts, el, a.T));
   const int n = (a.K + 7) / 8;
-  if (!vec || n > 4096) {
-    const int threads = std::min(1024, ((n + 1) / 2 + 31) / 32 * 32);
+  if (n > 4096 || (!vec && std::is_same<T, float>::value)) {
+    const int threads = std::min(1024, ((n + 3) / 4 + 31) / 32 * 32);
     launch_k(any_rows_kernel<T, OP>, dim3((unsigned)a.T), dim3(threads), 0, s, a);
     return;
   }
-  if (n <= 32) return launch<T, OP, true, 1>(a, s);
-  if (n <= 64) return launch<T, OP, true, 2>(a, s);
-  if (n <= (OP == kRowsNorm ? 1024 : 256)) return launch<T, OP, false, 2>(a, s);
-  return launch<T, OP, false, 4>(a, s);
+  // Vectors a thread: 8192 rows of 5120, us, 1 / 2 / 4: quantise - / 25.6 /
+  // 24.6, norm 52.0 / 46.6 / 46.8, silu 42.7 / 43.7 / 40.8; 2048 rows of 4096:
+  // 6.5 / 5.7 / 5.9, 12.1 / 11.5 / 12.5, 10.0 / 9.8 / 9.7.
+  if (n <= 32) return launch<T, OP, true, 1>(a, vec, s);
+  if (n <= 64) return launch<T, OP, true, 2>(a, vec, s);
+  if (n <= (OP == kRowsNorm ? 1024 : 256)) return launch<T, OP, false, 2>(a, vec, s);
+  return launch<T, OP, false, 4>(a, vec, s);
 }
 
 // The float of byte i of u, whose bytes are integers with their top bit
@@ -385,15 +468,33 @@ __global__ void __launch_bounds__(512) values_kernel(Int8Values a) {
         }
       }
     }
+  } else if constexpr (std::is_same<T, float>::value) {
+    for (int c = at; c < a.K; c += step) out[c] = (float)q[c] * s;
   } else {
-    for (int c = at; c < a.K; c += step) out[c] = from_float<T>((float)q[c] * s);
+    // 8 elements a thread, integers and results on any byte and element; whole warps
+    for (int c = at * 8; c - (int)(threadIdx.x % 32) * 8 < a.K; c += step * 8) {
+      uint2 u = make_uint2(0, 0);
+      if (c + 8 <= a.K && (reinterpret_cast<uintptr_t>(q + c) & 7) == 0) {
+        u = *reinterpret_cast<const uint2*>(q + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < a.K) (e < 4 ? u.x : u.y) |= (uint32_t)(uint8_t)q[c + e] << (8 * (e % 4));
+      }
+      u.x ^= 0x80808080u;
+      u.y ^= 0x80808080u;
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = value(e < 4 ? u.x : u.y, e % 4) * s;
+      store_anywhere(out, c, a.K, pack8<T>(f));
+    }
   }
 }
 
 template <typename T>
 void launch_values(const Int8Values& a, cudaStream_t s) {
   const bool vec = a.K % 16 == 0 && on16(a.out, a.os, sizeof(T), a.T) && on16(a.q, a.qs, 1, a.T);
-  const int items = vec ? a.K / 16 : a.K;
+  const int items = vec ? a.K / 16 : std::is_same<T, float>::value ? a.K : (a.K + 7) / 8;
   const int y = (items + 511) / 512, threads = ((items + y - 1) / y + 31) / 32 * 32;
   const dim3 grid((unsigned)a.T, (unsigned)(y < 64 ? y : 64));
   if (vec)

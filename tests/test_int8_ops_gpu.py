@@ -42,7 +42,8 @@ def check_rows(q, scales, y, roundings, scale_roundings):
 
 
 # widths: one element, below a vector, whole vectors, odd, each variant's largest, read twice
-WIDTHS = [1, 7, 8, 100, 128, 256, 512, 513, 1000, 1024, 2047, 2048, 4096, 5120, 6144, 8192, 13824, 16384, 32768, 32776]
+WIDTHS = [1, 7, 8, 17, 100, 128, 255, 256, 257, 512, 513, 1000, 1024, 2047, 2048, 4096, 5119, 5120, 6144, 8192, 8195, 13824,
+          16384, 32767, 32768, 32776]
 
 
 @pytest.mark.parametrize("k", WIDTHS)
@@ -146,7 +147,7 @@ def test_silu_large_gates():
 
 def test_rows_of_any_stride():
     from kunserve_b200.ops import add_rms_norm_int8, dequantize_int8, quantize_int8, silu_mul_int8
-    for k, wide, at in ((64, 72, 3), (64, 96, 16), (1000, 2048, 8), (37, 41, 1)):
+    for k, wide, at in ((64, 72, 3), (64, 96, 16), (1000, 2048, 8), (37, 41, 1), (2051, 2100, 5)):
         buf = _randn(k, 9, wide).bfloat16()
         x = buf[:, at:at + k]
         w = _randn(1, k).bfloat16()
@@ -154,6 +155,16 @@ def test_rows_of_any_stride():
         for f in (quantize_int8, lambda v: silu_mul_int8(v, v), lambda v: add_rms_norm_int8(v, w, residual=v)):
             for a, b in zip(f(x), f(c)):
                 assert torch.equal(a, b)
+        for shift in range(8):                      # sums around rows that start on any element
+            flat = torch.full((9 * k + 16,), 3.0, device="cuda").bfloat16()
+            out = flat[shift:shift + 9 * k].view(9, k)
+            want = add_rms_norm_int8(x, w, residual=c)
+            got = add_rms_norm_int8(x, w, residual=x, out=out)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            assert (flat[:shift] == 3).all() and (flat[shift + 9 * k:] == 3).all()
+            v = dequantize_int8(*want[:2], out=out)
+            assert torch.equal(v, dequantize_int8(*want[:2]))
+            assert (flat[:shift] == 3).all() and (flat[shift + 9 * k:] == 3).all()
         rep = buf[:1, at:at + k].expand(9, k)       # one row for all tokens
         for a, b in zip(quantize_int8(rep), quantize_int8(rep.clone())):
             assert torch.equal(a, b)
