@@ -25,11 +25,15 @@ KUS_DEVICE float max_nan(float a, float b) {
   return r;
 }
 
-// 1 / (1 + e^-g) to five roundings: one step of each function, one of the
-// sum.  Zero from g < -87 on, where it leaves the normal range.
+// 1 / (1 + e^-g).  Of its roundings that of g log2 e grows with g: e^-g is off
+// by 2 + 1.2 |g| units in the last place, of which the sum takes up the share
+// e^-g / (1 + e^-g), so that silu is off by 5.4 * 2^-24 of the gate at most (the
+// share falls where |g| grows, or else silu itself does).  expf would hold it
+// to 2^-23; a row of 14336 takes 115 us then where this takes 105.  Zero from
+// g < -87 on, where it leaves the normal range.
 KUS_DEVICE float sigmoid(float g) {
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + expf(-g)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
   return r;
 }
 

@@ -5,7 +5,7 @@ import torch
 
 from test_cache_ops_streams_gpu import _behind_queued_work
 from test_int8_ops_gpu import BF, F32, HALF, U, _linear_inputs, _no_device_error, _randn, check_linear, \
-    check_rows  # noqa: F401
+    check_rows, silu_roundings  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -172,7 +172,7 @@ def test_layer(tokens, shape):
             check_rows(args[1], args[2], args[0].double(), 2, 1)
         elif kind == "silu":
             g, u = args[0].double().chunk(2, 1)
-            check_rows(args[1], args[2], g / (1 + torch.exp(-g)) * u, 16, 8)
+            check_rows(args[1], args[2], g / (1 + torch.exp(-g)) * u, *silu_roundings(g))
         else:
             q, s, weight, y = args
             check_linear(y, q, s, unpacked(weight), weight.scales)
