@@ -583,21 +583,24 @@ namespace i8gemm {
 
 // What a cut is expected to take, in us (less what every cut takes).  Of its
 // products, stage by stage: the loads (104 bytes a clock of a CTA alone on its
-// SM, 60 of each of two), 2 clocks a token, at least 290 clocks (145) of
-// latency; of the results 20 ns a token and tile to write; of the bytes that
+// SM, 60 of each of two), 2 clocks a token and a clock for 600 bytes (what they
+// take of the power: of tiles with as many rounds the widest wins under the
+// power limit, 8192 x 14336 x 4096 in tiles of 256 346 us, of 224 361), at least
+// 290 clocks (145) of latency; of the results 20 ns a token and tile to write; of the bytes that
 // HBM moves.  Each hides some of the others: their root of squares.  The last
 // tile is written when nothing is left to hide it, a round takes 0.63 us to
 // fill the stages, and adding up parts of K 2 us.  The numbers were fitted to
 // 863 cuts of 75 products (1 to 12000 tokens, 64 to 28672 channels, K 64 to
 // 16384): times are off by 10 % on average, and the cut that is cheapest by
-// this takes 1.4 % longer than the best, 12 % at most.
+// this takes 1.9 % longer than the best, 13 % at most.
 double cost(const Int8Plan& p, int M, int N, int K, int element, const Int8Slots& slots) {
   const int ctas = p.pair ? 2 : 1, blocks = (int)int8_blocks(K), units = p.token_tiles * p.channel_tiles;
   const int each = (blocks + p.splits - 1) / p.splits;
   // times that one CTA after another runs on an SM; two at once share it
   const int waves = p.splits > 1 ? 1 : (units + slots.clusters[ctas] - 1) / slots.clusters[ctas];
   const int rounds = p.splits > 1 && !p.alone ? 2 : waves;
-  const double stage = std::max({stage_bytes(p) / (p.alone ? 104.0 : 60.0), 2.0 * p.width, p.alone ? 290.0 : 145.0});
+  const double stage = std::max({stage_bytes(p) / (p.alone ? 104.0 : 60.0), 2.0 * p.width + stage_bytes(p) / 600.0,
+                                 p.alone ? 290.0 : 145.0});
   const double write = 0.02 * p.width;
   const double products = rounds * each * stage / 1.9e3, writes = p.splits > 1 ? 0 : rounds * write;
   const double moved = ((double)N * K + (double)M * K + (double)M * N * element) / 7.2e6;
