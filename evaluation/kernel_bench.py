@@ -2,6 +2,7 @@
 
     python evaluation/kernel_bench.py gemm --m 1 16 256 4096 --n 6144 --k 4096
     python evaluation/kernel_bench.py gemm-cublas --m 16 --n 4096 --k 4096
+    python evaluation/kernel_bench.py int8 --m 1 64 306 8192 --n 28672 --k 4096
     python evaluation/kernel_bench.py attention --batch 64 --ctx 1024
     python evaluation/kernel_bench.py decode-step --batch 1 32 128
 
@@ -84,6 +85,44 @@ def bench_gemm(args, cublas=False):
                 print(json.dumps(rec), flush=True)
 
 
+def bench_int8(args):
+    """The 8-bit operators of a projection: the rows' kernels over [m, k] and
+    the product with [n, k] weights."""
+    from kunserve_b200 import ops
+    bw, fl, src = peaks()
+
+    def report(kernel, t, bytes_, flops=0, **sizes):
+        rec = {"kernel": kernel, **sizes, "us": round(t * 1e6, 2), "TB_s": round(bytes_ / t / 1e12, 3),
+               "bw_frac": round(bytes_ / t / bw, 3)}
+        if flops:   # the integer rate is twice the bf16 one
+            rec.update(TOP_s=round(flops / t / 1e12, 1), flop_frac=round(flops / t / (2 * fl), 3))
+        print(json.dumps({**rec, "peaks": src}), flush=True)
+
+    for K in args.k:
+        for M in args.m:
+            nbuf = min(64, max(2, math.ceil(256e6 / (M * K * 2))))
+            xs = [torch.randn(M, 2 * K, device="cuda").bfloat16() for _ in range(nbuf)]
+            w = torch.ones(K, device="cuda").bfloat16()
+            halves = [(x[:, :K], x[:, K:]) for x in xs]
+            qs = [ops.quantize_int8(a) for a, _ in halves]
+            out = torch.empty(M, K, device="cuda", dtype=torch.bfloat16)
+            for name, per, fn in (
+                    ("quantize_int8", 3, lambda i: ops.quantize_int8(halves[i % nbuf][0])),
+                    ("add_rms_norm_int8", 7,
+                     lambda i: ops.add_rms_norm_int8(halves[i % nbuf][0], w, residual=halves[i % nbuf][1], out=out)),
+                    ("silu_mul_int8", 5, lambda i: ops.silu_mul_int8(*halves[i % nbuf])),
+                    ("dequantize_int8", 3, lambda i: ops.dequantize_int8(*qs[i % nbuf], out=out))):
+                report(name, timeit(fn, args.warmup, args.iters), per * M * K, M=M, K=K)
+            del xs, halves
+            for N in args.n:
+                ws = [ops.Int8Weight.quantize(torch.randn(N, K, device="cuda").bfloat16())
+                      for _ in range(min(8, max(2, math.ceil(256e6 / (N * K)))))]
+                y = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
+                t = timeit(lambda i: ops.int8_linear(*qs[i % nbuf], ws[i % len(ws)], out=y), args.warmup, args.iters)
+                report("int8_linear", t, M * K + N * K + 2 * M * N, 2.0 * M * N * K, M=M, N=N, K=K)
+            ops.check_error()
+
+
 def bench_attention(args):
     from kunserve_b200.engine.native_runner import pack_meta, prefill_splits
     from kunserve_b200.engine.step import StepInput
@@ -163,7 +202,7 @@ def bench_copy(args):
 
 def main():
     p = argparse.ArgumentParser()
-    p.add_argument("what", choices=["gemm", "gemm-cublas", "attention", "copy"])
+    p.add_argument("what", choices=["gemm", "gemm-cublas", "int8", "attention", "copy"])
     p.add_argument("--m", type=int, nargs="+", default=[1, 16, 64, 256])
     p.add_argument("--n", type=int, nargs="+", default=[6144, 4096, 28672])
     p.add_argument("--k", type=int, nargs="+", default=[4096])
@@ -190,6 +229,8 @@ def main():
         bench_gemm(a)
     elif a.what == "gemm-cublas":
         bench_gemm(a, cublas=True)
+    elif a.what == "int8":
+        bench_int8(a)
     elif a.what == "attention":
         bench_attention(a)
     else:

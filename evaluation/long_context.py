@@ -4,6 +4,7 @@ decoder of random weights.
     python evaluation/long_context.py shared --requests 64 --prefix 4096 --steps 32
     python evaluation/long_context.py capped --requests 8 --prompt 6000 --cap 1024 --steps 32
     python evaluation/long_context.py shared --check
+    python evaluation/long_context.py capped --int8
 
 ``shared``: requests behind one system prompt.  The prompt's keys are stored
 once; every step appends each request's token with rotary positions scaled
@@ -15,6 +16,9 @@ before the next eviction).  Every step accumulates each cached token's
 attention weight (``weighted_decode_attention``); a request over the cap keeps
 its first and newest tokens and the heaviest of the rest
 (``select_evictions``, ``compact_cache``), and the pages behind are free.
+
+``--int8``: the projections in 8-bit integers (``add_rms_norm_int8``,
+``quantize_int8``, ``int8_linear``).
 
 ``--check`` compares the attention outputs of both ways to store the same
 requests, behind a shared prefix and in whole caches whose cap is never
@@ -40,9 +44,11 @@ SCALING = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_f
 
 
 class Decoder:
-    """Attention layers of random bf16 weights over a paged cache."""
+    """Attention layers of random bf16 weights over a paged cache; ``int8``: their
+    projections in 8-bit integers."""
 
-    def __init__(self, pages: int, layers=4, hidden=1024, nq=16, nkv=4, hd=128, vocab=4096, block=16, seed=0):
+    def __init__(self, pages: int, layers=4, hidden=1024, nq=16, nkv=4, hd=128, vocab=4096, block=16, seed=0,
+                 int8=False):
         g = torch.Generator(device="cuda").manual_seed(seed)
 
         def weight(*shape):
@@ -52,6 +58,9 @@ class Decoder:
         self.embed = weight(vocab, hidden) * math.sqrt(hidden)
         self.w_qkv = [weight((nq + 2 * nkv) * hd, hidden) for _ in range(layers)]
         self.w_o = [weight(hidden, nq * hd) for _ in range(layers)]
+        self.int8, self.norm = int8, torch.ones(hidden, dtype=torch.bfloat16, device="cuda")
+        if int8:
+            self.w_qkv, self.w_o = ([ops.Int8Weight.quantize(w) for w in ws] for ws in (self.w_qkv, self.w_o))
         self.layout = KVLayout(pages, layers, block, nkv, hd, 2)
         self.pool = torch.empty(self.layout.base_bytes // 2, dtype=torch.bfloat16, device="cuda")
         self.kv = ops.PagedKV(self.pool, self.layout)
@@ -67,13 +76,24 @@ class Decoder:
         i32 = [torch.tensor(v, dtype=torch.int32, device="cuda") for v in (positions, pages, slots)]
         h = self.embed[tokens]
         self.attended = []
+        added = None                 # in 8 bits: what the layer before adds to h, with its norm
         for layer in range(self.layers):
-            x = torch.nn.functional.rms_norm(h, h.shape[-1:])
-            qkv = (x @ self.w_qkv[layer].t()).view(len(positions), -1, self.hd)
+            if self.int8:
+                x, residual = (h, None) if added is None else (added, h)
+                q, s, h = ops.add_rms_norm_int8(x, self.norm, torch.finfo(h.dtype).eps, residual=residual)
+                qkv = ops.int8_linear(q, s, self.w_qkv[layer])
+            else:
+                qkv = torch.nn.functional.rms_norm(h, h.shape[-1:]) @ self.w_qkv[layer].t()
+            qkv = qkv.view(len(positions), -1, self.hd)
             ops.rotary_append(qkv, *i32, self.rotary, self.kv, layer, weights=self.weights[layer],
                               slot_positions=self.positions[layer])
             self.attended.append(attend(layer, qkv[:, :self.nq]).flatten(1))
-            h = h + self.attended[-1] @ self.w_o[layer].t()
+            if self.int8:
+                added = ops.int8_linear(*ops.quantize_int8(self.attended[-1]), self.w_o[layer])
+            else:
+                h = h + self.attended[-1] @ self.w_o[layer].t()
+        if added is not None:
+            h = h + added
         return torch.nn.functional.rms_norm(h, h.shape[-1:]) @ self.embed.t()
 
 
@@ -216,6 +236,7 @@ def main():
     ap.add_argument("--cap", type=int, default=1024)
     ap.add_argument("--slack", type=int, default=16)
     ap.add_argument("--steps", type=int, default=32)
+    ap.add_argument("--int8", action="store_true", help="projections in 8-bit integers")
     ap.add_argument("--check", action="store_true")
     args = ap.parse_args()
     if args.check:
@@ -224,10 +245,10 @@ def main():
         return 0 if max(diffs) < CHECK_BOUND else 1
     block = 16
     tokens = args.prefix + args.requests * (args.prompt + args.steps + block)
-    model = Decoder(-(-tokens // block) + args.requests + 1)
+    model = Decoder(-(-tokens // block) + args.requests + 1, int8=args.int8)
     pool = Pages(model.kv.pages_total, block)
     prompts = random_prompts(args.requests, max(1, args.prompt // 2), args.prompt, 4096, 1)
-    rec = {"mode": args.mode, "requests": args.requests, "steps": args.steps}
+    rec = {"mode": args.mode, "requests": args.requests, "steps": args.steps, "int8": args.int8}
     if args.mode == "shared":
         _, _, s = decode_shared(model, pool, random_prompts(1, args.prefix, args.prefix, 4096, 2)[0], prompts,
                                 args.steps)
