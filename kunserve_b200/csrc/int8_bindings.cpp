@@ -331,7 +331,7 @@ void bind_int8_ops(py::module& m) {
     for (int c = 0; c < 9; ++c) s.clusters[c] = slots.at(c);
     const Int8Plan p = int8_plan(M, N, K, element, s);
     return std::map<std::string, int>{{"pair", p.pair},     {"width", p.width}, {"token_tiles", p.token_tiles},
-                                      {"channel_tiles", p.channel_tiles},       {"splits", p.splits}, {"alone", p.alone},
+                                      {"channel_tiles", p.channel_tiles},       {"splits", p.splits}, {"alone", p.alone}, {"apart", p.apart},
                                       {"group", p.group},   {"grid", p.grid},   {"stages", p.stages},
                                       {"tmem_columns", p.tmem_columns}};
   });

@@ -35,8 +35,15 @@ KUS_HOST_DEVICE constexpr int out_bytes(int element) { return 4 * kChunk * token
 
 KUS_HOST_DEVICE int x_rows(const Int8Plan& p) { return p.pair ? p.width / 2 : p.width; }   // tokens a CTA loads
 KUS_HOST_DEVICE int stage_bytes(const Int8Plan& p) { return kWBytes + x_rows(p) * kBK; }
+// Beside the stages: of whole units the results' buffers and two tiles' token
+// scales, of split ones the parts of the sums that this CTA adds up (or over
+// the stages).
+KUS_HOST_DEVICE int side_bytes(const Int8Plan& p, int element) {
+  if (p.splits == 1) return out_bytes(element) + 2 * p.width * 4;
+  return p.apart ? (p.width + p.splits - 1) / p.splits * p.splits * kInt8Block * 4 : 0;
+}
 int smem_bytes(const Int8Plan& p, int element) {
-  return p.stages * stage_bytes(p) + out_bytes(element) + 2 * p.width * 4 + kBarriers * 8 + 16 + 1024;
+  return p.stages * stage_bytes(p) + side_bytes(p, element) + kBarriers * 8 + 16 + 1024;
 }
 
 // D(tmem, s32) (+)= A(smem, s8) * B(smem, s8)^T; of a pair: A rows 128 and
@@ -89,13 +96,12 @@ KUS_DEVICE void tmem_ld16(uint32_t taddr, int (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-KUS_DEVICE int4 ld_cluster(uint32_t addr) {
-  int4 v;
-  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
+// The halves of cluster_sync.
+KUS_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+KUS_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+KUS_DEVICE void st_cluster(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 template <typename O>
@@ -219,9 +225,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stages = p.stages, stage_size = stage_bytes(p);
-  uint8_t* staged = smem + stages * stage_size;
+  uint8_t* side = smem + stages * stage_size;
+  uint8_t* staged = side;
   float* scales = reinterpret_cast<float*>(staged + out_bytes(sizeof(O)));
-  uint64_t* full = reinterpret_cast<uint64_t*>(scales + 2 * p.width);
+  uint64_t* full = reinterpret_cast<uint64_t*>(side + side_bytes(p, sizeof(O)));
   uint64_t* empty = full + kMostStages;
   uint64_t* tfull = empty + kMostStages;
   uint64_t* tempty = tfull + 2;
@@ -242,6 +249,21 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int first = (int)blockIdx.x / (SPLIT ? kCtas * p.splits : kCtas);
   const int step = SPLIT ? units : (int)gridDim.x / kCtas;
 
+  const uint32_t lead_full = PAIR ? mapa_shared(smem_u32(full), lead) : 0u;
+  auto load_w = [&](int st, const Unit& at, int kb) {
+    uint8_t* to = smem + st * stage_size;
+    const int row = ((at.n * kCtas + half) * blocks + kb) * kInt8Block;
+    if (leads) mbar_arrive_expect_tx(&full[st], (uint32_t)stage_size * kCtas);    // both CTAs' bytes
+    if (PAIR)
+      tma_load_2d_pair(to, &tmW, lead_full + 8u * st, 0, row);
+    else
+      tma_load_2d(to, &tmW, &full[st], 0, row);
+  };
+  // The first stages' weights are on their way while this kernel sets up and
+  // the one before ends: none but pack_kernel writes weights, and nothing
+  // starts before that one has ended.
+  const Unit start = unit_at(p, first);
+  const int early = first < units ? min(stages, kb1 - kb0) : 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
@@ -253,11 +275,19 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     mbar_init(drained, 1);
     fence_barrier_init();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the copies find the barriers ready
+    if (!PAIR)
+      for (int j = 0; j < early; ++j) load_w(j, start, kb0 + j);
   }
   if (warp == 1) PAIR ? tmem_alloc_pair(tmem_holder, p.tmem_columns) : tmem_alloc(tmem_holder, p.tmem_columns);
   tc_fence_before();
   __syncthreads();
-  if (PAIR) cluster_sync();    // both CTAs' barriers are ready before the other arrives on them
+  // A pair's barriers are ready before the other CTA arrives on them; the
+  // other CTAs of a split only have to run before they are given their parts.
+  if (PAIR)
+    cluster_sync();
+  else if (SPLIT)
+    cluster_arrive();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
 
@@ -266,21 +296,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     pdl_trigger();
   }
 
+  bool summed = false;      // SPLIT: this warp's part of the sums is in TMEM
   if (warp == 0) {
     if (elect_one_sync()) {
-      prefetch_tmap(&tmW);
-      prefetch_tmap(&tmX);
-      const uint32_t bytes = (uint32_t)stage_size * kCtas;    // both CTAs' count on the leader's barrier
-      const uint32_t lead_full = PAIR ? mapa_shared(smem_u32(full), lead) : 0u;
-      auto load_w = [&](int st, const Unit& at, int kb) {
-        uint8_t* to = smem + st * stage_size;
-        const int row = ((at.n * kCtas + half) * blocks + kb) * kInt8Block;
-        if (leads) mbar_arrive_expect_tx(&full[st], bytes);
-        if (PAIR)
-          tma_load_2d_pair(to, &tmW, lead_full + 8u * st, 0, row);
-        else
-          tma_load_2d(to, &tmW, &full[st], 0, row);
-      };
       auto load_x = [&](int st, const Unit& at, int kb) {
         uint8_t* to = smem + st * stage_size + kWBytes;
         const int row = at.t * p.width + half * x_rows(p);
@@ -289,12 +307,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         else
           tma_load_2d(to, &tmX, &full[st], kb * kBK, row);
       };
-      // the first stages' weights are on their way while the kernel before
-      // ends: none but pack_kernel writes weights, and nothing starts before
-      // that one has ended
-      const Unit start = unit_at(p, first);
-      const int early = first < units ? min(stages, kb1 - kb0) : 0;
-      for (int j = 0; j < early; ++j) load_w(j, start, kb0 + j);
+      prefetch_tmap(&tmX);
+      if (PAIR)
+        for (int j = 0; j < early; ++j) load_w(j, start, kb0 + j);
       pdl_wait();
       pdl_trigger();
       for (int j = 0; j < early; ++j) load_x(j, start, kb0 + j);
@@ -408,16 +423,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         tc_fence_before();
         named_barrier(3 + group, 128);
         if (gt == 0) PAIR ? mbar_arrive_remote(lead_tempty + 8u * acc) : mbar_arrive(&tempty[acc]);
-      } else if (ok) {
-        // this CTA's part of the sums, over the stages: all of them are used up
-        int* sums = reinterpret_cast<int*>(smem);
-#pragma unroll 1
-        for (int c = group * kChunk; c < tokens; c += 2 * kChunk) {
-          int v[16];
-          tmem_ld16(taddr + c, v);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sums[(c + i) * kInt8Block + row] = v[i];
-        }
+      } else {
+        summed = ok;
       }
       if (++acc == 2) {
         acc = 0;
@@ -425,56 +432,79 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
   }
-  tc_fence_before();
-  __syncthreads();
-  if (PAIR || SPLIT) cluster_sync();     // the cluster's sums are written; a pair is done with both TMEMs and barriers
-  if (warp == 1) PAIR ? tmem_dealloc_pair(tmem_base, p.tmem_columns) : tmem_dealloc(tmem_base, p.tmem_columns);
-  if (SPLIT) {
-    // the CTAs that hold parts of the same sums share the tile's tokens: each
-    // adds up all parts of its own (integers: any order gives the same)
-    const Unit at = unit_at(p, first);
-    const int t0 = at.t * p.width, tokens = min(p.width, a.M - t0);
-    const int share = (tokens + p.splits - 1) / p.splits;
-    const int n = (at.n * kCtas + half) * kInt8Block + lane * 4;
-    const uint32_t sums = smem_u32(smem);
-    const Results<O> results(a);
-    const O* bias = reinterpret_cast<const O*>(a.bias);
-    float ws[4], b[4];
+  if (!SPLIT) {
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync();      // the pair is done with both TMEMs and barriers
+    if (warp == 1) PAIR ? tmem_dealloc_pair(tmem_base, p.tmem_columns) : tmem_dealloc(tmem_base, p.tmem_columns);
+    return;
+  }
+
+  // The CTAs that hold parts of the same sums share the tile's tokens: each
+  // gives the others their tokens' parts, [part][token][128] in the owner's
+  // memory, and adds up all parts of its own (integers: any order gives the
+  // same).  Over the stages where there is no room beside them, once every CTA
+  // has used them up.
+  const int t0 = start.t * p.width, tokens = min(p.width, a.M - t0);
+  const int share = (tokens + p.splits - 1) / p.splits, mine = part * share;
+  const int n = (start.n * kCtas + half) * kInt8Block + lane * 4;
+  const Results<O> results(a);
+  float ws[4], b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ws[i] = n + i < a.N ? a.w_scales[n + i] : 0.f;
-      b[i] = bias && n + i < a.N ? float_of<O>(bias[n + i]) : 0.f;
-    }
-    for (int c = part * share + warp; c < min(tokens, (part + 1) * share); c += kThreads / 32) {
-      const float xs = a.x_scales[t0 + c];
-      const uint32_t at_c = sums + (uint32_t)(c * kInt8Block + lane * 4) * 4;
-      int s[4] = {0, 0, 0, 0};
+  for (int i = 0; i < 4; ++i) {
+    ws[i] = n + i < a.N ? a.w_scales[n + i] : 0.f;
+    b[i] = a.bias && n + i < a.N ? float_of<O>(reinterpret_cast<const O*>(a.bias)[n + i]) : 0.f;
+  }
+  const int most = (p.width + p.splits - 1) / p.splits;
+  uint8_t* parts = p.apart ? side : smem;
+  if (!PAIR) cluster_wait();
+  if (!p.apart) cluster_sync();
+  if (summed) {
+    const int quarter = warp & 3;
+    const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t to = smem_u32(parts) + (uint32_t)((part * most * kInt8Block + quarter * 32 + lane) * 4);
+#pragma unroll 1
+    for (int c = (warp - 2) / 4 * 16; c < tokens; c += 32) {
+      int v[16];
+      tmem_ld16(taddr + c, v);
+      int owner = c / share, at = c - owner * share;
 #pragma unroll
-      for (int r = 0; r < 8 / kCtas; ++r) {
-        if (r < p.splits) {
-          const int4 v = ld_cluster(mapa_shared(at_c, r * kCtas + half));
-          s[0] += v.x;
-          s[1] += v.y;
-          s[2] += v.z;
-          s[3] += v.w;
+      for (int i = 0; i < 16; ++i) {
+        if (c + i < tokens) st_cluster(mapa_shared(to + at * (kInt8Block * 4), owner * kCtas + half), v[i]);
+        if (++at == share) {
+          at = 0;
+          ++owner;
         }
       }
-      O* dst = results.out + (t0 + c) * results.ldc + n;
-      alignas(16) O y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = out_of<O>(fmaf((float)s[i] * xs, ws[i], b[i]));
-      if (results.aligned && n + 4 <= a.N) {
-        if constexpr (sizeof(O) == 2)
-          *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
-        else
-          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n + i < a.N) dst[i] = y[i];
-      }
     }
-    cluster_sync();    // no CTA ends while others read its part
+  }
+  tc_fence_before();
+  cluster_sync();      // all parts are where they belong; a pair is done with both TMEMs
+  if (warp == 1) PAIR ? tmem_dealloc_pair(tmem_base, p.tmem_columns) : tmem_dealloc(tmem_base, p.tmem_columns);
+  for (int c = warp; c < min(share, tokens - mine); c += kThreads / 32) {
+    const float xs = a.x_scales[t0 + mine + c];
+    int s[4] = {0, 0, 0, 0};
+    for (int r = 0; r < p.splits; ++r) {
+      const int4 v = *reinterpret_cast<const int4*>(parts + ((r * most + c) * kInt8Block + lane * 4) * 4);
+      s[0] += v.x;
+      s[1] += v.y;
+      s[2] += v.z;
+      s[3] += v.w;
+    }
+    O* dst = results.out + (t0 + mine + c) * results.ldc + n;
+    alignas(16) O y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = out_of<O>(fmaf((float)s[i] * xs, ws[i], b[i]));
+    if (results.aligned && n + 4 <= a.N) {
+      if constexpr (sizeof(O) == 2)
+        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+      else
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < a.N) dst[i] = y[i];
+    }
   }
 }
 
@@ -661,6 +691,7 @@ Int8Plan int8_plan(int M, int N, int K, int element, const Int8Slots& slots) {
   p.grid = ctas * (p.splits > 1 ? units * p.splits : std::min(units, most));
   p.tmem_columns = 32;
   while (p.tmem_columns < 2 * p.width) p.tmem_columns *= 2;
+  p.apart = p.splits > 1 && p.width <= (p.alone ? 64 : 32);
   p.stages = kMostStages;
   while (smem_bytes(p, element) > (p.alone ? kSmemAlone : kSmemHalf)) --p.stages;
   // the tokens of a group: at most 32 MB

@@ -65,6 +65,7 @@ struct Int8Plan {
   int token_tiles, channel_tiles;
   int splits;                // CTAs (pairs) of a cluster that share a tile's K
   int alone;                 // one CTA an SM; else two
+  int apart;                 // the parts of a split lie beside the stages, else over them
   int group;                 // token tiles walked before the next channel tile
   int grid;                  // CTAs
   int stages, tmem_columns;

@@ -41,12 +41,18 @@ def test_every_tile_once(seed, slots):
             assert p["grid"] == ctas * units * p["splits"]
         else:
             assert 0 < p["grid"] <= ctas * units
-        # shared memory: stages, two buffers for each epilogue group, scales, barriers; the parts of a split lie over
-        # the stages.  TMEM: two accumulators, of each of two CTAs an SM
+        # shared memory: stages and barriers; of whole units two buffers for each epilogue group and two tiles' scales,
+        # of split ones the parts of a share of the tokens, beside the stages or over them.  TMEM: two accumulators, of
+        # each of two CTAs an SM
         stage = 128 * 128 + p["width"] // ctas * 128
-        staged = 4 * 16 * (128 * element + (16 if element == 2 else 0))
-        assert 2 <= p["stages"] <= 8 and p["width"] * 512 <= p["stages"] * stage or p["splits"] == 1
-        assert p["stages"] * stage + staged + 8 * p["width"] + 21 * 8 + 16 + 1024 <= SHARED[bool(p["alone"])]
+        parts = -(-p["width"] // p["splits"]) * p["splits"] * 512
+        assert 2 <= p["stages"] <= 8 and (p["splits"] > 1 or not p["apart"])
+        if p["splits"] == 1:
+            side = 4 * 16 * (128 * element + (16 if element == 2 else 0)) + 8 * p["width"]
+        else:
+            side = parts if p["apart"] else 0
+            assert p["apart"] or parts <= p["stages"] * stage
+        assert p["stages"] * stage + side + 21 * 8 + 16 + 1024 <= SHARED[bool(p["alone"])]
         assert 2 * p["width"] <= p["tmem_columns"] <= (512 if p["alone"] else 256)
         if units < 20000:
             seen = set(_units(p))
