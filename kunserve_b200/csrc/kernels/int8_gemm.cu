@@ -296,7 +296,23 @@ __global__ void __launch_bounds__(kThreads, 2)
     pdl_trigger();
   }
 
-  bool summed = false;      // SPLIT: this warp's part of the sums is in TMEM
+  // SPLIT: this CTA's share of the unit's tokens, and what an epilogue warp
+  // multiplies their sums with, loaded while they are computed
+  bool summed = false;      // this warp's part of the sums is in TMEM
+  const int t0_split = start.t * p.width, tokens_split = min(p.width, a.M - t0_split);
+  const int share = (tokens_split + p.splits - 1) / p.splits, mine = t0_split + part * share;
+  const int shared_tokens = min(share, tokens_split - part * share);
+  const int n_split = (start.n * kCtas + half) * kInt8Block + lane * 4;
+  float ws_split[4] = {0.f, 0.f, 0.f, 0.f}, b_split[4] = {0.f, 0.f, 0.f, 0.f}, xs_split = 0.f;
+  if (SPLIT && warp >= 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n_split + i >= a.N) continue;
+      ws_split[i] = a.w_scales[n_split + i];
+      if (a.bias) b_split[i] = float_of<O>(reinterpret_cast<const O*>(a.bias)[n_split + i]);
+    }
+    if (warp - 2 < shared_tokens) xs_split = a.x_scales[mine + warp - 2];
+  }
   if (warp == 0) {
     if (elect_one_sync()) {
       auto load_x = [&](int st, const Unit& at, int kb) {
@@ -445,16 +461,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   // memory, and adds up all parts of its own (integers: any order gives the
   // same).  Over the stages where there is no room beside them, once every CTA
   // has used them up.
-  const int t0 = start.t * p.width, tokens = min(p.width, a.M - t0);
-  const int share = (tokens + p.splits - 1) / p.splits, mine = part * share;
-  const int n = (start.n * kCtas + half) * kInt8Block + lane * 4;
   const Results<O> results(a);
-  float ws[4], b[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    ws[i] = n + i < a.N ? a.w_scales[n + i] : 0.f;
-    b[i] = a.bias && n + i < a.N ? float_of<O>(reinterpret_cast<const O*>(a.bias)[n + i]) : 0.f;
-  }
   const int most = (p.width + p.splits - 1) / p.splits;
   uint8_t* parts = p.apart ? side : smem;
   if (!PAIR) cluster_wait();
@@ -464,13 +471,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t to = smem_u32(parts) + (uint32_t)((part * most * kInt8Block + quarter * 32 + lane) * 4);
 #pragma unroll 1
-    for (int c = (warp - 2) / 4 * 16; c < tokens; c += 32) {
+    for (int c = (warp - 2) / 4 * 16; c < tokens_split; c += 32) {
       int v[16];
       tmem_ld16(taddr + c, v);
       int owner = c / share, at = c - owner * share;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        if (c + i < tokens) st_cluster(mapa_shared(to + at * (kInt8Block * 4), owner * kCtas + half), v[i]);
+        if (c + i < tokens_split) st_cluster(mapa_shared(to + at * (kInt8Block * 4), owner * kCtas + half), v[i]);
         if (++at == share) {
           at = 0;
           ++owner;
@@ -481,8 +488,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_before();
   cluster_sync();      // all parts are where they belong; a pair is done with both TMEMs
   if (warp == 1) PAIR ? tmem_dealloc_pair(tmem_base, p.tmem_columns) : tmem_dealloc(tmem_base, p.tmem_columns);
-  for (int c = warp; c < min(share, tokens - mine); c += kThreads / 32) {
-    const float xs = a.x_scales[t0 + mine + c];
+  if (warp < 2) return;
+  for (int c = warp - 2; c < shared_tokens; c += 8) {
+    const float xs = c < 8 ? xs_split : a.x_scales[mine + c];
     int s[4] = {0, 0, 0, 0};
     for (int r = 0; r < p.splits; ++r) {
       const int4 v = *reinterpret_cast<const int4*>(parts + ((r * most + c) * kInt8Block + lane * 4) * 4);
@@ -491,11 +499,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       s[2] += v.z;
       s[3] += v.w;
     }
-    O* dst = results.out + (t0 + mine + c) * results.ldc + n;
+    O* dst = results.out + (mine + c) * results.ldc + n_split;
     alignas(16) O y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = out_of<O>(fmaf((float)s[i] * xs, ws[i], b[i]));
-    if (results.aligned && n + 4 <= a.N) {
+    for (int i = 0; i < 4; ++i) y[i] = out_of<O>(fmaf((float)s[i] * xs, ws_split[i], b_split[i]));
+    if (results.aligned && n_split + 4 <= a.N) {
       if constexpr (sizeof(O) == 2)
         *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
       else
@@ -503,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (n + i < a.N) dst[i] = y[i];
+        if (n_split + i < a.N) dst[i] = y[i];
     }
   }
 }
@@ -694,6 +702,10 @@ Int8Plan int8_plan(int M, int N, int K, int element, const Int8Slots& slots) {
   p.apart = p.splits > 1 && p.width <= (p.alone ? 64 : 32);
   p.stages = kMostStages;
   while (smem_bytes(p, element) > (p.alone ? kSmemAlone : kSmemHalf)) --p.stages;
+  // what a CTA fills once needs no more room than that: more of the next
+  // kernel fits beside it
+  if (p.splits > 1 ? p.apart : units <= most)
+    p.stages = std::min(p.stages, std::max(2, (blocks + p.splits - 1) / p.splits));
   // the tokens of a group: at most 32 MB
   p.group = (int)std::max(1ll, std::min<long long>(p.token_tiles, (32ll << 20) / ((long long)p.width * K)));
   return p;
