@@ -620,37 +620,38 @@ Int8Slots int8_slots() {
 namespace i8gemm {
 
 // What a cut is expected to take, in us (less what every cut takes).  Of its
-// products, stage by stage: the loads (104 bytes a clock of a CTA alone on its
-// SM, 60 of each of two), 2 clocks a token and a clock for 600 bytes (what they
+// products, stage by stage: the loads (92 bytes a clock of a CTA alone on its
+// SM, 52 of each of two), 2 clocks a token and a clock for 600 bytes (what they
 // take of the power: of tiles with as many rounds the widest wins under the
-// power limit, 8192 x 14336 x 4096 in tiles of 256 346 us, of 224 361), at least
-// 290 clocks (145) of latency; of the results 20 ns a token and tile to write; of the bytes that
-// HBM moves.  Each hides some of the others: their root of squares.  The last
-// tile is written when nothing is left to hide it, a round takes 0.63 us to
-// fill the stages, and adding up parts of K 2 us.  The numbers were fitted to
-// 863 cuts of 75 products (1 to 12000 tokens, 64 to 28672 channels, K 64 to
-// 16384): times are off by 10 % on average, and the cut that is cheapest by
-// this takes 1.9 % longer than the best, 13 % at most.
+// power limit, 8192 x 14336 x 4096 in tiles of 256 346 us, of 224 361), at
+// least 300 clocks (150) of latency; of the results 17 ns a token and tile to
+// write; of the bytes that HBM moves.  Each hides some of the others: their
+// root of squares.  The last tile is written when nothing is left to hide it, a
+// round takes 0.67 us to fill the stages, adding up parts of K 0.7 us and 14 ns
+// a token.  The numbers were fitted to 1251 cuts of 95 products (1 to 12000
+// tokens, 64 to 45000 channels, K 64 to 16384) queued one behind the other:
+// times are off by 14 % on average, and the cut that is cheapest by this takes
+// 2.7 % longer than the best (up to a quarter for a few products of 4 to 6 us).
 double cost(const Int8Plan& p, int M, int N, int K, int element, const Int8Slots& slots) {
   const int ctas = p.pair ? 2 : 1, blocks = (int)int8_blocks(K), units = p.token_tiles * p.channel_tiles;
   const int each = (blocks + p.splits - 1) / p.splits;
   // times that one CTA after another runs on an SM; two at once share it
   const int waves = p.splits > 1 ? 1 : (units + slots.clusters[ctas] - 1) / slots.clusters[ctas];
   const int rounds = p.splits > 1 && !p.alone ? 2 : waves;
-  const double stage = std::max({stage_bytes(p) / (p.alone ? 104.0 : 60.0), 2.0 * p.width + stage_bytes(p) / 600.0,
-                                 p.alone ? 290.0 : 145.0});
-  const double write = 0.02 * p.width;
+  const double stage = std::max({stage_bytes(p) / (p.alone ? 92.0 : 52.0), 2.0 * p.width + stage_bytes(p) / 600.0,
+                                 p.alone ? 300.0 : 150.0});
+  const double write = 0.017 * p.width;
   const double products = rounds * each * stage / 1.9e3, writes = p.splits > 1 ? 0 : rounds * write;
-  const double moved = ((double)N * K + (double)M * K + (double)M * N * element) / 7.2e6;
+  const double moved = ((double)N * K + (double)M * K + (double)M * N * element) / 8.5e6;
   double t = std::sqrt(products * products + writes * writes + moved * moved) + write;
-  t += 0.63 * (p.alone ? waves : (waves + 1) / 2);
-  if (p.splits > 1) t += 2.0 + 0.005 * p.width * (p.splits - 1) / p.splits;
+  t += 0.67 * (p.alone ? waves : (waves + 1) / 2);
+  if (p.splits > 1) t += 0.73 + 0.014 * p.width * (p.splits - 1) / p.splits;
   return t;
 }
 
 }  // namespace i8gemm
 
-// The cheapest of: single CTAs (up to 200 tokens; from there pairs, which load
+// The cheapest of: single CTAs (up to 400 tokens; from there pairs, which load
 // half the tokens each, took less in every case) or pairs, tiles of 16 to 256
 // tokens, K whole or split over a cluster's CTAs, one CTA an SM or two.
 // Clusters of a split all run at once: a second wave would double the time
@@ -662,7 +663,7 @@ Int8Plan int8_plan(int M, int N, int K, int element, const Int8Slots& slots) {
   const int blocks = (int)int8_blocks(K);
   Int8Plan best{};
   double least = 0;
-  for (int pair = M > 200; pair < 2; ++pair) {
+  for (int pair = M > 400; pair < 2; ++pair) {
     const int ctas = pair ? 2 : 1, step = 16 * ctas;
     int last = 0;
     for (int tile = step; tile <= 256; tile += tile < 32 ? 16 : 32) {
