@@ -1,11 +1,30 @@
 // Matrix product of 8-bit tokens with 8-bit weights on tcgen05 (kind::i8):
 //   y[t, n] = (sum_k q[t, k] w[n, k]) s[t] v[n] + b[n]
-// with exact int32 sums in TMEM.
+// with exact int32 sums in TMEM, scaled in fp32 and rounded once.
 //
-// The weights are the MMA's M side (128 channels a tile) whatever the number
-// of tokens, the tokens its N side (a tile of 16 to 256): a decode step pads
-// its few tokens to 16 and no further.  A k-block is 128 bytes of K, 32 a
-// product.
+// The weights are the MMA's M side whatever the number of tokens, the tokens
+// its N side (a tile of 16 to 256): a decode step pads its few tokens to 16
+// and no further.  A k-block is 128 bytes of K, 32 a product.  The weights
+// lie in blocks of 128 channels x 128 bytes, so that a stage is one
+// contiguous read of 16 KB.
+//
+// What bounds it.  Few tokens: the weights' bytes; 64 x 5120 x 27648 takes
+// 24.4 us of the 22.2 that its bytes take at the copy bandwidth.  K is then
+// split over the CTAs of a cluster until they fill the GPU, and their parts
+// go through distributed shared memory: integers add up in any order, so no
+// workspace, counter or second kernel is needed (64 x 5120 x 5120: 7.9 us in
+// three parts, 14 whole).  Many tokens: the tensor cores, and for them what an
+// SM can load: a tile of 128 x 256 needs 96 bytes a clock at the int8 rate,
+// one of 256 x 256 on a pair of CTAs (cta_group::2), each loading half of
+// either side, 64.  8192 x 4096 x 28672: 856 us in single CTAs, 564 in pairs
+// with the pipe active for 94 % of the cycles, at 1.5 GHz under the power
+// limit (3.4 PFLOP/s; 645 us, 3.0, when it runs on).
+//
+// Results: one warp a scheduler could not scale, convert and store a tile
+// while the next one was multiplied (10 us against 9).  Two groups of four
+// warps take every other 16 tokens, read TMEM as MMA fragments, and stmatrix
+// turns channels into rows of 16 bytes; with direct 2-byte stores 8192 x 4096
+// x 28672 took 806 us, through shared memory by 2-byte stores 684.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -714,7 +733,9 @@ Int8Plan int8_plan(int M, int N, int K, int element, const Int8Slots& slots) {
 
 bool int8_weight_map(CUtensorMap* map, const int8_t* packed, int N, int K) {
   const long long rows = int8_blocks(N) * int8_blocks(K) * kInt8Block;
-  return rows < (1ll << 31) && i8gemm::byte_map(map, packed, rows, kInt8Block, kInt8Block, kInt8Block);
+  // (an odd pair asks for the block behind the last: zeros)
+  return rows + int8_blocks(K) * kInt8Block < (1ll << 31) &&
+         i8gemm::byte_map(map, packed, rows, kInt8Block, kInt8Block, kInt8Block);
 }
 
 bool int8_token_map(CUtensorMap* map, const int8_t* x, long long stride, int M, int K, const Int8Plan& p) {
