@@ -87,23 +87,39 @@ torch::Tensor empty_rows8(int64_t rows, int64_t columns, const torch::Device& de
   return wide == columns ? t : t.narrow(1, 0, columns);
 }
 
-// Such rows and their scales, behind them in one block of memory: a second
-// allocation takes as long as a small call has.
-std::tuple<torch::Tensor, torch::Tensor> empty_quantized(int64_t rows, int64_t columns, const torch::Device& device) {
-  const int64_t wide = (columns + 15) / 16 * 16;
-  const torch::Tensor block = empty({rows * wide + 4 * rows}, torch::kInt8, device);
-  auto view = [&](torch::ScalarType type, at::IntArrayRef sizes, at::IntArrayRef strides, int64_t offset) {
+// Such rows and their scales, behind them in one block of memory, and behind
+// those a tensor of the rows' sizes where `total` asks for one and it is small
+// (64 KB: it may outlive the integers, whose memory it then keeps).  An
+// allocation takes a tenth of a small call.
+constexpr int64_t kSmallTotal = 64 << 10;
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> empty_quantized(const torch::Tensor& like, bool total) {
+  const int64_t rows = like.size(0), columns = like.size(1), wide = (columns + 15) / 16 * 16;
+  const int64_t scales_at = rows * wide, total_at = (scales_at + 4 * rows + 15) / 16 * 16;
+  const int64_t total_bytes = rows * columns * like.element_size();
+  const bool together = total && total_bytes <= kSmallTotal;
+  const torch::Tensor block = empty({together ? total_at + total_bytes : total_at}, torch::kInt8, like.device());
+  auto view = [&](torch::ScalarType type, at::IntArrayRef sizes, at::IntArrayRef strides, int64_t at_byte) {
     torch::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(block.storage()),
                                                                c10::DispatchKeySet(c10::DispatchKey::CUDA),
                                                                c10::scalarTypeToTypeMeta(type));
-    t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides, offset);
+    t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides, at_byte / (int64_t)c10::elementSize(type));
     return t;
   };
-  return {view(torch::kInt8, {rows, columns}, {wide, 1}, 0), view(torch::kFloat32, {rows}, {1}, rows * wide / 4)};
+  torch::Tensor sum;
+  if (total)
+    sum = together ? view(like.scalar_type(), {rows, columns}, {columns, 1}, total_at)
+                   : empty(like.sizes(), like.scalar_type(), like.device());
+  return {view(torch::kInt8, {rows, columns}, {wide, 1}, 0), view(torch::kFloat32, {rows}, {1}, scales_at), sum};
 }
 
-std::tuple<torch::Tensor, torch::Tensor> run_rows(Int8Rows a, const torch::Tensor& x) {
-  auto [q, scales] = empty_quantized(x.size(0), x.size(1), x.device());
+// `total`: where the sum goes; asked for one (a.other) and given none, it is made.
+std::tuple<torch::Tensor, torch::Tensor> run_rows(Int8Rows a, const torch::Tensor& x, torch::Tensor* total = nullptr) {
+  auto [q, scales, sum] = empty_quantized(x, total && !total->defined());
+  if (total) {
+    if (!total->defined()) *total = sum;
+    a.total = total->data_ptr();
+    a.ts = total->stride(0);
+  }
   a.x = x.data_ptr();
   a.xs = x.stride(0);
   a.q = q.data_ptr<int8_t>();
@@ -141,25 +157,26 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> add_rms_norm_int8_op(con
   c10::cuda::CUDAGuard guard(x.device());
   a.weight = weight.data_ptr();
   a.eps = (float)eps;
-  torch::Tensor total = x;
-  if (residual.has_value()) {
-    check_like(*residual, x, "residual");
-    no_gradient(*residual, "residual");
-    total = out.has_value() ? *out : empty(x.sizes(), x.scalar_type(), x.device());
+  if (!residual.has_value()) {
+    KUS_CHECK(!out.has_value(), "out takes the sum of x and residual: without a residual there is none");
+    auto [q, scales] = run_rows(a, x);
+    return {q, scales, x};
+  }
+  check_like(*residual, x, "residual");
+  no_gradient(*residual, "residual");
+  a.other = residual->data_ptr();
+  a.os = residual->stride(0);
+  torch::Tensor total;
+  if (out.has_value()) {
+    total = *out;
     check_like(total, x, "out");
     no_gradient(total, "out");
     check_written(total, "out");
     check_in_place(total, x, "x");
     check_in_place(total, *residual, "residual");
     KUS_CHECK(apart(total, weight), "out overlaps weight");
-    a.other = residual->data_ptr();
-    a.os = residual->stride(0);
-    a.total = total.data_ptr();
-    a.ts = total.stride(0);
-  } else {
-    KUS_CHECK(!out.has_value(), "out takes the sum of x and residual: without a residual there is none");
   }
-  auto [q, scales] = run_rows(a, x);
+  auto [q, scales] = run_rows(a, x, &total);
   return {q, scales, total};
 }
 

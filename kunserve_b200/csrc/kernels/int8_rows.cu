@@ -453,7 +453,20 @@ void launch_op(const Int8Rows& a, cudaStream_t s) {
 // quarter of the rate.)
 KUS_DEVICE float value(uint32_t u, int i) { return __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + i)) - 8388736.f; }
 
-// A row a block; VEC: 16 elements a thread and step.
+// The 8 values of two words of integers.
+KUS_DEVICE void values8(uint2 u, float s, float (&f)[8]) {
+  u.x ^= 0x80808080u;
+  u.y ^= 0x80808080u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = value(e < 4 ? u.x : u.y, e % 4) * s;
+}
+
+// A row a block.  VEC: whole vectors, four groups of 8 elements a thread and
+// step, a block's width apart: a warp's store is one piece (each of two that
+// write 16 neighbours a thread fills half of the sectors that it touches), and
+// four loads are on their way at once.  8192 rows of 14336, us: one group 75,
+// two 62, four 54 (352 MB at the copy bandwidth), 16 neighbours 60.
+constexpr int kGroups = 4;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(512) values_kernel(Int8Values a) {
   pdl_wait();
@@ -464,19 +477,24 @@ __global__ void __launch_bounds__(512) values_kernel(Int8Values a) {
   const float s = a.scales[t];
   const int at = blockIdx.y * blockDim.x + threadIdx.x, step = gridDim.y * blockDim.x;
   if (VEC) {
-    for (int c = at * 16; c < a.K; c += step * 16) {
-      const uint4 u = *reinterpret_cast<const uint4*>(q + c);
-      const uint32_t w[4] = {u.x ^ 0x80808080u, u.y ^ 0x80808080u, u.z ^ 0x80808080u, u.w ^ 0x80808080u};
+    for (int c0 = at * 8; c0 < a.K; c0 += kGroups * step * 8) {
+      uint2 u[kGroups];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int g = 0; g < kGroups; ++g) {
+        const int c = c0 + g * step * 8;
+        u[g] = c < a.K ? *reinterpret_cast<const uint2*>(q + c) : make_uint2(0, 0);
+      }
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int c = c0 + g * step * 8;
+        if (c >= a.K) continue;
         float f[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = value(w[2 * h + e / 4], e % 4) * s;
+        values8(u[g], s, f);
         if constexpr (std::is_same<T, float>::value) {
-          reinterpret_cast<float4*>(out + c + 8 * h)[0] = make_float4(f[0], f[1], f[2], f[3]);
-          reinterpret_cast<float4*>(out + c + 8 * h)[1] = make_float4(f[4], f[5], f[6], f[7]);
+          reinterpret_cast<float4*>(out + c)[0] = make_float4(f[0], f[1], f[2], f[3]);
+          reinterpret_cast<float4*>(out + c)[1] = make_float4(f[4], f[5], f[6], f[7]);
         } else {
-          *reinterpret_cast<uint4*>(out + c + 8 * h) = pack8<T>(f);
+          *reinterpret_cast<uint4*>(out + c) = pack8<T>(f);
         }
       }
     }
@@ -493,11 +511,8 @@ __global__ void __launch_bounds__(512) values_kernel(Int8Values a) {
         for (int e = 0; e < 8; ++e)
           if (c + e < a.K) (e < 4 ? u.x : u.y) |= (uint32_t)(uint8_t)q[c + e] << (8 * (e % 4));
       }
-      u.x ^= 0x80808080u;
-      u.y ^= 0x80808080u;
       float f[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = value(e < 4 ? u.x : u.y, e % 4) * s;
+      values8(u, s, f);
       store_anywhere(out, c, a.K, pack8<T>(f));
     }
   }
@@ -505,8 +520,9 @@ __global__ void __launch_bounds__(512) values_kernel(Int8Values a) {
 
 template <typename T>
 void launch_values(const Int8Values& a, cudaStream_t s) {
-  const bool vec = a.K % 16 == 0 && on16(a.out, a.os, sizeof(T), a.T) && on16(a.q, a.qs, 1, a.T);
-  const int items = vec ? a.K / 16 : std::is_same<T, float>::value ? a.K : (a.K + 7) / 8;
+  const bool vec = a.K % 8 == 0 && on16(a.out, a.os, sizeof(T), a.T) &&
+                   reinterpret_cast<uintptr_t>(a.q) % 8 == 0 && (a.T <= 1 || a.qs % 8 == 0);
+  const int items = vec ? (a.K / 8 + kGroups - 1) / kGroups : std::is_same<T, float>::value ? a.K : (a.K + 7) / 8;
   const int y = (items + 511) / 512, threads = ((items + y - 1) / y + 31) / 32 * 32;
   const dim3 grid((unsigned)a.T, (unsigned)(y < 64 ? y : 64));
   if (vec)
