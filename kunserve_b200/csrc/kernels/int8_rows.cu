@@ -10,9 +10,9 @@
 // over registers, and each element is read once and written once.
 //
 // Bound by HBM and, nearly as much, by instructions: 8192 rows of 5120 in
-// bf16 take 25 us to quantise (126 MB, 15 instructions an element, 79 % of the
-// issue slots), 47 to add and norm (294 MB at 0.95 of the copy bandwidth), 38
-// with SiLU (210 MB), 22 back (126 MB).  So integers come out of the adder
+// bf16 take 24 us to quantise (126 MB, 13 instructions an element, most of the
+// issue slots), 48 to add and norm (294 MB at 0.93 of the copy bandwidth), 38
+// with SiLU (210 MB), 21 back (126 MB).  So integers come out of the adder
 // (Quotient), inputs of a quantisation stay as they are until they are
 // written, and a thread has 16 to 32 elements to share the reduction's cost.
 // All loads of a row are issued ahead of its arithmetic; a persistent block
@@ -218,28 +218,22 @@ struct Row {
 
 // The integers nearest to 127 v / top, two's complement, in the low bytes:
 // adding 1.5 * 2^23 rounds to a whole number and leaves it in the low bits (a
-// conversion runs at a quarter of the rate).  Of quantised inputs the quotient
-// is that of a product with 1 / top, put right by its remainder once
-// (Markstein 1990): where 127 v / top is a float, a half say, the result is
-// that float, and halves go to even.  Computed values have roundings of their
-// own: v times 127 / top does.
+// conversion runs at a quarter of the rate).  127 / top is held in two floats,
+// its rounding and what that left out, so that v times it is off by half a
+// step and 2^-47 of itself: where 127 v / top is a float, a half say, the
+// product is that float, and halves of quantised inputs go to even.  Computed
+// values have roundings of their own; they take the first float alone.
 struct Quotient {
-  float times, over, inverse, factor;
-  bool exact;
-  KUS_DEVICE Quotient(float top, bool sound, bool exact_) {
-    const bool range = top > 1e36f || top < 1e-30f;
-    const float small = top > 1e36f ? 0x1p-10f : top < 1e-30f ? 0x1p60f : 1.f;   // 127 v and 1 / top stay in range
-    over = sound && top > 0.f ? top * small : 1.f;
-    times = sound ? 127.f * small : 0.f;
-    inverse = 1.f / over;
-    factor = 127.f / over;
-    exact = exact_ || range;
+  float high, low, small;
+  KUS_DEVICE Quotient(float top, bool sound) {
+    // 127 / top and its rest stay in range
+    small = top > 1e30f ? 0x1p-30f : top < 1e-30f ? 0x1p60f : 1.f;
+    const float over = sound && top > 0.f ? top * small : 1.f;
+    high = 127.f / over;
+    low = fmaf(-high, over, 127.f) / over;
   }
-  KUS_DEVICE uint32_t near(float v) const { return __float_as_uint(fmaf(v, factor, 12582912.f)); }
-  KUS_DEVICE uint32_t nearest(float v) const {
-    const float t = v * times, r = t * inverse;
-    return __float_as_uint(fmaf(fmaf(-r, over, t), inverse, r) + 12582912.f);
-  }
+  KUS_DEVICE uint32_t near(float v) const { return __float_as_uint(fmaf(v, high, 12582912.f)); }
+  KUS_DEVICE uint32_t nearest(float v) const { return __float_as_uint(fmaf(v, high, v * low) + 12582912.f); }
 };
 
 // Over the warp, and over the block through `part` (32 entries, not written
@@ -270,16 +264,16 @@ struct Writer {
       : q(a.q + t * a.qs),
         K(a.K),
         sound(top < INFINITY && (OP != kRowsNorm || sum < INFINITY)),
-        quotient(top, sound, OP == kRowsQuantize) {
+        quotient(top, sound) {
     if (first) a.scales[t] = sound ? top / 127.f * (OP == kRowsNorm ? rsqrtf(sum / (float)a.K + a.eps) : 1.f) : NAN;
   }
   KUS_DEVICE void integers(const float (&v)[8], uint32_t (&r)[8]) const {
-    if (OP == kRowsQuantize || quotient.exact) {
+    if (quotient.small != 1.f) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = quotient.nearest(v[e]);
+      for (int e = 0; e < 8; ++e) r[e] = quotient.nearest(v[e] * quotient.small);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = quotient.near(v[e]);
+      for (int e = 0; e < 8; ++e) r[e] = OP == kRowsQuantize ? quotient.nearest(v[e]) : quotient.near(v[e]);
     }
   }
   // 8 columns from c, a multiple of 8 (rows of q start on 16 bytes).
@@ -372,7 +366,7 @@ struct Held {
 
 // One row a warp (ONE_WARP; eight of them a block) or a block.
 template <typename T, int OP, bool ONE_WARP, int HELD, bool ANYWHERE>
-__global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_kernel(Int8Rows a) {
+KUS_DEVICE void one_row(const Int8Rows& a) {
   __shared__ float2 part[32];
   pdl_wait();
   pdl_trigger();
@@ -385,6 +379,16 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_kernel(Int8Rows a)
   reduce_warp(OP, sum, top);
   if (!ONE_WARP) reduce_block(OP, sum, top, part);
   held.write(Writer<OP>(a, t, sum, top, lane == 0), lane, lanes);
+}
+template <typename T, int OP, bool ONE_WARP, int HELD, bool ANYWHERE>
+__global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_kernel(Int8Rows a) {
+  one_row<T, OP, ONE_WARP, HELD, ANYWHERE>(a);
+}
+// A quantisation in 16 bits: in 40 registers a thread more rows are under way
+// (8192 x 14336: 64 us, 79 in the 45 that it would take).
+template <typename T, bool ONE_WARP, int HELD, bool ANYWHERE>
+__global__ void __maxnreg__(40) quantize_kernel(Int8Rows a) {
+  one_row<T, kRowsQuantize, ONE_WARP, HELD, ANYWHERE>(a);
 }
 
 // Any row, read twice and element by element, a row a block: what is too long
@@ -417,10 +421,14 @@ template <typename T, int OP, bool ONE_WARP, int HELD>
 void launch(const Int8Rows& a, bool vec, cudaStream_t s) {
   const int threads = ONE_WARP ? 256 : ((a.K + 8 * HELD - 1) / (8 * HELD) + 31) / 32 * 32;
   const dim3 grid((unsigned)(ONE_WARP ? (a.T + 7) / 8 : a.T));
-  if (vec) {
+  if constexpr (std::is_same<T, float>::value) {
     launch_k(rows_kernel<T, OP, ONE_WARP, HELD, false>, grid, dim3(threads), 0, s, a);
-  } else if constexpr (!std::is_same<T, float>::value) {
-    launch_k(rows_kernel<T, OP, ONE_WARP, HELD, true>, grid, dim3(threads), 0, s, a);
+  } else if constexpr (OP == kRowsQuantize) {
+    launch_k(vec ? quantize_kernel<T, ONE_WARP, HELD, false> : quantize_kernel<T, ONE_WARP, HELD, true>, grid,
+             dim3(threads), 0, s, a);
+  } else {
+    launch_k(vec ? rows_kernel<T, OP, ONE_WARP, HELD, false> : rows_kernel<T, OP, ONE_WARP, HELD, true>, grid,
+             dim3(threads), 0, s, a);
   }
 }
 
