@@ -2,6 +2,7 @@
 // checked here; kunserve_b200/ops/int8.py documents them.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 #include <cmath>
@@ -80,14 +81,8 @@ void check_in_place(const torch::Tensor& out, const torch::Tensor& in, const cha
 torch::Tensor empty(at::IntArrayRef sizes, torch::ScalarType type, const torch::Device& device) {
   return torch::Tensor(at::detail::empty_cuda(sizes, type, device, {}));
 }
-// 8-bit rows that start on 16 bytes, as the matrix product reads them.
-torch::Tensor empty_rows8(int64_t rows, int64_t columns, const torch::Device& device) {
-  const int64_t wide = (columns + 15) / 16 * 16;
-  torch::Tensor t = empty({rows, wide}, torch::kInt8, device);
-  return wide == columns ? t : t.narrow(1, 0, columns);
-}
-
-// Such rows and their scales, behind them in one block of memory, and behind
+// 8-bit rows that start on 16 bytes, as the matrix product reads them, and
+// their scales, behind them in one block of memory, and behind
 // those a tensor of the rows' sizes where `total` asks for one and it is small
 // (64 KB: it may outlive the integers, whose memory it then keeps).  An
 // allocation takes a tenth of a small call.
@@ -301,14 +296,17 @@ torch::Tensor int8_linear_op(const torch::Tensor& q, const torch::Tensor& scales
   weight->use(st);
   if (M == 0) return o;
   // the kernel reads rows that start on 16 bytes
-  torch::Tensor x = q;
-  const bool on16 = reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 &&
-                    (M == 1 || (q.stride(0) % 16 == 0 && q.stride(0) >= q.size(1)));
-  if (!on16) {
-    x = empty_rows8(M, weight->K, q.device());
-    x.copy_(q);
+  const int8_t* x = q.data_ptr<int8_t>();
+  int64_t stride = (weight->K + 15) / 16 * 16;
+  c10::DataPtr copied;
+  if (reinterpret_cast<uintptr_t>(x) % 16 == 0 && (M == 1 || (q.stride(0) % 16 == 0 && q.stride(0) >= weight->K))) {
+    if (M > 1) stride = q.stride(0);
+  } else {
+    copied = c10::cuda::CUDACachingAllocator::get()->allocate(M * stride);
+    int8_align(x, q.stride(0), (int)M, weight->K, static_cast<int8_t*>(copied.get()), st);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    x = static_cast<const int8_t*>(copied.get());
   }
-  const int64_t stride = M == 1 ? (weight->K + 15) / 16 * 16 : x.stride(0);
   a.M = (int)M;
   a.N = (int)N;
   a.K = weight->K;
@@ -319,7 +317,7 @@ torch::Tensor int8_linear_op(const torch::Tensor& q, const torch::Tensor& scales
   KUS_CHECK(int8_blocks(M) * int8_blocks(N) < (1LL << 28), "the product is too large for one launch");
   const Int8Plan& plan = weight->plan_of(a.M, (int)o.element_size());
   CUtensorMap tokens;
-  KUS_CHECK(int8_token_map(&tokens, x.data_ptr<int8_t>(), stride, a.M, a.K, plan), "q cannot be mapped");
+  KUS_CHECK(int8_token_map(&tokens, x, stride, a.M, a.K, plan), "q cannot be mapped");
   int8_gemm(a, plan, weight->map, tokens, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return o;

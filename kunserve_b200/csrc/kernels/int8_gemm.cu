@@ -560,6 +560,33 @@ __global__ void __launch_bounds__(256) pack_kernel(const int8_t* w, long long st
   }
 }
 
+// Rows that start anywhere, to rows on 16 bytes (their ends up to the next 16
+// bytes are never multiplied): 16 bytes a thread, inside a row from the two
+// aligned vectors that hold them.
+__global__ void __launch_bounds__(256) align_kernel(const int8_t* q, long long stride, int M, int K, int8_t* out) {
+  pdl_wait();
+  pdl_trigger();
+  const int per = (K + 15) / 16;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)M * per; i += (long long)gridDim.x * 256) {
+    const long long t = i / per;
+    const int k = (int)(i - t * per) * 16;
+    const int8_t* from = q + t * stride + k;
+    union {
+      int8_t b[16];
+      uint4 v;
+    } x;
+    if (k >= 16 && k + 32 <= K) {
+      const int by = (int)(reinterpret_cast<uintptr_t>(from) & 15);
+      const uint4* p = reinterpret_cast<const uint4*>(from - by);
+      x.v = by ? i8rows::shifted(p[0], p[1], by) : p[0];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x.b[e] = k + e < K ? from[e] : (int8_t)0;
+    }
+    reinterpret_cast<uint4*>(out)[i] = x.v;
+  }
+}
+
 bool byte_map(CUtensorMap* map, const void* base, long long rows, int cols, long long stride, int box_rows) {
   auto fn = gemm_impl::get_encode_fn();
   if (!fn) return false;
@@ -596,6 +623,13 @@ void int8_pack(const int8_t* w, long long stride, int N, int K, int8_t* packed, 
   const long long grid = (vectors + 255) / 256;
   i8gemm::pack_kernel<<<(unsigned)(grid < 148 * 64 ? grid : 148 * 64), 256, 0, s>>>(w, stride, N, K, blocks, packed,
                                                                                  vectors, on16);
+}
+
+void int8_align(const int8_t* q, long long stride, int M, int K, int8_t* out, cudaStream_t s) {
+  LaunchBehind behind;
+  const long long grid = ((long long)M * ((K + 15) / 16) + 255) / 256;
+  launch_k(i8gemm::align_kernel, dim3((unsigned)std::min<long long>(grid, 148 * 32)), dim3(256), 0, s, q, stride, M, K,
+           out);
 }
 
 Int8Slots int8_slots() {

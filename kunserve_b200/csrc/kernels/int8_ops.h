@@ -49,6 +49,9 @@ inline long long int8_blocks(long long n) { return (n + kInt8Block - 1) / kInt8B
 
 void int8_pack(const int8_t* w, long long stride, int N, int K, int8_t* packed, cudaStream_t s);
 
+// Tokens whose rows start anywhere, in rows of K rounded up to 16 bytes.
+void int8_align(const int8_t* q, long long stride, int M, int K, int8_t* out, cudaStream_t s);
+
 struct Int8Gemm {
   int M, N, K;
   const float* x_scales;     // [M]

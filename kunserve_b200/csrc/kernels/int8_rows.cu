@@ -96,7 +96,7 @@ KUS_DEVICE T from_float(float x) { return Elem<T>::from_f(x); }
 template <>
 KUS_DEVICE float from_float<float>(float x) { return x; }
 
-// 16 bytes from byte `by` (even, below 16) of 32.
+// 16 bytes from byte `by` (below 16) of 32.
 KUS_DEVICE uint4 shifted(const uint4& a, const uint4& b, int by) {
   uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   if (by & 8) {
@@ -107,7 +107,7 @@ KUS_DEVICE uint4 shifted(const uint4& a, const uint4& b, int by) {
 #pragma unroll
     for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
   }
-  const int bits = (by & 2) * 8;
+  const int bits = (by & 3) * 8;
   return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
                     __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
 }

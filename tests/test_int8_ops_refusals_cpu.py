@@ -50,7 +50,7 @@ def test_weights_alone_are_loaded_ahead_of_the_wait():
     # and what writes weights lets nothing start before it has ended
     text = _source("int8_gemm.cu")
     pack = text[text.index("pack_kernel("):]
-    pack = pack[:pack.index("byte_map(")]
+    pack = pack[:pack.index("align_kernel(")]
     assert "pdl_wait();" in pack and "pdl_trigger" not in pack
     launch = text[text.index("void int8_pack("):]
     assert "pack_kernel<<<" in launch[:launch.index("Int8Slots")]
