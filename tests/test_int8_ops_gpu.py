@@ -63,6 +63,15 @@ def test_quantize(k, dtype):
         assert v.dtype == out and torch.equal(v, (q.float() * s[:, None]).to(out))
 
 
+def test_no_tokens():
+    from kunserve_b200 import ops
+    x = torch.empty(0, 48, device="cuda", dtype=BF)
+    for q, s, *h in (ops.quantize_int8(x), ops.silu_mul_int8(x, x), ops.add_rms_norm_int8(
+            x, torch.ones(48, device="cuda", dtype=BF), residual=x)):
+        assert q.shape == (0, 48) and s.shape == (0,) and all(t.shape == (0, 48) for t in h)
+    assert ops.dequantize_int8(*ops.quantize_int8(x)).shape == (0, 48)
+
+
 @pytest.mark.parametrize("tokens", [0, 1, 3, 257])
 def test_quantize_tokens(tokens):
     from kunserve_b200.ops import dequantize_int8, quantize_int8
@@ -104,7 +113,7 @@ def test_norm(k, dtype, residual):
 
 
 @pytest.mark.parametrize("where", ["x", "residual", "columns"])
-@pytest.mark.parametrize("k", [24, 1000, 4096, 32776])
+@pytest.mark.parametrize("k", [24, 37, 1000, 1003, 4096, 5119, 32776])
 def test_norm_sum_in_place(where, k):
     """The sum over x, over the residual, or in other columns of their buffer."""
     from kunserve_b200.ops import add_rms_norm_int8

@@ -102,6 +102,31 @@ def test_gradients_are_refused():
             f()
 
 
+@pytest.mark.parametrize("tokens", [2, 500])
+def test_results_are_plain_tensors(tokens):
+    """Whether they share their memory or not: copied, changed in place, kept
+    apart from the others, used by what records gradients and by what does not."""
+    import copy
+
+    from kunserve_b200 import ops
+    x, w = _randn(1, tokens, 200).bfloat16(), torch.ones(200, device="cuda", dtype=BF)
+    q, s, h = ops.add_rms_norm_int8(x, w, residual=x)
+    saved = [t.clone() for t in (q, s, h)]
+    assert all(torch.equal(copy.deepcopy(t), c) and torch.equal(t.cpu(), c.cpu()) for t, c in zip((q, s, h), saved))
+    h.add_(1)
+    assert torch.equal(h, saved[2] + 1) and torch.equal(q, saved[0]) and torch.equal(s, saved[1])
+    q.zero_(), s.fill_(3)
+    assert torch.equal(h, saved[2] + 1) and (q == 0).all() and (s == 3).all()
+    p = torch.nn.Parameter(torch.ones(200, device="cuda", dtype=BF))
+    (h * p).sum().backward()
+    assert p.grad is not None and not h.requires_grad
+    with torch.inference_mode():
+        q2, s2, h2 = ops.add_rms_norm_int8(x, w, residual=x)
+        y = ops.int8_linear(q2, s2, ops.Int8Weight.quantize(w[None].repeat(3, 1)))
+        h2.mul_(2)
+    assert y.shape == (tokens, 3) and torch.equal(h2, saved[2] * 2)
+
+
 # ------------------------------------------------------------- a layer of them
 class Layer:
     """Projections of a decoder layer in 8 bits; every value's group of heads
@@ -310,3 +335,33 @@ def test_results_repeat():
         want = ops.int8_linear(q, s, weight, dtype=HALF)
         for _ in range(10):
             assert torch.equal(ops.int8_linear(q, s, weight, dtype=HALF), want)
+
+
+# ------------------------------------------------------- offsets past 32 bits
+def test_rows_past_32_bits():
+    from kunserve_b200 import ops
+    t, k = 70001, 32768
+    x = torch.empty(t, k, device="cuda", dtype=BF)
+    x[-3:] = _randn(1, 3, k).bfloat16()
+    x[:2] = _randn(2, 2, k).bfloat16()
+    w = _randn(3, k).bfloat16()
+    edge = torch.cat([x[:2], x[-3:]])
+    for f in (ops.quantize_int8, lambda v: ops.silu_mul_int8(v, v), lambda v: ops.add_rms_norm_int8(v, w)[:2]):
+        x[2:-3] = 1
+        (q, s), (q1, s1) = f(x), f(edge)
+        assert torch.equal(torch.cat([q[:2], q[-3:]]), q1) and torch.equal(torch.cat([s[:2], s[-3:]]), s1)
+        v = ops.dequantize_int8(q, s)
+        assert torch.equal(v[-3:], ops.dequantize_int8(q1, s1)[-3:])
+        del q, v
+
+
+def test_products_past_32_bits():
+    from kunserve_b200 import ops
+    # the result: 2.3e9 elements; the weights: 2.3e9 bytes
+    for m, k, n in ((17001, 40, 135000), (5, 16400, 140001)):
+        q, s, w, v = _linear_inputs(m, k, n)
+        y = ops.int8_linear(q, s, ops.Int8Weight(w, v))
+        rows, last = torch.tensor([0, m // 2, m - 1], device="cuda"), n - 200
+        check_linear(y[rows][:, last:], q[rows], s[rows], w[last:], v[last:])
+        check_linear(y[rows][:, :300], q[rows], s[rows], w[:300], v[:300])
+        del y, w
