@@ -13,7 +13,8 @@
 // split over the CTAs of a cluster until they fill the GPU, and their parts
 // go through distributed shared memory: integers add up in any order, so no
 // workspace, counter or second kernel is needed (64 x 5120 x 5120: 7.9 us in
-// three parts, 14 whole).  Many tokens: the tensor cores, and for them what an
+// three parts, 9.0 whole where the next products start on the SMs left idle,
+// 14 alone).  Many tokens: the tensor cores, and for them what an
 // SM can load: a tile of 128 x 256 needs 96 bytes a clock at the int8 rate,
 // one of 256 x 256 on a pair of CTAs (cta_group::2), each loading half of
 // either side, 64.  8192 x 4096 x 28672: 856 us in single CTAs, 564 in pairs
