@@ -17,15 +17,16 @@
 // 14 alone).  Many tokens: the tensor cores, and for them what an
 // SM can load: a tile of 128 x 256 needs 96 bytes a clock at the int8 rate,
 // one of 256 x 256 on a pair of CTAs (cta_group::2), each loading half of
-// either side, 64.  8192 x 4096 x 28672: 856 us in single CTAs, 564 in pairs
-// with the pipe active for 94 % of the cycles, at 1.5 GHz under the power
-// limit (3.4 PFLOP/s; 645 us, 3.0, when it runs on).
+// either side, 64.  8192 x 4096 x 28672: 789 us in single CTAs where pairs took
+// 684, and 564 on a cool GPU with the pipe active for 94 % of the cycles, at
+// 1.5 GHz under the power limit (3.4 PFLOP/s; 645 us, 3.0, when it runs on).
 //
 // Results: one warp a scheduler could not scale, convert and store a tile
 // while the next one was multiplied (10 us against 9).  Two groups of four
 // warps take every other 16 tokens, read TMEM as MMA fragments, and stmatrix
-// turns channels into rows of 16 bytes; with direct 2-byte stores 8192 x 4096
-// x 28672 took 806 us, through shared memory by 2-byte stores 684.
+// turns channels into rows of 16 bytes.  The same product took 884 us with
+// direct 2-byte stores and 805 with one group that went through shared memory
+// by 2-byte stores, where this took 684.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
