@@ -365,3 +365,11 @@ def test_products_past_32_bits():
         check_linear(y[rows][:, last:], q[rows], s[rows], w[last:], v[last:])
         check_linear(y[rows][:, :300], q[rows], s[rows], w[:300], v[:300])
         del y, w
+
+
+def test_clusters_that_the_device_holds():
+    """What cuts are chosen by: of single CTAs one an SM, of clusters no more than fit."""
+    from kunserve_b200.ops import native
+    slots = native().int8_slots()
+    sms = native().num_sms()
+    assert slots[1] == sms and all(1 <= slots[c] and c * slots[c] <= sms for c in range(2, 9))
