@@ -30,6 +30,7 @@
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <utility>
 
 #include "../common.cuh"
 #include "cache_elem.cuh"
@@ -46,6 +47,7 @@ constexpr int kMostStages = 8;
 constexpr int kBarriers = 2 * kMostStages + 5;
 // Shared memory of a CTA: alone on its SM, or one of two.
 constexpr int kSmemAlone = 232448, kSmemHalf = 115712;
+constexpr int kSmemSm = 233472, kSmemKept = 1024;      // of an SM, and what the driver keeps of it for each CTA
 
 // Results go through shared memory, so that whole lines are written: each
 // group of epilogue warps has two buffers of 16 tokens x 128 channels, the
@@ -758,10 +760,15 @@ Int8Plan int8_plan(int M, int N, int K, int element, const Int8Slots& slots) {
   p.apart = p.splits > 1 && p.width <= (p.alone ? 64 : 32);
   p.stages = kMostStages;
   while (smem_bytes(p, element) > (p.alone ? kSmemAlone : kSmemHalf)) --p.stages;
-  // what a CTA fills once needs no more room than that: more of the next
-  // kernel fits beside it
-  if (p.splits > 1 ? p.apart : units <= most)
-    p.stages = std::min(p.stages, std::max(2, (blocks + p.splits - 1) / p.splits));
+  // What a CTA fills once needs no more room than that: more of the next
+  // kernel fits beside it.  But never so many CTAs an SM that their TMEM would
+  // not fit: one that waits for it while its pair's other CTA holds some could
+  // wait for a pair that waits for this one.
+  if (p.splits > 1 ? p.apart : units <= most) {
+    int stages = std::min(p.stages, std::max(2, (blocks + p.splits - 1) / p.splits));
+    std::swap(stages, p.stages);
+    while (p.stages < stages && kSmemSm / (smem_bytes(p, element) + kSmemKept) * p.tmem_columns > 512) ++p.stages;
+  }
   // the tokens of a group: at most 32 MB
   p.group = (int)std::max(1ll, std::min<long long>(p.token_tiles, (32ll << 20) / ((long long)p.width * K)));
   return p;

@@ -52,7 +52,10 @@ def test_every_tile_once(seed, slots):
         else:
             side = parts if p["apart"] else 0
             assert p["apart"] or parts <= p["stages"] * stage
-        assert p["stages"] * stage + side + 21 * 8 + 16 + 1024 <= SHARED[bool(p["alone"])]
+        used = p["stages"] * stage + side + 21 * 8 + 16 + 1024
+        assert used <= SHARED[bool(p["alone"])]
+        # however many such CTAs an SM has room for, of one product or of several: their TMEM fits
+        assert 233472 // (used + 1024) * p["tmem_columns"] <= 512
         assert 2 * p["width"] <= p["tmem_columns"] <= (512 if p["alone"] else 256)
         if units < 20000:
             seen = set(_units(p))
