@@ -348,6 +348,6 @@ void bind_int8_ops(py::module& m) {
     return std::map<std::string, int>{{"pair", p.pair},     {"width", p.width}, {"token_tiles", p.token_tiles},
                                       {"channel_tiles", p.channel_tiles},       {"splits", p.splits}, {"alone", p.alone}, {"apart", p.apart},
                                       {"group", p.group},   {"grid", p.grid},   {"stages", p.stages},
-                                      {"tmem_columns", p.tmem_columns}};
+                                      {"tmem_columns", p.tmem_columns},         {"smem", p.smem}};
   });
 }

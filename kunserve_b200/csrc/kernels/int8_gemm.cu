@@ -48,6 +48,7 @@ constexpr int kBarriers = 2 * kMostStages + 5;
 // Shared memory of a CTA: alone on its SM, or one of two.
 constexpr int kSmemAlone = 232448, kSmemHalf = 115712;
 constexpr int kSmemSm = 233472, kSmemKept = 1024;      // of an SM, and what the driver keeps of it for each CTA
+constexpr int kTmemSm = 512;                           // columns of an SM
 
 // Results go through shared memory, so that whole lines are written: each
 // group of epilogue warps has two buffers of 16 tokens x 128 channels, the
@@ -68,6 +69,13 @@ KUS_HOST_DEVICE int side_bytes(const Int8Plan& p, int element) {
 int smem_bytes(const Int8Plan& p, int element) {
   return p.stages * stage_bytes(p) + side_bytes(p, element) + kBarriers * 8 + 16 + 1024;
 }
+// The least that a CTA asks for.  CTAs wait for TMEM without a limit, those of
+// a cluster for one another, and CTAs of other products may hold it: two
+// clusters that each had a part of what the other waits for would never end.
+// So a CTA's share of an SM's shared memory is no less than its share of the
+// TMEM, and whatever meets on an SM fits both.  (The framework's other
+// clusters with TMEM, pairs of the bf16 product, leave room for no CTA here.)
+int least_smem(int tmem_columns) { return (tmem_columns * kSmemSm + kTmemSm - 1) / kTmemSm - kSmemKept; }
 
 // D(tmem, s32) (+)= A(smem, s8) * B(smem, s8)^T; of a pair: A rows 128 and
 // up and the second half of B's rows are the other CTA's (umma_f16_pair).
@@ -607,7 +615,7 @@ template <typename O, bool PAIR, bool SPLIT>
 void launch(const Int8Gemm& a, const Int8Plan& p, const CUtensorMap& w, const CUtensorMap& x, cudaStream_t s) {
   const auto kernel = gemm_kernel<O, PAIR, SPLIT>;
   ensure_smem_attr(reinterpret_cast<const void*>(kernel), kSmemAlone);
-  launch_kc(kernel, dim3(p.grid), dim3(kThreads), smem_bytes(p, sizeof(O)), s, (PAIR ? 2 : 1) * p.splits, w, x, a, p);
+  launch_kc(kernel, dim3(p.grid), dim3(kThreads), p.smem, s, (PAIR ? 2 : 1) * p.splits, w, x, a, p);
 }
 
 template <typename O>
@@ -760,15 +768,15 @@ Int8Plan int8_plan(int M, int N, int K, int element, const Int8Slots& slots) {
   p.apart = p.splits > 1 && p.width <= (p.alone ? 64 : 32);
   p.stages = kMostStages;
   while (smem_bytes(p, element) > (p.alone ? kSmemAlone : kSmemHalf)) --p.stages;
-  // What a CTA fills once needs no more room than that: more of the next
-  // kernel fits beside it.  But never so many CTAs an SM that their TMEM would
-  // not fit: one that waits for it while its pair's other CTA holds some could
-  // wait for a pair that waits for this one.
+  const int asked = least_smem(p.tmem_columns);
+  // What a CTA fills once needs no more room than that, and what it asks for
+  // anyway: more of the next kernel fits beside it.
   if (p.splits > 1 ? p.apart : units <= most) {
     int stages = std::min(p.stages, std::max(2, (blocks + p.splits - 1) / p.splits));
     std::swap(stages, p.stages);
-    while (p.stages < stages && kSmemSm / (smem_bytes(p, element) + kSmemKept) * p.tmem_columns > 512) ++p.stages;
+    while (p.stages < stages && smem_bytes(p, element) < asked) ++p.stages;
   }
+  p.smem = std::max(smem_bytes(p, element), asked);
   // the tokens of a group: at most 32 MB
   p.group = (int)std::max(1ll, std::min<long long>(p.token_tiles, (32ll << 20) / ((long long)p.width * K)));
   return p;

@@ -72,6 +72,7 @@ struct Int8Plan {
   int group;                 // token tiles walked before the next channel tile
   int grid;                  // CTAs
   int stages, tmem_columns;
+  int smem;                  // bytes of dynamic shared memory a CTA asks for
 };
 // Clusters of 1 to 8 CTAs that the device holds at once, with one CTA an SM.
 struct Int8Slots {
