@@ -256,10 +256,16 @@ struct Int8Weight {
     K = (int)q.size(1);
     const int64_t blocks = int8_blocks(N) * int8_blocks(K);
     packed = empty({blocks, kInt8Block, kInt8Block}, torch::kInt8, q.device());
-    scales = s.clone();
+    scales = empty({N}, torch::kFloat32, q.device());
     KUS_CHECK(int8_weight_map(&map, packed.data_ptr<int8_t>(), N, K), "the weight is too large");
-    int8_pack(q.data_ptr<int8_t>(), q.stride(0), N, K, packed.data_ptr<int8_t>(), at::cuda::getCurrentCUDAStream());
+    int8_pack(q.data_ptr<int8_t>(), q.stride(0), N, K, packed.data_ptr<int8_t>(), made_on);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
+    // Behind the packing, and no kernel: it begins once the packing has ended
+    // and its writes are seen, and what comes after it begins no earlier.  A
+    // product behind the packing itself could start as soon as the last of its
+    // blocks had left, and reads its first weights before it waits.
+    C10_CUDA_CHECK(cudaMemcpyAsync(scales.data_ptr<float>(), s.data_ptr<float>(), N * sizeof(float),
+                                   cudaMemcpyDeviceToDevice, made_on));
   }
   // The weights outlive the work queued on `st`.
   void use(const c10::cuda::CUDAStream& st) const {

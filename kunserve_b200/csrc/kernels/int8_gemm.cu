@@ -291,8 +291,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       tma_load_2d(to, &tmW, &full[st], 0, row);
   };
   // The first stages' weights are on their way while this kernel sets up and
-  // the one before ends: none but pack_kernel writes weights, and nothing
-  // starts before that one has ended.
+  // the one before ends: none but pack_kernel writes weights, and a copy
+  // behind it keeps whatever follows from starting early.
   const Unit start = unit_at(p, first);
   const int early = first < units ? min(stages, kb1 - kb0) : 0;
   if (threadIdx.x == 0) {
@@ -550,8 +550,6 @@ __global__ void __launch_bounds__(kThreads, 2)
 // 16 bytes of a packed block a thread.
 __global__ void __launch_bounds__(256) pack_kernel(const int8_t* w, long long stride, int N, int K, int blocks,
                                                    int8_t* packed, long long vectors, bool on16) {
-  // the next kernel may read weights ahead of its wait: this one never lets
-  // it start early
   pdl_wait();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < vectors; i += (long long)gridDim.x * 256) {
     const long long block = i / (kInt8Block * kBK / 16);

@@ -47,6 +47,9 @@ constexpr int kInt8Block = 128;
 constexpr int kInt8MaxK = 131071;   // 2^31 / (128 * 128) terms fit an int32 sum
 inline long long int8_blocks(long long n) { return (n + kInt8Block - 1) / kInt8Block; }
 
+// A product reads its first weights ahead of its wait for the kernel before it,
+// which alone makes that one's writes visible: behind int8_pack the caller
+// queues something that never lets another start early, a copy say.
 void int8_pack(const int8_t* w, long long stride, int N, int K, int8_t* packed, cudaStream_t s);
 
 // Tokens whose rows start anywhere, in rows of K rounded up to 16 bytes.
