@@ -254,13 +254,14 @@ KUS_DEVICE bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
 }
 
 // Bounded wait on a barrier that the other CTA of the pair arrives on.
+template <bool DRAIN = false>
 KUS_DEVICE bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int err_code) {
   if (mbar_try_wait_cluster(bar, parity)) return true;
   const unsigned long long t0 = global_ns();
   for (uint32_t i = 1; i < kSpinLimit; ++i) {
     if (mbar_try_wait_cluster(bar, parity)) return true;
     if ((i & 255u) == 0) {
-      if (wait_failed()) return false;
+      if (!DRAIN && wait_failed()) return false;
       if (global_ns() - t0 > kWaitNs) break;
     }
   }

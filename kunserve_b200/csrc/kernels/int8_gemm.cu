@@ -44,7 +44,7 @@ constexpr int kBK = kInt8Block;        // bytes of K per stage
 constexpr int kWBytes = kInt8Block * kBK;
 
 constexpr int kMostStages = 8;
-constexpr int kBarriers = 2 * kMostStages + 5;
+constexpr int kBarriers = 2 * kMostStages + 6;
 // Shared memory of a CTA: alone on its SM, or one of two.
 constexpr int kSmemAlone = 232448, kSmemHalf = 115712;
 constexpr int kSmemSm = 233472, kSmemKept = 1024;      // of an SM, and what the driver keeps of it for each CTA
@@ -130,6 +130,11 @@ KUS_DEVICE void tmem_ld16(uint32_t taddr, int (&r)[16]) {
 // The halves of cluster_sync.
 KUS_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 KUS_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// As if `bytes` of a copy had landed.
+KUS_DEVICE void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 
 KUS_DEVICE void st_cluster(uint32_t addr, int v) {
   asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
@@ -264,7 +269,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* tfull = empty + kMostStages;
   uint64_t* tempty = tfull + 2;
   uint64_t* drained = tempty + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
+  uint64_t* told = drained + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(told + 1);
+  int* other_fills = reinterpret_cast<int*>(tmem_holder + 1);      // of a pair's leader: the other CTA's
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int blocks = (a.K + kBK - 1) / kBK;
@@ -305,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(&tempty[b], 2 * kCtas);      // each group of epilogue warps
     }
     mbar_init(drained, 1);
+    mbar_init(told, 1);
     fence_barrier_init();
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the copies find the barriers ready
     if (!PAIR)
@@ -381,11 +389,24 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         kb = kb0;
       }
-      // every copy has landed before the CTA ends (a pair's, before the
-      // leader meets the other CTA at the end)
-      if (leads)
-        for (int f = max(0, fills - stages); f < fills; ++f)
+      // Every copy has landed before the CTA ends (a pair's, before the leader
+      // meets the other CTA at the end).  Where waits ran out, one CTA of a pair
+      // may have filled stages that the other did not: the leader then expects
+      // or makes up for one CTA's bytes.  Neither is ahead by more than the
+      // stages, since a stage is free again once both have filled it.
+      if (leads) {
+        int other = fills;
+        if (PAIR && mbar_wait_cluster<true>(told, 0, kErrWaitFull)) other = *other_fills;
+        const int filled = max(fills, other);
+        for (int f = max(0, filled - stages); f < filled; ++f) {
+          if (PAIR && f >= fills) mbar_arrive_expect_tx(&full[f % stages], (uint32_t)stage_size);
+          if (PAIR && f >= other) mbar_complete_tx(&full[f % stages], (uint32_t)stage_size);
           mbar_wait<true>(&full[f % stages], (f / stages) & 1, kErrWaitFull);
+        }
+      } else {
+        st_cluster(mapa_shared(smem_u32(other_fills), lead), fills);
+        mbar_arrive_remote(mapa_shared(smem_u32(told), lead));
+      }
     }
   } else if (warp == 1) {
     if (leads && elect_one_sync()) {
