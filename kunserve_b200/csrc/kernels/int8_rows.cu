@@ -252,6 +252,10 @@ KUS_DEVICE void reduce_block(int op, float& sum, float& top, float2* part) {
   reduce_warp(op, sum, top);
 }
 
+// The largest scale whose 127-fold is finite: the float nearest to the largest
+// float / 127 is one above.
+constexpr float kMostScale = 0x810203p98f;
+
 // A row's scale, and its integers.  A row without finite values has scale NaN.
 template <int OP>
 struct Writer {
@@ -265,7 +269,9 @@ struct Writer {
         K(a.K),
         sound(top < INFINITY && (OP != kRowsNorm || sum < INFINITY)),
         quotient(top, sound) {
-    if (first) a.scales[t] = sound ? top / 127.f * (OP == kRowsNorm ? rsqrtf(sum / (float)a.K + a.eps) : 1.f) : NAN;
+    if (!first) return;
+    const float scale = OP == kRowsNorm ? top / 127.f * rsqrtf(sum / (float)a.K + a.eps) : fminf(top / 127.f, kMostScale);
+    a.scales[t] = sound ? scale : NAN;
   }
   KUS_DEVICE void integers(const float (&v)[8], uint32_t (&r)[8]) const {
     if (quotient.small != 1.f) {

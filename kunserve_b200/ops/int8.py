@@ -8,8 +8,9 @@ each, weights with one scale per output channel.
     x = ops.int8_linear(q, s, w_o)
     q, s = ops.silu_mul_int8(gate, up)                        # views of one projection's output
 
-A row's scale is its largest magnitude / 127 (fp32) and an element's integer
-the nearest to 127 times it over that magnitude, halves to even; a row of
+A row's scale is its largest magnitude / 127 (fp32; the float below where 127
+times it would leave the range) and an element's integer the nearest to 127
+times it over that magnitude, halves to even; a row of
 zeros has scale 0.  A row with a NaN or an infinity, or whose values leave
 fp32's range on the way, has scale NaN and integers 0: everything computed of
 it is NaN.
