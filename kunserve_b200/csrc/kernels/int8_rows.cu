@@ -264,14 +264,18 @@ struct Writer {
   bool sound;
   Quotient quotient;
 
+  KUS_DEVICE static float factor(const Int8Rows& a, float sum) {
+    return OP == kRowsNorm ? rsqrtf(sum / (float)a.K + a.eps) : 1.f;
+  }
+  // Whether the row's values are finite.  Of a norm the factor counts, at most
+  // 2.7e22 (of the least eps): its cost is met by rows beyond 1e16 alone.
+  KUS_DEVICE static bool finite(const Int8Rows& a, float sum, float top) {
+    if (OP == kRowsNorm && top > 1e16f) return sum < INFINITY && top * factor(a, sum) < INFINITY;
+    return top < INFINITY && (OP != kRowsNorm || sum < INFINITY);
+  }
   KUS_DEVICE Writer(const Int8Rows& a, long long t, float sum, float top, bool first)
-      : q(a.q + t * a.qs),
-        K(a.K),
-        sound(top < INFINITY && (OP != kRowsNorm || sum < INFINITY)),
-        quotient(top, sound) {
-    if (!first) return;
-    const float scale = OP == kRowsNorm ? top / 127.f * rsqrtf(sum / (float)a.K + a.eps) : fminf(top / 127.f, kMostScale);
-    a.scales[t] = sound ? scale : NAN;
+      : q(a.q + t * a.qs), K(a.K), sound(finite(a, sum, top)), quotient(top, sound) {
+    if (first) a.scales[t] = sound ? fminf(top / 127.f * factor(a, sum), kMostScale) : NAN;
   }
   KUS_DEVICE void integers(const float (&v)[8], uint32_t (&r)[8]) const {
     if (quotient.small != 1.f) {

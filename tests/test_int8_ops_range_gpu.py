@@ -32,3 +32,46 @@ def test_largest_rows_come_back_finite(k, dtype):
     if t != F32:
         assert torch.equal(s, top[:, 0].float() / 127)
     assert dequantize_int8(q, s, t).isfinite().all()
+
+
+@pytest.mark.parametrize("k", [64, 333, 4096, 40000])
+def test_norms_that_leave_the_range_say_so(k):
+    """h w is finite, its norm is not: scale NaN and integers 0, as of any row
+    that leaves fp32 on the way.  Rows beside it, near the range's end too, keep
+    their values."""
+    from kunserve_b200.ops import add_rms_norm_int8, dequantize_int8
+    w = torch.full((k,), 3e38, device="cuda").bfloat16()
+    x = torch.zeros(4, k, device="cuda").bfloat16()
+    x[0, 3] = 0.5                      # sqrt(k) times the weight
+    x[1] = 0.5                         # the weight itself
+    x[2, 3], x[2, 4:] = 1.0, 1e-3      # below sqrt(k) times it, above it for k > 1
+    q, s, _ = add_rms_norm_int8(x, w, 1e-5)
+    v = dequantize_int8(q, s, F32)
+    total = x.double()
+    y = total / (total.square().mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+    top = y.abs().amax(1)
+    assert (top > torch.finfo(F32).max).tolist() == [True, False, True, False]
+    assert s.isnan().tolist() == [True, False, True, False] and (q[[0, 2]] == 0).all()
+    assert v.isnan().all(1).tolist() == [True, False, True, False]
+    # 33 + 12: of the squares' sum and the factors (more where a row is read twice), as for other norms
+    u = (10 + 8 * -(-k // 8192) + 32) * U
+    assert v[[1, 3]].isfinite().all()
+    assert ((v - y).abs()[[1, 3]] <= (0.5 / 127 + u) * top[[1, 3], None]).all()
+
+
+def test_norms_near_the_range_keep_their_values():
+    """A weight so large that the norm ends just inside fp32."""
+    from kunserve_b200.ops import add_rms_norm_int8, dequantize_int8
+    k, big = 64, torch.finfo(torch.bfloat16).max
+    x = torch.zeros(1, k, device="cuda").bfloat16()
+    x[0, 0] = 1.0                      # 8 times the weight, less 1 in 3200 for eps
+    for share, inside in ((1.0, True), (1.01, False), (0.5, True)):
+        w = torch.full((k,), big / 8 * share, device="cuda").bfloat16()
+        q, s, _ = add_rms_norm_int8(x, w, 1e-5)
+        v = dequantize_int8(q, s, F32)
+        want = float(w[0].double()) / (1 / k + 1e-5) ** 0.5
+        assert (want <= torch.finfo(F32).max) == inside
+        if inside:
+            assert q[0, 0] == 127 and abs(v[0, 0].item() - want) <= 45 * U * want and (v[0, 1:] == 0).all()
+        else:
+            assert (q == 0).all() and v.isnan().all()
