@@ -26,6 +26,8 @@ int value_type(torch::ScalarType t, bool fp32, const char* what) {
 void no_gradient(const torch::Tensor& t, const char* what) {
   TORCH_CHECK_VALUE(!(t.requires_grad() && at::GradMode::is_enabled()), what,
                     " requires a gradient, but 8-bit results carry none (call under torch.no_grad())");
+  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), what,
+                    " carries a forward-mode tangent, but 8-bit results carry none (detach it)");
 }
 
 // [T, K] on a GPU, the elements of a row next to one another.

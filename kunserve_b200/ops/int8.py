@@ -17,7 +17,8 @@ it is NaN.
 
 All run on the current CUDA stream of their tensors' device and allocate what
 they return from it.  They serve: results carry no gradient, and arguments that
-require one are refused while gradients are recorded.
+require one are refused while gradients are recorded, as are arguments with a
+forward-mode tangent.
 """
 from typing import Optional, Tuple
 
