@@ -61,6 +61,10 @@ bool apart(const torch::Tensor& a, const torch::Tensor& b) {
   const auto x = span(a), y = span(b);
   return x.first == x.second || y.first == y.second || x.second <= y.first || y.second <= x.first;
 }
+// A kernel writes over `t`: what gradients were recorded with it shows as changed.
+void changed(const torch::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 // A written tensor's rows lie apart from one another.
 void check_written(const torch::Tensor& t, const char* what) {
   KUS_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), what, "'s rows overlap: sizes ", t.sizes(), " strides ",
@@ -174,6 +178,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> add_rms_norm_int8_op(con
     KUS_CHECK(apart(total, weight), "out overlaps weight");
   }
   auto [q, scales] = run_rows(a, x, &total);
+  if (out.has_value()) changed(total);
   return {q, scales, total};
 }
 
@@ -220,6 +225,7 @@ torch::Tensor dequantize_int8_op(const torch::Tensor& q, const torch::Tensor& sc
   a.K = (int)q.size(1);
   int8_values(a, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (out.has_value()) changed(o);
   return o;
 }
 
@@ -328,6 +334,7 @@ torch::Tensor int8_linear_op(const torch::Tensor& q, const torch::Tensor& scales
   KUS_CHECK(int8_token_map(&tokens, x, stride, a.M, a.K, plan), "q cannot be mapped");
   int8_gemm(a, plan, weight->map, tokens, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (out.has_value()) changed(o);
   return o;
 }
 
