@@ -11,7 +11,7 @@
 //
 // Bound by HBM and, nearly as much, by instructions: 8192 rows of 5120 in
 // bf16 take 24 us to quantise (126 MB, 13 instructions an element, most of the
-// issue slots), 48 to add and norm (294 MB at 0.93 of the copy bandwidth), 38
+// issue slots), 48 to add and norm (294 MB at 0.93 of the copy bandwidth), 39
 // with SiLU (210 MB), 21 back (126 MB).  So integers come out of the adder
 // (Quotient), inputs of a quantisation stay as they are until they are
 // written, and a thread has 16 to 32 elements to share the reduction's cost.
@@ -34,20 +34,70 @@ KUS_DEVICE float max_nan(float a, float b) {
   return r;
 }
 
-// 1 / (1 + e^-g).  Of its roundings that of g log2 e grows with g: e^-g is off
-// by 2 + 1.2 |g| units in the last place, of which the sum takes up the share
-// e^-g / (1 + e^-g).  silu is off by 5.4 * 2^-24 of the gate at most, where
-// expf would leave 5: 8192 rows of 14336 take 105 us with this, 115 with expf.
-// Zero from g < -87 on, where it leaves the normal range.
-KUS_DEVICE float sigmoid(float g) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
-  return r;
+// Pairs of floats in one instruction each.
+struct Pair {
+  unsigned long long v;
+  KUS_DEVICE Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  KUS_DEVICE explicit Pair(float a) : Pair(a, a) {}
+  KUS_DEVICE float2 get() const {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
+};
+KUS_DEVICE Pair operator*(Pair a, const Pair& b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+KUS_DEVICE Pair operator+(Pair a, const Pair& b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+KUS_DEVICE Pair fma(Pair a, const Pair& b, const Pair& c) {
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(a.v) : "l"(b.v), "l"(c.v));
+  return a;
+}
+
+// g / (1 + e^-g) * u of two gates within kWide of zero.  e^-g = 2^n e^d: n is
+// -g log2 e rounded, whose rounding would cost e^-g |g| units in the last
+// place, and d what that left out, from an exact product and log2 e in two
+// floats.  y is off by at most 10 * 2^-24 of itself: 2^n by 4 (two units), its
+// product with 1 + d by 1, the sum by 1, the reciprocal by 2, two products by
+// 1 each.  8192 rows of 14336 take 106 us with this in bf16 and 104 in fp16;
+// 103 and 108 with e^-g of n alone, by which y is off by 1.2 |g| units more.
+constexpr float kWide = 80.f;
+KUS_DEVICE void silu_pair(float& g0, float& g1, float u0, float u1) {
+  constexpr float kLog2e = 0x1.715476p+0f, kRest = 0x1.4ae0bep-26f, kLn2 = 0x1.62e430p-1f;
+  const Pair g(g0, g1), n = g * Pair(-kLog2e);
+  const Pair d = fma(g, Pair(kRest), fma(g, Pair(kLog2e), n)) * Pair(-kLn2);
+  const float2 m = n.get();
+  const Pair e(ex2(m.x), ex2(m.y));
+  float2 r = (fma(e, d, e) + Pair(1.f)).get();
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.y));
+  const float2 y = (g * Pair(r.x, r.y) * Pair(u0, u1)).get();
+  g0 = y.x;
+  g1 = y.y;
+}
+// Of a gate beyond kWide 1 + e^-g is 1 or e^-g to a float's last place, and
+// e^-g may leave the range where y does not: e^g is taken as a square.  Off by
+// 11 * 2^-24 of y (two exponentials by 4 each, three products).
+KUS_DEVICE float silu_wide(float g, float u) {
+  if (g > 0.f) return g * u;
+  const float h = expf(0.5f * g);
+  return (g * h) * (u * h);
 }
 
 // The largest of non-negative floats, NaN above all: their bits' order.
 KUS_DEVICE float warp_top(float v) {
   return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+
+KUS_DEVICE float top_of(const float (&f)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(f[e]));
+  return m;
 }
 
 // 8 neighbours of a row as they lie in memory.
@@ -79,11 +129,9 @@ struct Raw8<float> {
     f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
   }
   KUS_DEVICE float top() const {
-    float f[8], m = 0.f;
+    float f[8];
     values(f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(f[e]));
-    return m;
+    return top_of(f);
   }
 };
 
@@ -190,9 +238,15 @@ struct Row {
       y[e] *= w[e];
     }
   }
-  KUS_DEVICE static void gate(float (&y)[8], const float (&o)[8]) {
+  // `wide` gains the gates' magnitudes; with one beyond kWide y stays undone.
+  // (The branch for each group also keeps a group's arithmetic ahead of later
+  // groups' loads: 106 us for 8192 x 14336, 113 without.)
+  KUS_DEVICE static void gate(float (&y)[8], const float (&o)[8], float& wide) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = y[e] * sigmoid(y[e]) * o[e];
+    for (int e = 0; e < 8; ++e) wide = fmaxf(wide, fabsf(y[e]));
+    if (wide > kWide) return;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) silu_pair(y[e], y[e + 1], o[e], o[e + 1]);
   }
 
   // Element by element; `keep`: write x + residual.
@@ -212,7 +266,15 @@ struct Row {
       }
     }
     if (OP == kRowsNorm) combine(y, w, sum);
-    if (OP == kRowsSilu) gate(y, o);
+    if (OP == kRowsSilu) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float g0 = y[e], g1 = y[e + 1];
+        silu_pair(y[e], y[e + 1], o[e], o[e + 1]);
+        if (fabsf(g0) > kWide) y[e] = silu_wide(g0, o[e]);
+        if (fabsf(g1) > kWide) y[e + 1] = silu_wide(g1, o[e + 1]);
+      }
+    }
   }
 };
 
@@ -236,10 +298,12 @@ struct Quotient {
   KUS_DEVICE uint32_t nearest(float v) const { return __float_as_uint(fmaf(v, high, v * low) + 12582912.f); }
 };
 
-// Over the warp, and over the block through `part` (32 entries, not written
+// Of squares the sum, of SiLU's gates the largest magnitude, and of values the
+// largest: over the warp, and over the block through `part` (32 entries, not written
 // again before every thread has read them).
 KUS_DEVICE void reduce_warp(int op, float& sum, float& top) {
   if (op == kRowsNorm) sum = warp_sum(sum);
+  if (op == kRowsSilu) sum = warp_top(sum);
   top = warp_top(top);
 }
 KUS_DEVICE void reduce_block(int op, float& sum, float& top, float2* part) {
@@ -353,10 +417,9 @@ struct Held {
           w.values(f);
           Row<T, OP>::combine(y[j], f, sum);
         } else {
-          Row<T, OP>::gate(y[j], f);
+          Row<T, OP>::gate(y[j], f, sum);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(y[j][e]));
+        top = max_nan(top, top_of(y[j]));
       }
     }
   }
@@ -374,6 +437,26 @@ struct Held {
   }
 };
 
+// Any row, read twice and element by element.
+template <typename T, int OP, bool ONE_WARP>
+KUS_DEVICE void row_in_two_passes(const Int8Rows& a, long long t, int lane, int lanes, float2* part) {
+  const Row<T, OP> row(a, t);
+  float sum = 0.f, top = 0.f, y[8];
+  for (int c = lane * 8; c < a.K; c += lanes * 8) {
+    row.values(c, false, y, sum);
+    top = max_nan(top, top_of(y));
+  }
+  reduce_warp(OP, sum, top);
+  if (!ONE_WARP) reduce_block(OP, sum, top, part);
+  const Writer<OP> writer(a, t, sum, top, lane == 0);
+  // the sum x + residual is written in the second pass: it may lie over either of them
+  for (int c = lane * 8; c < a.K; c += lanes * 8) {
+    float unused = 0.f;
+    row.values(c, true, y, unused);
+    writer.write(c, y);
+  }
+}
+
 // One row a warp (ONE_WARP; eight of them a block) or a block.
 template <typename T, int OP, bool ONE_WARP, int HELD, bool ANYWHERE>
 KUS_DEVICE void one_row(const Int8Rows& a) {
@@ -388,6 +471,13 @@ KUS_DEVICE void one_row(const Int8Rows& a) {
   held.read(Row<T, OP>(a, t), lane, lanes, sum, top);
   reduce_warp(OP, sum, top);
   if (!ONE_WARP) reduce_block(OP, sum, top, part);
+  if (OP == kRowsSilu && sum > kWide) {
+    // A gate that silu_pair does not know: the row once more, each element by its
+    // own formula.  (Here and not where it is met: that took the registers of
+    // rows under way.)
+    if (!ONE_WARP) __syncthreads();
+    return row_in_two_passes<T, OP, ONE_WARP>(a, t, lane, lanes, part);
+  }
   held.write(Writer<OP>(a, t, sum, top, lane == 0), lane, lanes);
 }
 template <typename T, int OP, bool ONE_WARP, int HELD, bool ANYWHERE>
@@ -401,30 +491,14 @@ __global__ void __maxnreg__(40) quantize_kernel(Int8Rows a) {
   one_row<T, kRowsQuantize, ONE_WARP, HELD, ANYWHERE>(a);
 }
 
-// Any row, read twice and element by element, a row a block: what is too long
-// for registers, and fp32 that does not start on 16 bytes.
+// A row a block: what is too long for registers, and fp32 that does not start
+// on 16 bytes.
 template <typename T, int OP>
 __global__ void __launch_bounds__(1024) any_rows_kernel(Int8Rows a) {
   __shared__ float2 part[32];
   pdl_wait();
   pdl_trigger();
-  const long long t = blockIdx.x;
-  const Row<T, OP> row(a, t);
-  float sum = 0.f, top = 0.f, y[8];
-  for (int c = threadIdx.x * 8; c < a.K; c += blockDim.x * 8) {
-    row.values(c, false, y, sum);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(y[e]));
-  }
-  reduce_warp(OP, sum, top);
-  reduce_block(OP, sum, top, part);
-  const Writer<OP> writer(a, t, sum, top, threadIdx.x == 0);
-  // the sum x + residual is written in the second pass: it may lie over either of them
-  for (int c = threadIdx.x * 8; c < a.K; c += blockDim.x * 8) {
-    float unused = 0.f;
-    row.values(c, true, y, unused);
-    writer.write(c, y);
-  }
+  row_in_two_passes<T, OP, false>(a, blockIdx.x, threadIdx.x, blockDim.x, part);
 }
 
 template <typename T, int OP, bool ONE_WARP, int HELD>
