@@ -35,7 +35,8 @@ void check_rows(const torch::Tensor& t, const char* what) {
   KUS_CHECK(t.is_cuda() && t.dim() == 2 && t.size(1) > 0 && (t.size(1) == 1 || t.stride(1) == 1), what,
             " must be a CUDA tensor [rows, columns] with contiguous rows of at least one column, got ", t.device(), " ",
             t.sizes(), " strides ", t.strides());
-  KUS_CHECK(t.size(0) < (1LL << 31) && t.size(1) < (1LL << 30), what, " has too many rows or columns");
+  // (a tile of 256 that ends behind the last row still counts in 32 bits)
+  KUS_CHECK(t.size(0) <= (1LL << 31) - 512 && t.size(1) < (1LL << 30), what, " has too many rows or columns");
 }
 void check_like(const torch::Tensor& t, const torch::Tensor& like, const char* what) {
   check_rows(t, what);

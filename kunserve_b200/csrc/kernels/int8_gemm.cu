@@ -753,12 +753,12 @@ Int8Plan int8_plan(int M, int N, int K, int element, const Int8Slots& slots) {
     for (int tile = step; tile <= 256; tile += tile < 32 ? 16 : 32) {
       Int8Plan p{};
       p.pair = pair;
-      p.token_tiles = (M + tile - 1) / tile;
+      p.token_tiles = (int)(((long long)M + tile - 1) / tile);
       if (p.token_tiles > 64 && tile < 256) continue;
-      p.width = ((M + p.token_tiles - 1) / p.token_tiles + step - 1) / step * step;
+      p.width = (int)(((long long)M + p.token_tiles - 1) / p.token_tiles + step - 1) / step * step;
       if (p.width == last) continue;
       last = p.width;
-      p.token_tiles = (M + p.width - 1) / p.width;
+      p.token_tiles = (int)(((long long)M + p.width - 1) / p.width);
       p.channel_tiles = (int)((int8_blocks(N) + ctas - 1) / ctas);
       const int units = p.token_tiles * p.channel_tiles;
       for (int splits = 1; splits * ctas <= 8 && splits <= blocks; ++splits) {
