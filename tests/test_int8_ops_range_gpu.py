@@ -30,7 +30,7 @@ def test_largest_rows_come_back_finite(k, dtype):
     assert ((s.double() - top[:, 0] / 127).abs() <= 2 * U * (1 + 4 * U) * top[:, 0] / 127).all()
     assert ((v.double() - x.double()).abs() <= top / 127 * (0.5 + 127 * 6 * U)).all()
     if t != F32:
-        assert torch.equal(s, top[:, 0].float() / 127)
+        assert torch.equal(s, (top[:, 0] / 127).float())
     assert dequantize_int8(q, s, t).isfinite().all()
 
 
