@@ -11,7 +11,7 @@
 //
 // Bound by HBM and, nearly as much, by instructions: 8192 rows of 5120 in
 // bf16 take 24 us to quantise (126 MB, 13 instructions an element, most of the
-// issue slots), 48 to add and norm (294 MB at 0.93 of the copy bandwidth), 39
+// issue slots), 48 to add and norm (294 MB at 0.93 of the copy bandwidth), 36
 // with SiLU (210 MB), 21 back (126 MB).  So integers come out of the adder
 // (Quotient), inputs of a quantisation stay as they are until they are
 // written, and a thread has 16 to 32 elements to share the reduction's cost.
@@ -58,18 +58,29 @@ KUS_DEVICE Pair fma(Pair a, const Pair& b, const Pair& c) {
   return a;
 }
 
-// g / (1 + e^-g) * u of two gates within kWide of zero.  e^-g = 2^n e^d: n is
-// -g log2 e rounded, whose rounding would cost e^-g |g| units in the last
-// place, and d what that left out, from an exact product and log2 e in two
-// floats.  y is off by at most 10 * 2^-24 of itself: 2^n by 4 (two units), its
-// product with 1 + d by 1, the sum by 1, the reciprocal by 2, two products by
-// 1 each.  8192 rows of 14336 take 106 us with this in bf16 and 104 in fp16;
-// 103 and 108 with e^-g of n alone, by which y is off by 1.2 |g| units more.
-constexpr float kWide = 80.f;
+// g / (1 + e^-g) * u of two gates above -kWide.  e^-g = 2^n e^d: n is -g log2 e
+// as the exponential takes it, d what that leaves out, without which y would be
+// off by 1.2 |g| units more.  Of bf16, n is exact with log2 e in 16 bits, d the
+// rest's product, within 4e-4, and 1 + d e^d to its square; of fp16, n is
+// rounded, and d has the product's rounding and log2 e's.  y is off by at most
+// 11 * 2^-24 of itself: 2^n by 4 (two units), d's square and its rounding, the
+// product with 1 + d and the sum by 1 each, the reciprocal by 2, two products
+// by 1 each.  8192 rows of 14336 take 104 us with this (bf16; 100 in fp16), 103
+// (108) with e^-g of a rounded n alone.
+constexpr float kWide = 64.f;
+template <typename T>
 KUS_DEVICE void silu_pair(float& g0, float& g1, float u0, float u1) {
-  constexpr float kLog2e = 0x1.715476p+0f, kRest = 0x1.4ae0bep-26f, kLn2 = 0x1.62e430p-1f;
-  const Pair g(g0, g1), n = g * Pair(-kLog2e);
-  const Pair d = fma(g, Pair(kRest), fma(g, Pair(kLog2e), n)) * Pair(-kLn2);
+  const Pair g(g0, g1);
+  Pair n = g, d = g;
+  if constexpr (std::is_same<T, __half>::value) {
+    constexpr float kLog2e = 0x1.715476p+0f, kRest = 0x1.4ae0bep-26f, kLn2 = 0x1.62e430p-1f;
+    n = g * Pair(-kLog2e);
+    d = fma(g, Pair(kRest), fma(g, Pair(kLog2e), n)) * Pair(-kLn2);
+  } else {
+    constexpr float kLog2e = 0x1.7154p+0f, kRestLn2 = 0x1.480fb6p-18f;
+    n = g * Pair(-kLog2e);
+    d = g * Pair(-kRestLn2);
+  }
   const float2 m = n.get();
   const Pair e(ex2(m.x), ex2(m.y));
   float2 r = (fma(e, d, e) + Pair(1.f)).get();
@@ -79,9 +90,11 @@ KUS_DEVICE void silu_pair(float& g0, float& g1, float u0, float u1) {
   g0 = y.x;
   g1 = y.y;
 }
-// Of a gate beyond kWide 1 + e^-g is 1 or e^-g to a float's last place, and
-// e^-g may leave the range where y does not: e^g is taken as a square.  Off by
-// 11 * 2^-24 of y (two exponentials by 4 each, three products).
+// Whether silu_pair does not know g: below -kWide e^-g may leave the range where
+// y does not, and n does beyond 2e38.
+KUS_DEVICE bool silu_is_wide(float g) { return g < -kWide || g > 1e38f; }
+// Its y, of one exponential as a square: off by 11 * 2^-24 of itself too (4 for
+// each, three products).
 KUS_DEVICE float silu_wide(float g, float u) {
   if (g > 0.f) return g * u;
   const float h = expf(0.5f * g);
@@ -238,15 +251,25 @@ struct Row {
       y[e] *= w[e];
     }
   }
-  // `wide` gains the gates' magnitudes; with one beyond kWide y stays undone.
+  // `least` gains the gates' least, negated; with one below -kWide y stays undone.
   // (The branch for each group also keeps a group's arithmetic ahead of later
-  // groups' loads: 106 us for 8192 x 14336, 113 without.)
-  KUS_DEVICE static void gate(float (&y)[8], const float (&o)[8], float& wide) {
+  // groups' loads: 8192 x 14336 takes 5 us less than without.)
+  KUS_DEVICE static void gate(float (&y)[8], const float (&o)[8], float& least) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) wide = fmaxf(wide, fabsf(y[e]));
-    if (wide > kWide) return;
+    for (int e = 0; e < 8; ++e) least = fmaxf(least, -y[e]);
+    if (least > kWide) return;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) silu_pair(y[e], y[e + 1], o[e], o[e + 1]);
+    for (int e = 0; e < 8; e += 2) silu_pair<T>(y[e], y[e + 1], o[e], o[e + 1]);
+  }
+  // Any gates, each by its own formula.
+  KUS_DEVICE static void gate_any(float (&y)[8], const float (&o)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float g0 = y[e], g1 = y[e + 1];
+      silu_pair<T>(y[e], y[e + 1], o[e], o[e + 1]);
+      if (silu_is_wide(g0)) y[e] = silu_wide(g0, o[e]);
+      if (silu_is_wide(g1)) y[e + 1] = silu_wide(g1, o[e + 1]);
+    }
   }
 
   // Element by element; `keep`: write x + residual.
@@ -266,15 +289,7 @@ struct Row {
       }
     }
     if (OP == kRowsNorm) combine(y, w, sum);
-    if (OP == kRowsSilu) {
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float g0 = y[e], g1 = y[e + 1];
-        silu_pair(y[e], y[e + 1], o[e], o[e + 1]);
-        if (fabsf(g0) > kWide) y[e] = silu_wide(g0, o[e]);
-        if (fabsf(g1) > kWide) y[e + 1] = silu_wide(g1, o[e + 1]);
-      }
-    }
+    if (OP == kRowsSilu) gate_any(y, o);
   }
 };
 
@@ -437,22 +452,36 @@ struct Held {
   }
 };
 
-// Any row, read twice and element by element.
-template <typename T, int OP, bool ONE_WARP>
-KUS_DEVICE void row_in_two_passes(const Int8Rows& a, long long t, int lane, int lanes, float2* part) {
-  const Row<T, OP> row(a, t);
-  float sum = 0.f, top = 0.f, y[8];
+// SiLU of a row with any gates, read twice: 8192 rows of 14336 with one gate of
+// -90 each take 246 us.  (Done where such a gate is met, it took the registers
+// of rows under way.)
+template <typename T, bool ONE_WARP, bool ANYWHERE>
+KUS_DEVICE void row_of_any_gates(const Int8Rows& a, long long t, int lane, int lanes, float2* part) {
+  const Row<T, kRowsSilu> row(a, t);
+  auto group = [&](int c, float (&y)[8]) {
+    Raw8<T> x, o;
+    float f[8];
+    Held<T, kRowsSilu, 1, ANYWHERE>::load(x, row.x, c, a.K);
+    Held<T, kRowsSilu, 1, ANYWHERE>::load(o, row.other, c, a.K);
+    x.values(y);
+    o.values(f);
+    row.gate_any(y, f);
+  };
+  float none = 0.f, top = 0.f, y[8];
+#pragma unroll 1
   for (int c = lane * 8; c < a.K; c += lanes * 8) {
-    row.values(c, false, y, sum);
+    group(c, y);
     top = max_nan(top, top_of(y));
   }
-  reduce_warp(OP, sum, top);
-  if (!ONE_WARP) reduce_block(OP, sum, top, part);
-  const Writer<OP> writer(a, t, sum, top, lane == 0);
-  // the sum x + residual is written in the second pass: it may lie over either of them
+  reduce_warp(kRowsSilu, none, top);
+  if (!ONE_WARP) {
+    __syncthreads();
+    reduce_block(kRowsSilu, none, top, part);
+  }
+  const Writer<kRowsSilu> writer(a, t, 0.f, top, lane == 0);
+#pragma unroll 1
   for (int c = lane * 8; c < a.K; c += lanes * 8) {
-    float unused = 0.f;
-    row.values(c, true, y, unused);
+    group(c, y);
     writer.write(c, y);
   }
 }
@@ -471,13 +500,9 @@ KUS_DEVICE void one_row(const Int8Rows& a) {
   held.read(Row<T, OP>(a, t), lane, lanes, sum, top);
   reduce_warp(OP, sum, top);
   if (!ONE_WARP) reduce_block(OP, sum, top, part);
-  if (OP == kRowsSilu && sum > kWide) {
-    // A gate that silu_pair does not know: the row once more, each element by its
-    // own formula.  (Here and not where it is met: that took the registers of
-    // rows under way.)
-    if (!ONE_WARP) __syncthreads();
-    return row_in_two_passes<T, OP, ONE_WARP>(a, t, lane, lanes, part);
-  }
+  // gates that silu_pair does not know, or (NaN) may not have known
+  if (OP == kRowsSilu && (sum > kWide || !(top <= INFINITY)))
+    return row_of_any_gates<T, ONE_WARP, ANYWHERE>(a, t, lane, lanes, part);
   held.write(Writer<OP>(a, t, sum, top, lane == 0), lane, lanes);
 }
 template <typename T, int OP, bool ONE_WARP, int HELD, bool ANYWHERE>
@@ -491,14 +516,29 @@ __global__ void __maxnreg__(40) quantize_kernel(Int8Rows a) {
   one_row<T, kRowsQuantize, ONE_WARP, HELD, ANYWHERE>(a);
 }
 
-// A row a block: what is too long for registers, and fp32 that does not start
-// on 16 bytes.
+// Any row, read twice and element by element, a row a block: what is too long
+// for registers, and fp32 that does not start on 16 bytes.
 template <typename T, int OP>
 __global__ void __launch_bounds__(1024) any_rows_kernel(Int8Rows a) {
   __shared__ float2 part[32];
   pdl_wait();
   pdl_trigger();
-  row_in_two_passes<T, OP, false>(a, blockIdx.x, threadIdx.x, blockDim.x, part);
+  const long long t = blockIdx.x;
+  const Row<T, OP> row(a, t);
+  float sum = 0.f, top = 0.f, y[8];
+  for (int c = threadIdx.x * 8; c < a.K; c += blockDim.x * 8) {
+    row.values(c, false, y, sum);
+    top = max_nan(top, top_of(y));
+  }
+  reduce_warp(OP, sum, top);
+  reduce_block(OP, sum, top, part);
+  const Writer<OP> writer(a, t, sum, top, threadIdx.x == 0);
+  // the sum x + residual is written in the second pass: it may lie over either of them
+  for (int c = threadIdx.x * 8; c < a.K; c += blockDim.x * 8) {
+    float unused = 0.f;
+    row.values(c, true, y, unused);
+    writer.write(c, y);
+  }
 }
 
 template <typename T, int OP, bool ONE_WARP, int HELD>
