@@ -61,12 +61,12 @@ KUS_DEVICE Pair fma(Pair a, const Pair& b, const Pair& c) {
 // g / (1 + e^-g) * u of two gates above -kWide.  e^-g = 2^n e^d: n is -g log2 e
 // as the exponential takes it, d what that leaves out, without which y would be
 // off by 1.2 |g| units more.  Of bf16, n is exact with log2 e in 16 bits, d the
-// rest's product, within 4e-4, and 1 + d e^d to its square; of fp16, n is
+// rest's product, up to 3.2e-4, and 1 + d is e^d to its square; of fp16, n is
 // rounded, and d has the product's rounding and log2 e's.  y is off by at most
-// 11 * 2^-24 of itself: 2^n by 4 (two units), d's square and its rounding, the
-// product with 1 + d and the sum by 1 each, the reciprocal by 2, two products
-// by 1 each.  8192 rows of 14336 take 104 us with this (bf16; 100 in fp16), 103
-// (108) with e^-g of a rounded n alone.
+// 11 * 2^-24 of itself: 2^n by 4 (two units), d's square, the product with 1 + d
+// and the sum by 1 each, the reciprocal by 2, two products by 1 each.  (Beyond
+// 2e38 n is an infinity and e^-g zero.)  8192 rows of 14336 take 104 us with
+// this (bf16; 100 in fp16), 103 (108) with e^-g of a rounded n alone.
 constexpr float kWide = 64.f;
 template <typename T>
 KUS_DEVICE void silu_pair(float& g0, float& g1, float u0, float u1) {
@@ -90,13 +90,10 @@ KUS_DEVICE void silu_pair(float& g0, float& g1, float u0, float u1) {
   g0 = y.x;
   g1 = y.y;
 }
-// Whether silu_pair does not know g: below -kWide e^-g may leave the range where
-// y does not, and n does beyond 2e38.
-KUS_DEVICE bool silu_is_wide(float g) { return g < -kWide || g > 1e38f; }
-// Its y, of one exponential as a square: off by 11 * 2^-24 of itself too (4 for
-// each, three products).
+// y of a gate that silu_pair does not know: below -kWide e^-g may leave the range
+// where y does not.  Of one exponential as a square: off by 11 * 2^-24 of itself
+// too (4 for each, three products).
 KUS_DEVICE float silu_wide(float g, float u) {
-  if (g > 0.f) return g * u;
   const float h = expf(0.5f * g);
   return (g * h) * (u * h);
 }
@@ -267,8 +264,8 @@ struct Row {
     for (int e = 0; e < 8; e += 2) {
       const float g0 = y[e], g1 = y[e + 1];
       silu_pair<T>(y[e], y[e + 1], o[e], o[e + 1]);
-      if (silu_is_wide(g0)) y[e] = silu_wide(g0, o[e]);
-      if (silu_is_wide(g1)) y[e + 1] = silu_wide(g1, o[e + 1]);
+      if (g0 < -kWide) y[e] = silu_wide(g0, o[e]);
+      if (g1 < -kWide) y[e + 1] = silu_wide(g1, o[e + 1]);
     }
   }
 
@@ -453,7 +450,7 @@ struct Held {
 };
 
 // SiLU of a row with any gates, read twice: 8192 rows of 14336 with one gate of
-// -90 each take 246 us.  (Done where such a gate is met, it took the registers
+// -90 each take 236 us.  (Done where such a gate is met, it took the registers
 // of rows under way.)
 template <typename T, bool ONE_WARP, bool ANYWHERE>
 KUS_DEVICE void row_of_any_gates(const Int8Rows& a, long long t, int lane, int lanes, float2* part) {
@@ -500,8 +497,7 @@ KUS_DEVICE void one_row(const Int8Rows& a) {
   held.read(Row<T, OP>(a, t), lane, lanes, sum, top);
   reduce_warp(OP, sum, top);
   if (!ONE_WARP) reduce_block(OP, sum, top, part);
-  // gates that silu_pair does not know, or (NaN) may not have known
-  if (OP == kRowsSilu && (sum > kWide || !(top <= INFINITY)))
+  if (OP == kRowsSilu && sum > kWide)      // gates that silu_pair does not know
     return row_of_any_gates<T, ONE_WARP, ANYWHERE>(a, t, lane, lanes, part);
   held.write(Writer<OP>(a, t, sum, top, lane == 0), lane, lanes);
 }
@@ -514,6 +510,13 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_kernel(Int8Rows a)
 template <typename T, bool ONE_WARP, int HELD, bool ANYWHERE>
 __global__ void __maxnreg__(40) quantize_kernel(Int8Rows a) {
   one_row<T, kRowsQuantize, ONE_WARP, HELD, ANYWHERE>(a);
+}
+// SiLU of long rows, in 56: where that is a block more on an SM than the 60 that
+// it would take (8192 x 11008 in fp16: 80 us, 93 in 60; 8192 x 14336 in bf16,
+// two blocks either way: 105 and 103).
+template <typename T, bool ANYWHERE>
+__global__ void __maxnreg__(56) silu_kernel(Int8Rows a) {
+  one_row<T, kRowsSilu, false, 4, ANYWHERE>(a);
 }
 
 // Any row, read twice and element by element, a row a block: what is too long
@@ -551,6 +554,12 @@ void launch(const Int8Rows& a, bool vec, cudaStream_t s) {
     launch_k(vec ? quantize_kernel<T, ONE_WARP, HELD, false> : quantize_kernel<T, ONE_WARP, HELD, true>, grid,
              dim3(threads), 0, s, a);
   } else {
+    if constexpr (OP == kRowsSilu && HELD == 4) {
+      // warps that an SM's registers hold, 64 and 56 a thread
+      const int warps = threads / 32;
+      if (36 / warps > 32 / warps)
+        return launch_k(vec ? silu_kernel<T, false> : silu_kernel<T, true>, grid, dim3(threads), 0, s, a);
+    }
     launch_k(vec ? rows_kernel<T, OP, ONE_WARP, HELD, false> : rows_kernel<T, OP, ONE_WARP, HELD, true>, grid,
              dim3(threads), 0, s, a);
   }
