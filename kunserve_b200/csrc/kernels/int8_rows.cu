@@ -11,7 +11,7 @@
 //
 // Bound by HBM and, nearly as much, by instructions: 8192 rows of 5120 in
 // bf16 take 24 us to quantise (126 MB, 13 instructions an element, most of the
-// issue slots), 48 to add and norm (294 MB at 0.93 of the copy bandwidth), 36
+// issue slots), 48 to add and norm (294 MB at 0.93 of the copy bandwidth), 34
 // with SiLU (210 MB), 21 back (126 MB).  So integers come out of the adder
 // (Quotient), inputs of a quantisation stay as they are until they are
 // written, and a thread has 16 to 32 elements to share the reduction's cost.
@@ -581,8 +581,8 @@ void launch_op(const Int8Rows& a, cudaStream_t s) {
     return;
   }
   // Vectors a thread: 8192 rows of 5120, us, 1 / 2 / 4: quantise - / 25.6 /
-  // 24.6, norm 52.0 / 46.6 / 46.8, silu 42.7 / 43.7 / 40.8; 2048 rows of 4096:
-  // 6.5 / 5.7 / 5.9, 12.1 / 11.5 / 12.5, 10.0 / 9.8 / 9.7.
+  // 24.6, norm 52.0 / 46.6 / 46.8, silu 41.2 / 43.3 / 33.9; 2048 rows of 4096:
+  // 6.5 / 5.7 / 5.9, 12.1 / 11.5 / 12.5, 9.5 / 9.9 / 8.9.
   if (n <= 32) return launch<T, OP, true, 1>(a, vec, s);
   if (n <= 64) return launch<T, OP, true, 2>(a, vec, s);
   if (n <= (OP == kRowsNorm ? 1024 : 256)) return launch<T, OP, false, 2>(a, vec, s);

@@ -10,10 +10,9 @@ each, weights with one scale per output channel.
 
 A row's scale is its largest magnitude / 127 (fp32; the float below where 127
 times it would leave the range) and an element's integer the nearest to 127
-times it over that magnitude, halves to even; a row of
-zeros has scale 0.  A row with a NaN or an infinity, or whose values leave
-fp32's range on the way, has scale NaN and integers 0: everything computed of
-it is NaN.
+times it over that magnitude, halves to even; a row of zeros has scale 0.  A
+row with a NaN or an infinity, or whose values leave fp32's range on the way,
+has scale NaN and integers 0: everything computed of it is NaN.
 
 All run on the current CUDA stream of their tensors' device and allocate what
 they return from it.  They serve: results carry no gradient, and arguments that
@@ -50,13 +49,15 @@ def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
     ``x`` and ``residual`` are bf16 or fp16 [T, K] with any strides between
     rows, ``weight`` [K] is of their type.  h goes to ``out``, which may be
     ``x`` or ``residual``; it is rounded to their type once, the norm is taken of
-    the sum before that.  Without a residual h is ``x`` itself."""
+    the sum before that (the serving engine's own norm is taken of the rounded
+    one).  Without a residual h is ``x`` itself."""
     return native().add_rms_norm_int8(x, weight, eps, residual, out)
 
 
 def silu_mul_int8(gate: torch.Tensor, up: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """silu(gate) * up in 8 bits, (integers, scales), of bf16 or fp16 [T, K]:
-    the halves of a merged projection's output are passed as views."""
+    the halves of a merged projection's output are passed as views.  Values are
+    within 11 * 2^-24 of themselves, at any gate, before they go to 8 bits."""
     return native().silu_mul_int8(gate, up)
 
 
