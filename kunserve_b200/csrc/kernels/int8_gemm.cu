@@ -69,12 +69,21 @@ KUS_HOST_DEVICE int side_bytes(const Int8Plan& p, int element) {
 int smem_bytes(const Int8Plan& p, int element) {
   return p.stages * stage_bytes(p) + side_bytes(p, element) + kBarriers * 8 + 16 + 1024;
 }
-// The least that a CTA asks for.  CTAs wait for TMEM without a limit, those of
-// a cluster for one another, and CTAs of other products may hold it: two
-// clusters that each had a part of what the other waits for would never end.
-// So a CTA's share of an SM's shared memory is no less than its share of the
-// TMEM, and whatever meets on an SM fits both.  (The framework's other
-// clusters with TMEM, pairs of the bf16 product, leave room for no CTA here.)
+// What a CTA asks for, so that each wait for TMEM ends: it has no limit, and two
+// clusters that each held a part of what the other waits for would never end.
+//  - A CTA's share of an SM's shared memory is no less than its share of the
+//    TMEM: whatever meets on an SM, of products of several streams too, fits.
+//  - What fits may still find the columns cut up (they are given out on multiples
+//    of their number, 256 behind 32 start at 256, and a pair's are the same on
+//    both SMs).  CTAs that wait for others of their cluster while they hold TMEM
+//    (pairs, and splits whose parts lie over the stages) therefore have their
+//    SM's to themselves, or half of it: the other half is one more such CTA's, or
+//    that of CTAs that wait for none.  Those, whole products and splits with
+//    their parts beside the stages, free theirs as soon as they are done.
+// (The framework's other clusters with TMEM, pairs of the bf16 product, leave
+// room for no CTA here.)
+constexpr int kSmemLeast = 2 * (kWBytes + 16 * kBK);                     // less than any CTA has
+constexpr int kSmemLone = kSmemSm - kSmemKept - kSmemLeast - kSmemKept;  // beside it none has room
 int least_smem(int tmem_columns) { return (tmem_columns * kSmemSm + kTmemSm - 1) / kTmemSm - kSmemKept; }
 
 // D(tmem, s32) (+)= A(smem, s8) * B(smem, s8)^T; of a pair: A rows 128 and
@@ -318,15 +327,20 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (!PAIR)
       for (int j = 0; j < early; ++j) load_w(j, start, kb0 + j);
   }
-  if (warp == 1) PAIR ? tmem_alloc_pair(tmem_holder, p.tmem_columns) : tmem_alloc(tmem_holder, p.tmem_columns);
-  tc_fence_before();
-  __syncthreads();
   // A pair's barriers are ready before the other CTA arrives on them; the
-  // other CTAs of a split only have to run before they are given their parts.
+  // other CTAs of a split only have to run before they are given their parts
+  // (and do, whatever keeps them waiting for TMEM).
+  if (PAIR && warp == 1) tmem_alloc_pair(tmem_holder, p.tmem_columns);
+  tc_fence_before();
   if (PAIR)
     cluster_sync();
   else if (SPLIT)
     cluster_arrive();
+  if (!PAIR) {
+    if (warp == 1) tmem_alloc(tmem_holder, p.tmem_columns);
+    tc_fence_before();
+    __syncthreads();
+  }
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
 
@@ -538,8 +552,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   }
   tc_fence_before();
-  cluster_sync();      // all parts are where they belong; a pair is done with both TMEMs
-  if (warp == 1) PAIR ? tmem_dealloc_pair(tmem_base, p.tmem_columns) : tmem_dealloc(tmem_base, p.tmem_columns);
+  // all parts are where they belong; a pair is done with both TMEMs, other CTAs
+  // free theirs ahead of the wait
+  if (PAIR) {
+    cluster_sync();
+    if (warp == 1) tmem_dealloc_pair(tmem_base, p.tmem_columns);
+  } else {
+    cluster_arrive();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem_base, p.tmem_columns);
+    cluster_wait();
+  }
   if (warp < 2) return;
   for (int c = warp - 2; c < shared_tokens; c += 8) {
     const float xs = c < 8 ? xs_split : a.x_scales[mine + c];
@@ -787,7 +810,9 @@ Int8Plan int8_plan(int M, int N, int K, int element, const Int8Slots& slots) {
   p.apart = p.splits > 1 && p.width <= (p.alone ? 64 : 32);
   p.stages = kMostStages;
   while (smem_bytes(p, element) > (p.alone ? kSmemAlone : kSmemHalf)) --p.stages;
-  const int asked = least_smem(p.tmem_columns);
+  const bool waits = p.pair || (p.splits > 1 && !p.apart);      // for others, while it holds TMEM
+  if (waits && !p.alone) p.tmem_columns = kTmemSm / 2;
+  const int asked = std::max(least_smem(p.tmem_columns), waits && p.alone ? kSmemLone : 0);
   // What a CTA fills once needs no more room than that, and what it asks for
   // anyway: more of the next kernel fits beside it.
   if (p.splits > 1 ? p.apart : units <= most) {

@@ -1,5 +1,6 @@
 """TMEM of the 8-bit matrix product: CTAs wait for it without a limit, and
-those of a cluster for one another, so whatever meets on an SM has to fit."""
+those of a cluster for one another.  Whatever meets on an SM has to fit, and
+what waits while it holds some must not be kept from more by others that do."""
 import itertools
 import random
 
@@ -31,6 +32,29 @@ def test_share_of_shared_memory_covers_the_share_of_tmem(slots):
     for p in _plans(slots):
         assert (p["smem"] + KEPT) * COLUMNS >= SM * p["tmem_columns"], p
         assert p["smem"] + KEPT <= (SM if p["alone"] else SM // 2)
+
+
+def _waits(p):
+    """For others of its cluster, while it holds TMEM: pairs, and splits that put their parts over the stages."""
+    return p["pair"] or (p["splits"] > 1 and not p["apart"])
+
+
+@pytest.mark.parametrize("slots", [B200, SMALL])
+def test_what_waits_has_an_sm_or_half_of_it(slots):
+    """Columns are given out on multiples of their number.  Beside a CTA that has
+    half of them, on a multiple of half, one more such CTA always finds the other
+    half once CTAs that wait for none have ended; beside one that has the SM's to
+    itself no other starts."""
+    plans = _plans(slots)
+    least = min(p["smem"] for p in plans)
+    kinds = set()
+    for p in filter(_waits, plans):
+        kinds.add((bool(p["alone"]), bool(p["pair"])))
+        if p["alone"]:
+            assert SM - (p["smem"] + KEPT) < least + KEPT
+        else:
+            assert p["tmem_columns"] == COLUMNS // 2 and p["smem"] + KEPT == SM // 2
+    assert {(True, True), (True, False)} <= kinds and least >= 2 * (128 * 128 + 16 * 128)
 
 
 def test_two_products_on_an_sm():
