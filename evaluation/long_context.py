@@ -80,7 +80,8 @@ class Decoder:
         for layer in range(self.layers):
             if self.int8:
                 x, residual = (h, None) if added is None else (added, h)
-                q, s, h = ops.add_rms_norm_int8(x, self.norm, torch.finfo(h.dtype).eps, residual=residual)
+                # (the eps that rms_norm takes below, where it is given none)
+                q, s, h = ops.add_rms_norm_int8(x, self.norm, torch.finfo(torch.float32).eps, residual=residual)
                 qkv = ops.int8_linear(q, s, self.w_qkv[layer])
             else:
                 qkv = torch.nn.functional.rms_norm(h, h.shape[-1:]) @ self.w_qkv[layer].t()
