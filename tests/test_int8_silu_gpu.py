@@ -104,3 +104,21 @@ def test_gates_without_a_value():
     gate[6, 9], up[6, 9] = 3e38, 2.0       # and this product none
     q, s = silu_mul_int8(gate, up)
     assert s.isnan().tolist() == [True] * 5 + [False, True] and (q[[0, 1, 2, 3, 4, 6]] == 0).all() and q[5, 9] == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_every_gate_there_is(dtype):
+    """A row for each finite gate of the type: its scale is y / 127 to 12 U."""
+    from kunserve_b200.ops import silu_mul_int8
+    t = TYPES[dtype]
+    gate = torch.arange(65536, device="cuda", dtype=torch.int32).to(torch.int16).view(t)
+    gate = gate[gate.isfinite()][:, None].repeat(1, 8)
+    for u in (1.0, 1.328125, 1e30 if dtype == "bf16" else 1000.0):
+        up = torch.full_like(gate, u)
+        y = _exact(gate[:, 0], up[:, 0]).abs()
+        q, s = silu_mul_int8(gate, up)
+        inside = y < 0.999 * torch.finfo(F32).max
+        assert s[inside].isfinite().all()
+        keep = inside & (y > 127 * 2.0 ** -126)
+        assert ((s.double() - y / 127).abs() <= ROUNDINGS[1] * U * y / 127)[keep].all()
+        assert (q[keep].abs() == 127).all()
